@@ -378,6 +378,118 @@ size_t smaq_kmeans_workspace_size(int n_blocks, int64_t n_points);
 int smaq_kmeans(const float* data, int n_blocks, int64_t n_points, int dim, int n_centroids, int n_iters,
                 uint64_t seed, float* centroids, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------ exact paged step
+ *
+ * No counterpart in the reference (it leaves the exact path to its host engine).  These entry
+ * points serve layers, prompts and short histories that stay exact, beside the compressed rows:
+ * block tables and slot maps from request lengths, the per-head norm and rotation of queries and
+ * keys with the cache write, and attention over the exact paged cache.
+ *
+ * Exact cache: keys and values [n_pages, page_size, n_kv_heads, head_dim] of one dtype, head_dim
+ * contiguous, page / slot / head strides in elements and equal for K and V.  Token j of request b
+ * is slot j % page_size of page block_table[b * table_stride + j / page_size]. */
+
+/* Block bookkeeping of one step.  The pool is a stack: entries [0, *free_count) of free_blocks are
+ * free pages, the last one is taken first.  In order:
+ *   - finished[b] != 0: request b's ceil(context_lens[b] / page_size) pages go onto the stack, in
+ *     request and block order; it takes no part in the rest;
+ *   - request b grows by query_lens[b] (>= 0) tokens and takes the pages it lacks, in request order.
+ *     It is admitted if its blocks fit its table row and the pages taken so far, its own included,
+ *     do not exceed the stack; one that lacks no page needs none to be left.
+ * free_blocks and block_table are updated in place (the same call on the same inputs writes the
+ * same values again); everything else is written out of place:
+ *   cu_query [batch + 1]: prefix sums of query_lens; seq_lens [batch]: context + query, 0 for a
+ *   request that is finished or not admitted; positions / slots [n_tokens]: position and cache slot
+ *   (page * page_size + offset) of every token, slot -1 where the request was not admitted, and
+ *   position 0, slot -1 for tokens past the last request's; admitted [batch]; free_count_out [1]. */
+typedef struct smaq_tables_args {
+  int32_t* free_blocks;          /* [pool_size] */
+  const int32_t* free_count;     /* [1] */
+  const int32_t* context_lens;   /* [batch] tokens already cached */
+  const int32_t* query_lens;     /* [batch] tokens of this step */
+  const uint8_t* finished;       /* nullable, [batch] */
+  int32_t* block_table;          /* [batch, table_stride], max_blocks used */
+  int64_t table_stride;
+  int64_t pool_size;
+  int64_t n_tokens;
+  int batch;                     /* <= 16384 */
+  int max_blocks;
+  int page_size;
+  int32_t* cu_query;
+  int32_t* seq_lens;
+  int32_t* positions;
+  int64_t* slots;
+  uint8_t* admitted;
+  int32_t* free_count_out;
+} smaq_tables_args;
+int smaq_step_tables(const smaq_tables_args* args, void* stream);
+
+/* Per-head RMS norm (weights nullable: no norm) and rotation of queries and keys in one pass:
+ *   y = x / sqrt(mean(x^2) + eps) * w;  pairs (a, b) of the first rotary_dim channels, (i, i +
+ *   rotary_dim / 2) or, interleaved, (2i, 2i + 1), become (a cos - b sin, b cos + a sin) with row
+ *   positions[t] of the table [n_positions, rotary_dim] = cos | sin.
+ * 32-bit arithmetic, one rounding at the end.  A position outside the table gives NaN.  With a
+ * cache, keys and values (v) are written to slots[t] (skipped where the slot is outside the cache)
+ * and k_out may be NULL; without one, v and the cache are NULL and k_out is written. */
+typedef struct smaq_norm_rope_args {
+  const void* q;
+  const void* k;
+  const void* v;                 /* nullable */
+  int64_t q_stride_t, q_stride_h, k_stride_t, k_stride_h, v_stride_t, v_stride_h;
+  const int32_t* positions;      /* [n_tokens] */
+  const float* table;            /* [n_positions, rotary_dim] */
+  const float* q_weight;         /* nullable, [head_dim] */
+  const float* k_weight;         /* nullable, [head_dim] */
+  const int64_t* slots;          /* nullable, [n_tokens] */
+  void* q_out;                   /* [n_tokens, n_q_heads, head_dim] */
+  void* k_out;                   /* nullable, [n_tokens, n_kv_heads, head_dim] */
+  void* k_cache;                 /* nullable */
+  void* v_cache;
+  int64_t c_stride_page, c_stride_slot, c_stride_h;
+  int64_t n_tokens, n_positions, n_pages;
+  int dtype, n_q_heads, n_kv_heads, head_dim, rotary_dim, interleaved, page_size;
+  float eps;
+} smaq_norm_rope_args;
+int smaq_norm_rope(const smaq_norm_rope_args* args, void* stream);
+
+/* Attention over the exact paged cache.  Row t of request b is its token i = seq_lens[b] -
+ * n_b + (t - cu_query[b]) with n_b = cu_query[b + 1] - cu_query[b]; it sees token j when
+ *   j < prefix_lens[b], or j <= i and (window == 0 or j > i - window)      (0 <= j < seq_lens[b]).
+ * Scores: x = scale q.k;  softcap > 0: x = softcap tanh(x / softcap);  slopes: x -= slopes[h] |i - j|.
+ * Query head h reads KV head h / (n_q_heads / n_kv_heads).  A row that sees nothing, and rows past
+ * the last request's, give zeros and lse -infinity.  Slots that no row sees are never used, whatever
+ * they hold.  Page numbers are clamped to the cache and seq_lens to the table's width, so that no
+ * read leaves the cache.  lse: natural log of the sum of exp(score), [rows, n_q_heads].
+ *   smaq_paged_decode: one row per request (cu_query, prefix_lens unused), the cache split over the
+ *     GPU by length and joined; needs smaq_paged_decode_workspace_size bytes of workspace.
+ *   smaq_paged_prefill: n_rows rows. */
+typedef struct smaq_paged_args {
+  const void* q;
+  int64_t q_stride_t, q_stride_h;
+  const void* k_cache;
+  const void* v_cache;
+  int64_t c_stride_page, c_stride_slot, c_stride_h;
+  const int32_t* block_table;
+  int64_t table_stride;
+  const int32_t* seq_lens;
+  const int32_t* cu_query;       /* prefill: [batch + 1] */
+  const int32_t* prefix_lens;    /* nullable */
+  const float* slopes;           /* nullable, [n_q_heads] */
+  void* out;
+  int64_t o_stride_t, o_stride_h;
+  float* lse;                    /* nullable */
+  void* workspace;
+  size_t workspace_bytes;
+  int64_t n_pages, n_rows;
+  int batch, max_blocks, page_size, n_q_heads, n_kv_heads, head_dim, dtype, window;
+  float scale, softcap;
+} smaq_paged_args;
+size_t smaq_paged_decode_workspace_size(int batch, int n_q_heads, int n_kv_heads, int head_dim);
+int smaq_paged_decode(const smaq_paged_args* args, void* stream);
+int smaq_paged_prefill(const smaq_paged_args* args, void* stream);
+/* sizeof(smaq_tables_args), smaq_norm_rope_args, smaq_paged_args for which = 0, 1, 2, else 0. */
+size_t smaq_paged_args_size(int which);
+
 #ifdef __cplusplus
 }
 #endif

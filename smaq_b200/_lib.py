@@ -29,6 +29,8 @@ EXPORTS = (
     "smaq_key_scores", "smaq_attend_workspace_size", "smaq_attend_values", "smaq_kmeans_workspace_size",
     "smaq_kmeans", "smaq_comm_set_backend", "smaq_comm_unique_id", "smaq_comm_init", "smaq_comm_allgather",
     "smaq_comm_wait", "smaq_comm_status", "smaq_comm_abort", "smaq_comm_destroy",
+    "smaq_paged_args_size", "smaq_step_tables", "smaq_norm_rope", "smaq_paged_decode_workspace_size",
+    "smaq_paged_decode", "smaq_paged_prefill",
 )
 
 vp = C.c_void_p
@@ -101,6 +103,38 @@ class AttendArgs(C.Structure):
     ]
 
 
+class TablesArgs(C.Structure):
+    _fields_ = [
+        ("free_blocks", vp), ("free_count", vp), ("context_lens", vp), ("query_lens", vp), ("finished", vp),
+        ("block_table", vp), ("table_stride", i64), ("pool_size", i64), ("n_tokens", i64), ("batch", i32),
+        ("max_blocks", i32), ("page_size", i32), ("cu_query", vp), ("seq_lens", vp), ("positions", vp),
+        ("slots", vp), ("admitted", vp), ("free_count_out", vp),
+    ]
+
+
+class NormRopeArgs(C.Structure):
+    _fields_ = [
+        ("q", vp), ("k", vp), ("v", vp), ("q_stride_t", i64), ("q_stride_h", i64), ("k_stride_t", i64),
+        ("k_stride_h", i64), ("v_stride_t", i64), ("v_stride_h", i64), ("positions", vp), ("table", vp),
+        ("q_weight", vp), ("k_weight", vp), ("slots", vp), ("q_out", vp), ("k_out", vp), ("k_cache", vp),
+        ("v_cache", vp), ("c_stride_page", i64), ("c_stride_slot", i64), ("c_stride_h", i64), ("n_tokens", i64),
+        ("n_positions", i64), ("n_pages", i64), ("dtype", i32), ("n_q_heads", i32), ("n_kv_heads", i32),
+        ("head_dim", i32), ("rotary_dim", i32), ("interleaved", i32), ("page_size", i32), ("eps", C.c_float),
+    ]
+
+
+class PagedArgs(C.Structure):
+    _fields_ = [
+        ("q", vp), ("q_stride_t", i64), ("q_stride_h", i64), ("k_cache", vp), ("v_cache", vp),
+        ("c_stride_page", i64), ("c_stride_slot", i64), ("c_stride_h", i64), ("block_table", vp),
+        ("table_stride", i64), ("seq_lens", vp), ("cu_query", vp), ("prefix_lens", vp), ("slopes", vp), ("out", vp),
+        ("o_stride_t", i64), ("o_stride_h", i64), ("lse", vp), ("workspace", vp), ("workspace_bytes", C.c_size_t),
+        ("n_pages", i64), ("n_rows", i64), ("batch", i32), ("max_blocks", i32), ("page_size", i32),
+        ("n_q_heads", i32), ("n_kv_heads", i32), ("head_dim", i32), ("dtype", i32), ("window", i32),
+        ("scale", C.c_float), ("softcap", C.c_float),
+    ]
+
+
 _lib = None
 
 
@@ -122,6 +156,22 @@ def load() -> C.CDLL:
         if lib.smaq_args_size(which) != C.sizeof(mirror):
             raise RuntimeError(f"{path}: {mirror.__name__} is {C.sizeof(mirror)} bytes here but "
                                f"{lib.smaq_args_size(which)} in the library (stale build or ABI mismatch)")
+    lib.smaq_paged_args_size.argtypes = [i32]
+    lib.smaq_paged_args_size.restype = C.c_size_t
+    for which, mirror in ((0, TablesArgs), (1, NormRopeArgs), (2, PagedArgs)):
+        if lib.smaq_paged_args_size(which) != C.sizeof(mirror):
+            raise RuntimeError(f"{path}: {mirror.__name__} is {C.sizeof(mirror)} bytes here but "
+                               f"{lib.smaq_paged_args_size(which)} in the library (stale build or ABI mismatch)")
+    lib.smaq_step_tables.argtypes = [C.POINTER(TablesArgs), vp]
+    lib.smaq_step_tables.restype = i32
+    lib.smaq_norm_rope.argtypes = [C.POINTER(NormRopeArgs), vp]
+    lib.smaq_norm_rope.restype = i32
+    lib.smaq_paged_decode_workspace_size.argtypes = [i32, i32, i32, i32]
+    lib.smaq_paged_decode_workspace_size.restype = C.c_size_t
+    lib.smaq_paged_decode.argtypes = [C.POINTER(PagedArgs), vp]
+    lib.smaq_paged_decode.restype = i32
+    lib.smaq_paged_prefill.argtypes = [C.POINTER(PagedArgs), vp]
+    lib.smaq_paged_prefill.restype = i32
     lib.smaq_last_error.restype = C.c_char_p
     lib.smaq_append.argtypes = [C.POINTER(AppendArgs), vp]
     lib.smaq_append.restype = i32

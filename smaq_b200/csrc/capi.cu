@@ -45,4 +45,10 @@ extern "C" size_t smaq_args_size(int which) {
        : which == 3 ? sizeof(smaq_attend_args)
                     : 0;
 }
+extern "C" size_t smaq_paged_args_size(int which) {
+  return which == 0 ? sizeof(smaq_tables_args)
+       : which == 1 ? sizeof(smaq_norm_rope_args)
+       : which == 2 ? sizeof(smaq_paged_args)
+                    : 0;
+}
 extern "C" const char* smaq_last_error(void) { return smaq::g_err; }

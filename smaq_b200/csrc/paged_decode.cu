@@ -1,0 +1,819 @@
+// Attention of one new token a request over the exact paged cache, split over the cache's length.
+//
+//   out = sum_j 2^(x_j - m) v_j / sum_j 2^(x_j - m),  x = log2-domain scores, m their running maximum.
+//
+// Each visible key and value is read once (2 Hkv D L elements a request), 4 G flops an element: HBM-bound,
+// so the design is about bytes in flight and an even split.
+//
+// Split.  A segment is (request, KV head, tile of up to 16 query heads); its visible tokens are cut into
+// units of 64, and the units of all segments, in order, are cut into equal runs, one a CTA (two CTAs an
+// SM), whatever the lengths.  Each CTA finds its run from seq_lens by itself.  A segment that lies in one
+// run is finished there; of the others every CTA leaves (m, sum, accumulator) in slot cta + segment, which is
+// distinct because a run's walk raises one of the two at each step, and the join kernel, launched with
+// programmatic dependence, adds them in slot order: no atomics, the same result every time.
+//
+// paged_decode_kernel (bf16 / fp16, head_dim 64 / 128 / 256): four warps, each with its own ring of
+// 16-token stages (keys + values, cp.async, 96 KB a CTA and two CTAs an SM in flight), its own softmax
+// state and no block-wide barrier until the segment ends.  The page lookups of a stage are made one stage
+// before its copies.  Scores by m16n8k16 (rows = query heads of the group, zero rows above it); weights enter
+// the second product as hi + lo parts in the cache's type, which costs tensor time that is idle here and
+// keeps 16-bit rounding out of the weights.  Slots past the visible range are filled with zeros by the copy and
+// their scores replaced, so what they hold never matters.
+//
+// paged_simt_kernel (fp32 caches, other head dims and alignments): 16 groups of eight lanes, one token a
+// group, up to four query rows a tile, FMA; scores and weights stay in 32 bits.
+#include "paged.cuh"
+
+namespace smaq {
+
+int paged_check(const smaq_paged_args* args, bool prefill, PagedParams& p) {
+  if (!args) return fail(SMAQ_ERR_INVALID, "paged attention: null arguments");
+  const smaq_paged_args& a = *args;
+  if (a.dtype != SMAQ_F32 && a.dtype != SMAQ_BF16 && a.dtype != SMAQ_F16) return fail(SMAQ_ERR_INVALID, "paged attention: dtype %d", a.dtype);
+  if (a.n_kv_heads < 1 || a.n_q_heads < 1 || a.n_q_heads % a.n_kv_heads)
+    return fail(SMAQ_ERR_INVALID, "paged attention: head counts %d/%d", a.n_q_heads, a.n_kv_heads);
+  if (a.head_dim < 1 || a.head_dim > 256) return fail(SMAQ_ERR_UNSUPPORTED, "paged attention: head_dim %d not in 1..256", a.head_dim);
+  if (a.batch < 0 || a.n_rows < 0 || a.page_size < 1 || a.max_blocks < 0 || a.window < 0 || a.n_pages < 0)
+    return fail(SMAQ_ERR_INVALID, "paged attention: bad sizes (batch %d, rows %lld, page_size %d, window %d)", a.batch, (long long)a.n_rows,
+                a.page_size, a.window);
+  if (a.n_rows >= (int64_t(1) << 31) / a.n_q_heads || int64_t(a.batch) * a.n_q_heads >= (int64_t(1) << 31))
+    return fail(SMAQ_ERR_UNSUPPORTED, "paged attention: 2^31 rows or more");
+  if (!(a.softcap >= 0.f) || !(a.scale == a.scale)) return fail(SMAQ_ERR_INVALID, "paged attention: scale or softcap");
+  if (a.table_stride < a.max_blocks) return fail(SMAQ_ERR_INVALID, "paged attention: table stride below its width");
+  if (a.n_rows > 0) {
+    if (!a.q || !a.out) return fail(SMAQ_ERR_INVALID, "paged attention: null pointer");
+    if (a.batch && (!a.seq_lens || (a.max_blocks && a.n_pages && (!a.block_table || !a.k_cache || !a.v_cache))))
+      return fail(SMAQ_ERR_INVALID, "paged attention: null pointer");
+    if (prefill && !a.cu_query) return fail(SMAQ_ERR_INVALID, "paged attention: null cu_query");
+  }
+  p.a = a;
+  if (a.n_pages == 0) p.a.max_blocks = 0;  // an empty cache: every request reads as empty
+  p.group = a.n_q_heads / a.n_kv_heads;
+  p.scale_log2 = a.scale * kLog2e;
+  p.cap_in = a.softcap > 0.f ? 2.0f * kLog2e * a.scale / a.softcap : 0.f;
+  p.cap_log2 = a.softcap * kLog2e;
+  p.page_div = make_fastdiv(a.page_size);
+  p.group_div = make_fastdiv(p.group);
+  return SMAQ_OK;
+}
+
+bool paged_aligned(const smaq_paged_args& a) {
+  const int64_t e = a.dtype == SMAQ_F32 ? 4 : 2;
+  const uintptr_t ptrs = reinterpret_cast<uintptr_t>(a.q) | reinterpret_cast<uintptr_t>(a.k_cache) | reinterpret_cast<uintptr_t>(a.v_cache) |
+                         reinterpret_cast<uintptr_t>(a.out);
+  const int64_t strides = a.q_stride_t | a.q_stride_h | a.c_stride_page | a.c_stride_slot | a.c_stride_h | a.o_stride_t | a.o_stride_h;
+  return ptrs % 16 == 0 && (strides * e) % 16 == 0;
+}
+
+namespace {
+
+constexpr int PD_UNIT = 64;    // tokens a unit
+constexpr int PD_THREADS = 128;
+
+struct DecodeParamsX {
+  PagedParams p;
+  int tiles;      // tiles of query heads a KV head
+  int rows;       // query heads a tile, at most
+  int segs;       // n_kv_heads * tiles
+  int grid;
+  float* slots;   // [grid + batch * segs][rows][head_dim + 2]
+};
+
+struct Visible {
+  int lo, hi, units;
+};
+__device__ __forceinline__ Visible visible(const PagedParams& p, int b) {
+  Visible v;
+  v.hi = paged_len(p, b);
+  v.lo = p.a.window > 0 && v.hi > p.a.window ? v.hi - p.a.window : 0;
+  v.units = (v.hi - v.lo + PD_UNIT - 1) / PD_UNIT;
+  return v;
+}
+
+// Sum over the block (PD_THREADS threads) of one int64 a thread, and the sum before this thread.
+__device__ __forceinline__ int64_t block_prefix(int64_t v, int64_t* warp_sums, int64_t& before) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  int64_t x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t u = __shfl_up_sync(~0u, x, o);
+    if (lane >= o) x += u;
+  }
+  __syncthreads();
+  if (lane == 31) warp_sums[w] = x;
+  __syncthreads();
+  int64_t total = 0, base = 0;
+#pragma unroll
+  for (int i = 0; i < PD_THREADS / 32; ++i) {
+    if (i < w) base += warp_sums[i];
+    total += warp_sums[i];
+  }
+  before = base + x - v;
+  return total;
+}
+
+struct RunStart {
+  int64_t total;       // units of all segments
+  int b;               // request the run begins in
+  int64_t into;        // units into that request
+};
+
+// Total units, and where unit `u(total)` lies.
+template <class F>
+__device__ __forceinline__ RunStart find_run(const DecodeParamsX& d, int64_t* warp_sums, int* found_b, int64_t* found_into, F unit_of_total) {
+  RunStart r;
+  const int B = d.p.a.batch;
+  r.total = 0;
+  int64_t mine = 0, before = 0;
+  for (int b0 = 0; b0 < B; b0 += PD_THREADS) {
+    const int b = b0 + threadIdx.x;
+    mine = b < B ? int64_t(visible(d.p, b).units) * d.segs : 0;
+    r.total += block_prefix(mine, warp_sums, before);
+  }
+  const int64_t u = unit_of_total(r.total);
+  if (B <= PD_THREADS) {
+    if (u >= before && u < before + mine) {
+      *found_b = threadIdx.x;
+      *found_into = u - before;
+    }
+  } else {
+    int64_t base = 0;
+    for (int b0 = 0; b0 < B && base <= u; b0 += PD_THREADS) {
+      const int b = b0 + threadIdx.x;
+      mine = b < B ? int64_t(visible(d.p, b).units) * d.segs : 0;
+      const int64_t sum = block_prefix(mine, warp_sums, before);
+      if (u >= base + before && u < base + before + mine) {
+        *found_b = b;
+        *found_into = u - base - before;
+      }
+      base += sum;
+    }
+  }
+  __syncthreads();
+  r.b = *found_b;
+  r.into = *found_into;
+  return r;
+}
+
+// Walks the units of a run in order: request, segment of it, unit of the segment.
+struct Walk {
+  int b, s, t;
+  Visible v;
+  __device__ __forceinline__ void start(const DecodeParamsX& d, int b_, int64_t into) {
+    b = b_;
+    v = visible(d.p, b);
+    s = int(into / v.units);
+    t = int(into - int64_t(s) * v.units);
+  }
+  // to the next unit; the caller knows that one exists
+  __device__ __forceinline__ void next(const DecodeParamsX& d) {
+    if (++t < v.units) return;
+    t = 0;
+    if (++s < d.segs) return;
+    s = 0;
+    do {
+      ++b;
+      v = visible(d.p, b);
+    } while (v.units == 0 && b + 1 < d.p.a.batch);
+  }
+};
+
+// Run of CTA c: units [first(c), first(c + 1)).  With fewer units than CTAs the first `total` CTAs get one
+// each, so that no CTA within a segment's range is without a slot.
+__device__ __forceinline__ int64_t run_first(int64_t c, int64_t total, int grid) {
+  return total < grid ? min(c, total) : c * total / grid;
+}
+// The CTA that has unit u.
+__device__ __forceinline__ int run_of(int64_t u, int64_t total, int grid) {
+  return total < grid ? int(u) : int(((u + 1) * grid - 1) / total);
+}
+
+// Rows of requests that see nothing.
+__device__ __forceinline__ void write_empty(const DecodeParamsX& d) {
+  const smaq_paged_args& a = d.p.a;
+  for (int b = blockIdx.x; b < a.batch; b += gridDim.x) {
+    if (visible(d.p, b).units) continue;
+    for (int i = threadIdx.x; i < a.n_q_heads * a.head_dim; i += blockDim.x)
+      store_elem(a.out, a.dtype, b * a.o_stride_t + (i / a.head_dim) * a.o_stride_h + i % a.head_dim, 0.f);
+    if (a.lse)
+      for (int h = threadIdx.x; h < a.n_q_heads; h += blockDim.x) a.lse[int64_t(b) * a.n_q_heads + h] = -INFINITY;
+  }
+}
+
+// Accumulator of one row over tokens [lo, hi) for a known maximum m, by one warp in 32 bits, into acc[0, D).
+// The hi + lo parts of a weight times an infinite value give NaN where their sum gives the infinity; a row that
+// comes out without a finite value is redone here.
+template <bool CAP>
+__device__ __noinline__ void redo_row(const PagedParams& p, int b, int h, int lo, int hi, int last, float m, float* acc) {
+  const smaq_paged_args& a = p.a;
+  const int lane = threadIdx.x & 31, D = a.head_dim;
+  const int32_t* table = a.block_table + b * a.table_stride;
+  const float slope = a.slopes ? a.slopes[h] * kLog2e : 0.f;
+  float o[8] = {};
+  for (int j = lo; j < hi; ++j) {
+    const int64_t off = token_offset(p, table, j) + (h / p.group) * a.c_stride_h;
+    float x = 0.f;
+    for (int e = lane; e < D; e += 32)
+      x = fmaf(load_elem(a.q, a.dtype, b * a.q_stride_t + h * a.q_stride_h + e), load_elem(a.k_cache, a.dtype, off + e), x);
+    const float w = ex2(score_log2<CAP>(warp_sum(x), p) - slope * float(last - j) - m);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (lane + 32 * k < D) o[k] += w * load_elem(a.v_cache, a.dtype, off + lane + 32 * k);
+  }
+#pragma unroll
+  for (int k = 0; k < 8; ++k)
+    if (lane + 32 * k < D) acc[lane + 32 * k] = o[k];
+}
+
+template <int D>
+struct Cfg {
+  static constexpr int STAGE = 16 * D * 2 * 2;                   // bytes: 16 tokens, K and V
+  static constexpr int STAGES = D == 64 ? 6 : 3;
+  static constexpr int LD = D + 2;                               // floats of a merge row: accumulator, m, sum
+  static constexpr int SMEM = 4 * STAGES * STAGE + 2 * 16 * LD * 4;
+  static constexpr int CTAS = D == 256 ? 1 : 2;                  // an SM
+};
+
+template <class DT, int D, bool CAP>
+__global__ void __launch_bounds__(PD_THREADS, Cfg<D>::CTAS) paged_decode_kernel(const __grid_constant__ DecodeParamsX d) {
+  using T = typename DT::T;
+  constexpr int STAGE = Cfg<D>::STAGE, STAGES = Cfg<D>::STAGES, LD = Cfg<D>::LD;
+  constexpr int CH = D / 8;         // 16-byte chunks a row
+  constexpr int KS = D / 16;        // contraction steps of the scores
+  constexpr int NT = D / 8;         // output column tiles
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int64_t warp_sums[PD_THREADS / 32], found_into;
+  __shared__ int found_b;
+  const PagedParams& p = d.p;
+  const smaq_paged_args& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_launch_dependents();
+  write_empty(d);
+  const RunStart run = find_run(d, warp_sums, &found_b, &found_into,
+                                [&](int64_t total) { return run_first(blockIdx.x, total, d.grid); });
+  const int64_t u0 = run_first(blockIdx.x, run.total, d.grid), u1 = run_first(int64_t(blockIdx.x) + 1, run.total, d.grid);
+  const int count = int(u1 - u0);
+  if (count <= 0) return;
+
+  uint8_t* ring = smem + warp * STAGES * STAGE;
+  float* merge = reinterpret_cast<float*>(smem + 4 * STAGES * STAGE);
+
+  // ---- copies: the walk `in` runs ahead of the computing walk by STAGES - 1 units, its lookups by one more
+  Walk in;
+  in.start(d, run.b, run.into);
+  int looked = 0, issued = 0;
+  int64_t row_off = -1;  // offset of token (lane & 15) of the unit looked up last, < 0: not visible
+  auto look_up = [&]() {
+    if (looked >= count) return;
+    if (looked) in.next(d);
+    ++looked;
+    const int j = in.v.lo + in.t * PD_UNIT + warp * 16 + (lane & 15);
+    row_off = -1;
+    if (j < in.v.hi) row_off = token_offset(p, a.block_table + in.b * a.table_stride, j) + int64_t(in.s / d.tiles) * a.c_stride_h;
+  };
+  auto issue = [&]() {
+    if (issued < count) {
+      const uint32_t st = smem_u32(ring + (issued % STAGES) * STAGE);
+#pragma unroll
+      for (int i = 0; i < 16 * CH / 32; ++i) {
+        const int r = (i * 32 + lane) / CH, ch = (i * 32 + lane) % CH;
+        const int64_t off = __shfl_sync(~0u, row_off, r);
+        const uint32_t at = st + uint32_t(r * D * 2 + ((ch ^ (r & 7)) << 4));
+        const int64_t from = (off < 0 ? 0 : off) + ch * 8;
+        const uint32_t n = off < 0 ? 0u : 16u;
+        cp_async16(at, static_cast<const T*>(a.k_cache) + from, n);
+        cp_async16(at + 16 * D * 2, static_cast<const T*>(a.v_cache) + from, n);
+      }
+      ++issued;
+    }
+    cp_async_commit();
+  };
+  look_up();
+#pragma unroll 1
+  for (int i = 0; i < STAGES - 1; ++i) {
+    issue();
+    look_up();
+  }
+
+  // ---- compute
+  Walk at;
+  at.start(d, run.b, run.into);
+  uint32_t qf[KS][4];
+  float o[NT][4];
+  float m0, m1, l0, l1;  // rows lane / 4 and lane / 4 + 8
+  float slope0 = 0.f, slope1 = 0.f;
+  bool fresh = true;
+  int from = at.t;  // first unit of the segment in this run
+#pragma unroll 1
+  for (int i = 0; i < count; ++i) {
+    if (fresh) {
+      fresh = false;
+      m0 = m1 = -INFINITY;
+      l0 = l1 = 0.f;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+      const int kvh = at.s / d.tiles, tile = at.s - kvh * d.tiles;
+      const int first = kvh * p.group + tile * 16, rows = min(16, p.group - tile * 16);
+      const int r0 = lane >> 2, r1 = r0 + 8;
+      const T* q = static_cast<const T*>(a.q) + at.b * a.q_stride_t + 2 * (lane & 3);
+      const T* q0 = q + (first + r0) * a.q_stride_h;
+      const T* q1 = q + (first + r1) * a.q_stride_h;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        qf[k][0] = r0 < rows ? __ldg(reinterpret_cast<const uint32_t*>(q0 + k * 16)) : 0u;
+        qf[k][1] = r1 < rows ? __ldg(reinterpret_cast<const uint32_t*>(q1 + k * 16)) : 0u;
+        qf[k][2] = r0 < rows ? __ldg(reinterpret_cast<const uint32_t*>(q0 + k * 16 + 8)) : 0u;
+        qf[k][3] = r1 < rows ? __ldg(reinterpret_cast<const uint32_t*>(q1 + k * 16 + 8)) : 0u;
+      }
+      if (a.slopes) {
+        slope0 = r0 < rows ? a.slopes[first + r0] * kLog2e : 0.f;
+        slope1 = r1 < rows ? a.slopes[first + r1] * kLog2e : 0.f;
+      }
+    }
+    cp_async_wait<STAGES - 2>();
+    __syncwarp();
+    issue();
+    look_up();
+
+    const int j0 = at.v.lo + at.t * PD_UNIT + warp * 16;
+    if (j0 < at.v.hi) {
+      const uint32_t ks = smem_u32(ring + (i % STAGES) * STAGE), vs = ks + 16 * D * 2;
+      float c[2][4] = {};
+      // keys: tokens 0-7 / 8-15 (matrix pairs), channels 16k .. 16k + 15
+      const int kr = (lane & 7) + ((lane >> 4) << 3), kc = (lane >> 3) & 1;
+#pragma unroll
+      for (int k = 0; k < KS; ++k) {
+        uint32_t b[4];
+        ldmatrix4(b, ks + uint32_t(kr * D * 2 + (((2 * k + kc) ^ (kr & 7)) << 4)));
+        mma_16816<DT>(c[0], qf[k], b[0], b[1]);
+        mma_16816<DT>(c[1], qf[k], b[2], b[3]);
+      }
+      float mx0 = -INFINITY, mx1 = -INFINITY;
+      const int last = at.v.hi - 1;
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int j = j0 + n * 8 + 2 * (lane & 3) + e;
+          const float gap = float(last - j);
+          float x0 = score_log2<CAP>(c[n][e], p) - slope0 * gap, x1 = score_log2<CAP>(c[n][2 + e], p) - slope1 * gap;
+          c[n][e] = x0 = j <= last ? x0 : -INFINITY;
+          c[n][2 + e] = x1 = j <= last ? x1 : -INFINITY;
+          mx0 = fmaxf(mx0, x0);
+          mx1 = fmaxf(mx1, x1);
+        }
+#pragma unroll
+      for (int w = 1; w < 4; w <<= 1) {
+        mx0 = fmaxf(mx0, __shfl_xor_sync(~0u, mx0, w));
+        mx1 = fmaxf(mx1, __shfl_xor_sync(~0u, mx1, w));
+      }
+      if (__any_sync(~0u, mx0 > m0 || mx1 > m1)) {
+        const float n0 = fmaxf(m0, mx0), n1 = fmaxf(m1, mx1);
+        const float f0 = m0 == -INFINITY ? 0.f : ex2(m0 - n0), f1 = m1 == -INFINITY ? 0.f : ex2(m1 - n1);
+        m0 = n0;
+        m1 = n1;
+        l0 *= f0;
+        l1 *= f1;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          o[n][0] *= f0;
+          o[n][1] *= f0;
+          o[n][2] *= f1;
+          o[n][3] *= f1;
+        }
+      }
+      const float b0 = m0 == -INFINITY ? 0.f : m0, b1 = m1 == -INFINITY ? 0.f : m1;
+      uint32_t hi[4], lo[4];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const float p00 = ex2(c[n][0] - b0), p01 = ex2(c[n][1] - b0), p10 = ex2(c[n][2] - b1), p11 = ex2(c[n][3] - b1);
+        l0 += p00 + p01;
+        l1 += p10 + p11;
+        hi[2 * n] = pack2<DT>(p00, p01);
+        hi[2 * n + 1] = pack2<DT>(p10, p11);
+        const float2 h0 = unpack2<DT>(hi[2 * n]), h1 = unpack2<DT>(hi[2 * n + 1]);
+        lo[2 * n] = pack2<DT>(p00 - h0.x, p01 - h0.y);
+        lo[2 * n + 1] = pack2<DT>(p10 - h1.x, p11 - h1.y);
+      }
+      // values: tokens 0-7 / 8-15, channels 16n .. 16n + 15, transposed
+      const int vr = (lane & 7) + (((lane >> 3) & 1) << 3), vc = lane >> 4;
+#pragma unroll
+      for (int n = 0; n < NT / 2; ++n) {
+        uint32_t b[4];
+        ldmatrix4_trans(b, vs + uint32_t(vr * D * 2 + (((2 * n + vc) ^ (vr & 7)) << 4)));
+        mma_16816<DT>(o[2 * n], hi, b[0], b[1]);
+        mma_16816<DT>(o[2 * n + 1], hi, b[2], b[3]);
+        mma_16816<DT>(o[2 * n], lo, b[0], b[1]);
+        mma_16816<DT>(o[2 * n + 1], lo, b[2], b[3]);
+      }
+    }
+
+    const bool ends = at.t + 1 == at.v.units;
+    if (ends || i + 1 == count) {
+      // ---- the four warps' states into one: 2, 3 -> 0, 1; 1 -> 0
+      l0 += __shfl_xor_sync(~0u, l0, 1);
+      l1 += __shfl_xor_sync(~0u, l1, 1);
+      l0 += __shfl_xor_sync(~0u, l0, 2);
+      l1 += __shfl_xor_sync(~0u, l1, 2);
+      const int r0 = lane >> 2, r1 = r0 + 8, col = 2 * (lane & 3);
+      auto put = [&](float* dst) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          *reinterpret_cast<float2*>(dst + r0 * LD + n * 8 + col) = make_float2(o[n][0], o[n][1]);
+          *reinterpret_cast<float2*>(dst + r1 * LD + n * 8 + col) = make_float2(o[n][2], o[n][3]);
+        }
+        if ((lane & 3) == 0) {
+          *reinterpret_cast<float2*>(dst + r0 * LD + D) = make_float2(m0, l0);
+          *reinterpret_cast<float2*>(dst + r1 * LD + D) = make_float2(m1, l1);
+        }
+      };
+      auto add = [&](const float* src) {
+        const float2 s0 = *reinterpret_cast<const float2*>(src + r0 * LD + D), s1 = *reinterpret_cast<const float2*>(src + r1 * LD + D);
+        const float n0 = fmaxf(m0, s0.x), n1 = fmaxf(m1, s1.x);
+        const float z0 = n0 == -INFINITY ? 0.f : n0, z1 = n1 == -INFINITY ? 0.f : n1;
+        const float f0 = ex2(m0 - z0), f1 = ex2(m1 - z1), g0 = ex2(s0.x - z0), g1 = ex2(s1.x - z1);
+        m0 = n0;
+        m1 = n1;
+        l0 = l0 * f0 + s0.y * g0;
+        l1 = l1 * f1 + s1.y * g1;
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const float2 x0 = *reinterpret_cast<const float2*>(src + r0 * LD + n * 8 + col);
+          const float2 x1 = *reinterpret_cast<const float2*>(src + r1 * LD + n * 8 + col);
+          o[n][0] = o[n][0] * f0 + x0.x * g0;
+          o[n][1] = o[n][1] * f0 + x0.y * g0;
+          o[n][2] = o[n][2] * f1 + x1.x * g1;
+          o[n][3] = o[n][3] * f1 + x1.y * g1;
+        }
+      };
+      __syncthreads();  // the merge rows of the segment before are read
+      if (warp >= 2) put(merge + (warp - 2) * 16 * LD);
+      __syncthreads();
+      if (warp < 2) add(merge + warp * 16 * LD);
+      if (warp == 1) {
+        __syncwarp();  // all lanes have read the rows that the next lines overwrite
+        put(merge + 16 * LD);
+      }
+      __syncthreads();
+      if (warp == 0) {
+        add(merge + 16 * LD);
+        const int kvh = at.s / d.tiles, tile = at.s - kvh * d.tiles;
+        const int first = kvh * p.group + tile * 16, rows = min(16, p.group - tile * 16);
+        float odd0 = 0.f, odd1 = 0.f;  // NaN where the accumulator is not finite and the weights are
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          odd0 += (o[n][0] + o[n][1]) * 0.f;
+          odd1 += (o[n][2] + o[n][3]) * 0.f;
+        }
+        const uint32_t redo0 = __ballot_sync(~0u, odd0 != 0.f && l0 * 0.f == 0.f), redo1 = __ballot_sync(~0u, odd1 != 0.f && l1 * 0.f == 0.f);
+        if (redo0 | redo1) {
+          for (int r = 0; r < rows; ++r) {
+            if (!((r < 8 ? redo0 : redo1) >> (4 * (r & 7)) & 15u)) continue;
+            const float m = __shfl_sync(~0u, r < 8 ? m0 : m1, 4 * (r & 7));
+            redo_row<CAP>(p, at.b, first + r, at.v.lo + from * PD_UNIT, min(at.v.hi, at.v.lo + (at.t + 1) * PD_UNIT), at.v.hi - 1, m, merge);
+            __syncwarp();
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              const float2 x = *reinterpret_cast<const float2*>(merge + n * 8 + col);
+              if (r == r0) {
+                o[n][0] = x.x;
+                o[n][1] = x.y;
+              } else if (r == r1) {
+                o[n][2] = x.x;
+                o[n][3] = x.y;
+              }
+            }
+            __syncwarp();
+          }
+        }
+        if (ends && from == 0) {
+          const float i0 = l0 > 0.f ? 1.0f / l0 : (l0 == 0.f ? 0.f : l0), i1 = l1 > 0.f ? 1.0f / l1 : (l1 == 0.f ? 0.f : l1);
+          T* out = static_cast<T*>(a.out) + at.b * a.o_stride_t + col;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            if (r0 < rows) *reinterpret_cast<uint32_t*>(out + (first + r0) * a.o_stride_h + n * 8) = pack2<DT>(o[n][0] * i0, o[n][1] * i0);
+            if (r1 < rows) *reinterpret_cast<uint32_t*>(out + (first + r1) * a.o_stride_h + n * 8) = pack2<DT>(o[n][2] * i1, o[n][3] * i1);
+          }
+          if (a.lse && (lane & 3) == 0) {
+            float* lse = a.lse + int64_t(at.b) * a.n_q_heads + first;
+            if (r0 < rows) lse[r0] = (m0 + log2f(l0)) * kLn2;
+            if (r1 < rows) lse[r1] = (m1 + log2f(l1)) * kLn2;
+          }
+        } else {
+          float* slot = d.slots + (int64_t(blockIdx.x) + int64_t(at.b) * d.segs + at.s) * d.rows * LD;
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            if (r0 < rows) *reinterpret_cast<float2*>(slot + r0 * LD + n * 8 + col) = make_float2(o[n][0], o[n][1]);
+            if (r1 < rows) *reinterpret_cast<float2*>(slot + r1 * LD + n * 8 + col) = make_float2(o[n][2], o[n][3]);
+          }
+          if ((lane & 3) == 0) {
+            if (r0 < rows) *reinterpret_cast<float2*>(slot + r0 * LD + D) = make_float2(m0, l0);
+            if (r1 < rows) *reinterpret_cast<float2*>(slot + r1 * LD + D) = make_float2(m1, l1);
+          }
+        }
+      }
+      fresh = true;
+      from = 0;
+    }
+    if (i + 1 < count) at.next(d);
+  }
+}
+
+// ---------------------------------------------------------------- other types, head dims and alignments
+constexpr int PS_ROWS = 4;  // query heads a tile
+
+// NI vectors of four elements a lane, element 4 * (l + 8 * i); VEC: whole aligned vectors.
+template <class DT, int NI, bool VEC>
+__device__ __forceinline__ void load_row(const typename DT::T* row, int l, int D, float (&x)[NI][4]) {
+#pragma unroll
+  for (int i = 0; i < NI; ++i) {
+    const int e = 4 * (l + 8 * i);
+    if constexpr (VEC) {
+      if (e < D) load_vec<DT, 4>(row + e, x[i]);
+      else x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.f;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x[i][k] = e + k < D ? to_f(row[e + k]) : 0.f;
+    }
+  }
+}
+
+template <class DT, int NI, bool VEC>
+__global__ void __launch_bounds__(PD_THREADS) paged_simt_kernel(const __grid_constant__ DecodeParamsX d) {
+  using T = typename DT::T;
+  constexpr int GROUPS = PD_THREADS / 8;
+  __shared__ int64_t warp_sums[PD_THREADS / 32], found_into;
+  __shared__ int found_b;
+  __shared__ __align__(16) float qs[PS_ROWS][32 * NI];
+  __shared__ float acc[PD_THREADS / 32][PS_ROWS][32 * NI + 2];
+  const PagedParams& p = d.p;
+  const smaq_paged_args& a = p.a;
+  const int D = a.head_dim, LD = D + 2, l = threadIdx.x & 7, grp = threadIdx.x >> 3, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  pdl_launch_dependents();
+  write_empty(d);
+  const RunStart run = find_run(d, warp_sums, &found_b, &found_into,
+                                [&](int64_t total) { return run_first(blockIdx.x, total, d.grid); });
+  const int64_t u0 = run_first(blockIdx.x, run.total, d.grid), u1 = run_first(int64_t(blockIdx.x) + 1, run.total, d.grid);
+  int left = int(u1 - u0);
+  if (left <= 0) return;
+  Walk at;
+  at.start(d, run.b, run.into);
+  while (left > 0) {
+    const int n = min(left, at.v.units - at.t);  // units of this segment in the run
+    const int kvh = at.s / d.tiles, tile = at.s - kvh * d.tiles;
+    const int first = kvh * p.group + tile * PS_ROWS, rows = min(PS_ROWS, p.group - tile * PS_ROWS);
+    __syncthreads();
+    for (int i = threadIdx.x; i < PS_ROWS * 32 * NI; i += PD_THREADS) {
+      const int r = i / (32 * NI), e = i % (32 * NI);
+      qs[r][e] = r < rows && e < D ? load_elem(a.q, a.dtype, at.b * a.q_stride_t + (first + r) * a.q_stride_h + e) : 0.f;
+    }
+    __syncthreads();
+    float o[PS_ROWS][NI][4] = {}, m[PS_ROWS], s[PS_ROWS], slope[PS_ROWS];
+#pragma unroll
+    for (int r = 0; r < PS_ROWS; ++r) {
+      m[r] = -INFINITY;
+      s[r] = 0.f;
+      slope[r] = a.slopes && r < rows ? a.slopes[first + r] : 0.f;
+    }
+    const int lo = at.v.lo + at.t * PD_UNIT, hi = min(at.v.hi, lo + n * PD_UNIT), last = at.v.hi - 1;
+    const int32_t* table = a.block_table + at.b * a.table_stride;
+    const T* kc = static_cast<const T*>(a.k_cache) + kvh * a.c_stride_h;
+    const T* vc = static_cast<const T*>(a.v_cache) + kvh * a.c_stride_h;
+    for (int j0 = lo; j0 < hi; j0 += GROUPS) {  // the same number of steps for every group: whole warps shuffle
+      const int j = j0 + grp;
+      const bool seen = j < hi;
+      float k[NI][4], v[NI][4];
+      if (seen) {
+        const int64_t off = token_offset(p, table, j);
+        load_row<DT, NI, VEC>(kc + off, l, D, k);
+        load_row<DT, NI, VEC>(vc + off, l, D, v);
+      } else {
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) k[i][e] = v[i][e] = 0.f;
+      }
+#pragma unroll
+      for (int r = 0; r < PS_ROWS; ++r) {
+        float x = 0.f;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+          const float4 q = *reinterpret_cast<const float4*>(&qs[r][4 * (l + 8 * i)]);
+          x = fmaf(q.x, k[i][0], fmaf(q.y, k[i][1], fmaf(q.z, k[i][2], fmaf(q.w, k[i][3], x))));
+        }
+#pragma unroll
+        for (int w = 1; w < 8; w <<= 1) x += __shfl_xor_sync(~0u, x, w);
+        x *= a.scale;
+        if (a.softcap > 0.f) x = a.softcap * tanhf(x / a.softcap);
+        x = (x - slope[r] * float(last - j)) * kLog2e;
+        if (!seen) continue;
+        if (x > m[r]) {
+          const float f = ex2(m[r] - x);  // m = -infinity: 0
+          m[r] = x;
+          s[r] *= f;
+#pragma unroll
+          for (int i = 0; i < NI; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[r][i][e] *= f;
+        }
+        const float w = ex2(x - (m[r] == -INFINITY ? 0.f : m[r]));
+        s[r] += w;
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[r][i][e] = fmaf(w, v[i][e], o[r][i][e]);
+      }
+    }
+    // join the groups of a warp by exchange, the warps in shared memory
+#pragma unroll
+    for (int r = 0; r < PS_ROWS; ++r) {
+#pragma unroll
+      for (int w = 8; w < 32; w <<= 1) {
+        const float om = __shfl_xor_sync(~0u, m[r], w), os = __shfl_xor_sync(~0u, s[r], w);
+        const float nm = fmaxf(m[r], om), z = nm == -INFINITY ? 0.f : nm, f = ex2(m[r] - z), g = ex2(om - z);
+        m[r] = nm;
+        s[r] = s[r] * f + os * g;
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[r][i][e] = o[r][i][e] * f + __shfl_xor_sync(~0u, o[r][i][e], w) * g;
+      }
+      if (lane < 8) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[warp][r][4 * (l + 8 * i) + e] = o[r][i][e];
+        if (l == 0) {
+          acc[warp][r][32 * NI] = m[r];
+          acc[warp][r][32 * NI + 1] = s[r];
+        }
+      }
+    }
+    __syncthreads();
+    const bool all = at.t == 0 && n == at.v.units;
+    float* slot = d.slots + (int64_t(blockIdx.x) + int64_t(at.b) * d.segs + at.s) * d.rows * LD;
+    for (int i = threadIdx.x; i < rows * D; i += PD_THREADS) {
+      const int r = i / D, e = i - r * D;
+      float mm = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < PD_THREADS / 32; ++w) mm = fmaxf(mm, acc[w][r][32 * NI]);
+      const float z = mm == -INFINITY ? 0.f : mm;
+      float x = 0.f, sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < PD_THREADS / 32; ++w) {
+        const float f = ex2(acc[w][r][32 * NI] - z);
+        x += f * acc[w][r][e];
+        sum += f * acc[w][r][32 * NI + 1];
+      }
+      if (all) {
+        store_elem(a.out, a.dtype, at.b * a.o_stride_t + (first + r) * a.o_stride_h + e, sum == 0.f ? 0.f : x / sum);
+        if (a.lse && e == 0) a.lse[int64_t(at.b) * a.n_q_heads + first + r] = (mm + log2f(sum)) * kLn2;
+      } else {
+        slot[r * LD + e] = x;
+        if (e == 0) {
+          slot[r * LD + D] = mm;
+          slot[r * LD + D + 1] = sum;
+        }
+      }
+    }
+    left -= n;
+    if (left > 0) {
+      at.t += n - 1;
+      at.next(d);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- join
+// One CTA a (request, query head): the slots of its segment in CTA order.
+__global__ void __launch_bounds__(PD_THREADS) paged_join_kernel(const __grid_constant__ DecodeParamsX d, int tile_rows) {
+  __shared__ int64_t warp_sums[PD_THREADS / 32];
+  __shared__ int64_t my_first;
+  const PagedParams& p = d.p;
+  const smaq_paged_args& a = p.a;
+  const int b = blockIdx.x / a.n_q_heads, h = blockIdx.x - b * a.n_q_heads, D = a.head_dim, LD = D + 2;
+  const int kvh = h / p.group, tile = (h - kvh * p.group) / tile_rows, r = h - kvh * p.group - tile * tile_rows;
+  const int s = kvh * d.tiles + tile;
+  int64_t total = 0;
+  for (int b0 = 0; b0 < a.batch; b0 += PD_THREADS) {
+    const int i = b0 + threadIdx.x;
+    int64_t before;
+    const int64_t mine = i < a.batch ? int64_t(visible(p, i).units) * d.segs : 0;
+    const int64_t sum = block_prefix(mine, warp_sums, before);
+    if (i == b) my_first = total + before;
+    total += sum;
+  }
+  __syncthreads();
+  const int units = visible(p, b).units;
+  pdl_wait();  // the slots are complete from here on; every CTA waits, so this grid ends after the other
+  if (units == 0) return;
+  const int64_t f = my_first + int64_t(s) * units, e = f + units - 1;
+  const int c0 = run_of(f, total, d.grid), c1 = run_of(e, total, d.grid);
+  if (c0 == c1) return;
+  const int64_t step = int64_t(d.rows) * LD;
+  const float* slot = d.slots + (int64_t(c0) + int64_t(b) * d.segs + s) * step + r * LD;
+  const int n = c1 - c0 + 1;
+  float m = -INFINITY;
+  for (int i = 0; i < n; ++i) m = fmaxf(m, slot[i * step + D]);
+  const float z = m == -INFINITY ? 0.f : m;
+  float sum = 0.f;
+  for (int i = 0; i < n; ++i) sum += ex2(slot[i * step + D] - z) * slot[i * step + D + 1];
+  const float inv = sum == 0.f ? 0.f : 1.0f / sum;
+  for (int c = threadIdx.x; c < D; c += PD_THREADS) {
+    float x = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) x += ex2(slot[i * step + D] - z) * slot[i * step + c];
+    store_elem(a.out, a.dtype, b * a.o_stride_t + h * a.o_stride_h + c, x * inv);
+  }
+  if (a.lse && threadIdx.x == 0) a.lse[int64_t(b) * a.n_q_heads + h] = (m + log2f(sum)) * kLn2;
+}
+
+bool mma_eligible(const smaq_paged_args& a) {
+  return a.dtype != SMAQ_F32 && (a.head_dim == 64 || a.head_dim == 128 || a.head_dim == 256) && paged_aligned(a);
+}
+
+constexpr int PS_CTAS = 4;  // CTAs an SM of the SIMT kernel
+int tile_rows_of(bool mma) { return mma ? 16 : PS_ROWS; }
+
+template <class DT, int D>
+int launch_mma(const DecodeParamsX& d, cudaStream_t st) {
+  auto kern = d.p.a.softcap > 0.f ? paged_decode_kernel<DT, D, true> : paged_decode_kernel<DT, D, false>;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM);
+  if (e != cudaSuccess) return cuda_status(e, "paged_decode attr");
+  kern<<<d.grid, PD_THREADS, Cfg<D>::SMEM, st>>>(d);
+  return cuda_status(cudaGetLastError(), "paged_decode");
+}
+template <class DT>
+int launch_mma_dim(const DecodeParamsX& d, cudaStream_t st) {
+  switch (d.p.a.head_dim) {
+    case 64: return launch_mma<DT, 64>(d, st);
+    case 128: return launch_mma<DT, 128>(d, st);
+    default: return launch_mma<DT, 256>(d, st);
+  }
+}
+template <class DT>
+int launch_simt(const DecodeParamsX& d, cudaStream_t st) {
+  const int D = d.p.a.head_dim;
+  const bool vec = D % 4 == 0 && paged_aligned(d.p.a);
+  auto go = [&](auto kern) {
+    kern<<<d.grid, PD_THREADS, 0, st>>>(d);
+    return cuda_status(cudaGetLastError(), "paged_decode");
+  };
+  if (D <= 64) return vec ? go(paged_simt_kernel<DT, 2, true>) : go(paged_simt_kernel<DT, 2, false>);
+  if (D <= 128) return vec ? go(paged_simt_kernel<DT, 4, true>) : go(paged_simt_kernel<DT, 4, false>);
+  return vec ? go(paged_simt_kernel<DT, 8, true>) : go(paged_simt_kernel<DT, 8, false>);
+}
+
+}  // namespace
+
+}  // namespace smaq
+
+extern "C" size_t smaq_paged_decode_workspace_size(int batch, int n_q_heads, int n_kv_heads, int head_dim) {
+  using namespace smaq;
+  if (batch <= 0 || n_kv_heads <= 0 || n_q_heads < n_kv_heads || head_dim <= 0) return 0;
+  // enough for either kernel: the one with fewer rows a tile has as many rows in all
+  const int group = n_q_heads / n_kv_heads;
+  size_t most = 0;
+  for (const bool mma : {false, true}) {
+    const int tr = tile_rows_of(mma), tiles = (group + tr - 1) / tr, rows = group < tr ? group : tr;
+    const int ctas = num_sms() * (mma ? (head_dim == 256 ? 1 : 2) : PS_CTAS);
+    const size_t n = (size_t(ctas) + size_t(batch) * n_kv_heads * tiles) * rows * (head_dim + 2) * sizeof(float);
+    most = n > most ? n : most;
+  }
+  return most;
+}
+
+extern "C" int smaq_paged_decode(const smaq_paged_args* args, void* stream) {
+  using namespace smaq;
+  DecodeParamsX d;
+  if (const int st = paged_check(args, false, d.p)) return st;
+  const smaq_paged_args& a = d.p.a;
+  if (a.n_rows != a.batch) return fail(SMAQ_ERR_INVALID, "paged_decode: %lld rows for batch %d (one row a request)", (long long)a.n_rows, a.batch);
+  if (a.batch == 0) return SMAQ_OK;
+  const size_t need = smaq_paged_decode_workspace_size(a.batch, a.n_q_heads, a.n_kv_heads, a.head_dim);
+  if (!a.workspace || a.workspace_bytes < need)
+    return fail(SMAQ_ERR_WORKSPACE, "paged_decode: workspace %zu bytes, needs %zu", a.workspace ? a.workspace_bytes : size_t(0), need);
+  if (reinterpret_cast<uintptr_t>(a.workspace) % 16) return fail(SMAQ_ERR_INVALID, "paged_decode: workspace must be 16-byte aligned");
+  const bool mma = mma_eligible(a);
+  const int tr = tile_rows_of(mma);
+  d.tiles = (d.p.group + tr - 1) / tr;
+  d.rows = d.p.group < tr ? d.p.group : tr;
+  d.segs = a.n_kv_heads * d.tiles;
+  d.grid = num_sms() * (mma ? (a.head_dim == 256 ? 1 : 2) : PS_CTAS);
+  d.slots = static_cast<float*>(a.workspace);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  int rc;
+  if (mma) rc = a.dtype == SMAQ_BF16 ? launch_mma_dim<BF16>(d, st) : launch_mma_dim<F16>(d, st);
+  else rc = a.dtype == SMAQ_F32 ? launch_simt<F32>(d, st) : a.dtype == SMAQ_BF16 ? launch_simt<BF16>(d, st) : launch_simt<F16>(d, st);
+  if (rc) return rc;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(a.batch) * unsigned(a.n_q_heads));
+  cfg.blockDim = dim3(PD_THREADS);
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cuda_status(cudaLaunchKernelEx(&cfg, paged_join_kernel, d, tr), "paged_decode join");
+}

@@ -1,0 +1,392 @@
+// Attention of prompt chunks over the exact paged cache: causal behind any cached context, with a window,
+// a prefix that all rows see, capped scores and a distance bias.
+//
+// A CTA takes one tile of rows of one request and KV head (rows = tokens times the query heads of the group, so
+// grouped heads share every key and value that is brought on chip) and walks the tokens that some row of it
+// sees, with a running maximum and sum per row.  The tiles of all requests are numbered from cu_query on the
+// GPU; the host knows only the number of rows.  Tiles with the longest walks start first.
+//
+// prefill_mma_kernel (bf16 / fp16, head_dim 64 / 128 / 256): four warps of 16 rows, m16n8k16 products, blocks of
+//   64 (head_dim 256: 32) tokens brought by cp.async into two stages, page lookups two blocks ahead.
+// prefill_simt_kernel (fp32, other head dims and alignments): tiles of four rows, 16 lane groups with a token
+//   each; all arithmetic in 32 bits.
+#include "paged_prefill.cuh"
+
+namespace smaq {
+
+namespace {
+
+constexpr int PM_THREADS = 128;
+
+template <int D>
+struct PmCfg {
+  static constexpr int ROWS = 64;
+  static constexpr int N = D == 256 ? 32 : 64;       // tokens a block
+  static constexpr int Q = ROWS * D * 2;
+  static constexpr int STAGE = 2 * N * D * 2;
+  static constexpr int SMEM = Q + 2 * STAGE;
+};
+
+template <class DT, int D, bool CAP>
+__global__ void __launch_bounds__(PM_THREADS, 2) prefill_mma_kernel(const __grid_constant__ PagedParams p) {
+  using T = typename DT::T;
+  constexpr int N = PmCfg<D>::N, STAGE = PmCfg<D>::STAGE, CH = D / 8, NT = D / 8;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int64_t offs[2][N];
+  __shared__ int sums[PM_THREADS / 32], found[2];
+  const smaq_paged_args& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kvh = blockIdx.y;
+  write_padding(p, kvh, blockIdx.x, gridDim.x);
+  const PrefillTile t = find_tile<PM_THREADS>(p, blockIdx.x, PmCfg<D>::ROWS, true, sums, found);
+  if (t.rows == 0) return;
+  const PrefillBlocks blocks(t, N);
+  const uint32_t qs = smem_u32(smem), ring = qs + PmCfg<D>::Q;
+  const int32_t* table = a.block_table + t.b * a.table_stride;
+
+  for (int i = threadIdx.x; i < PmCfg<D>::ROWS * CH; i += PM_THREADS) {
+    const int r = i / CH, ch = i % CH, f = t.f0 + r, tok = fast_div(f, p.group_div);
+    const bool live = r < t.rows;
+    const T* src = static_cast<const T*>(a.q) + (live ? (t.first + tok) * a.q_stride_t + (kvh * p.group + f - tok * p.group) * a.q_stride_h + ch * 8 : 0);
+    cp_async16(qs + uint32_t(r * D * 2 + ((ch ^ (r & 7)) << 4)), src, live ? 16u : 0u);
+  }
+  auto look_up = [&](int k) {
+    if (k >= blocks.count || threadIdx.x >= N) return;
+    const int j = blocks.base(k, N) + threadIdx.x;
+    offs[k & 1][threadIdx.x] = tile_sees(t, j) ? token_offset(p, table, j) + kvh * a.c_stride_h : -1;
+  };
+  auto issue = [&](int k) {
+    if (k < blocks.count) {
+      const uint32_t st = ring + (k & 1) * STAGE;
+#pragma unroll
+      for (int i = 0; i < N * CH / PM_THREADS; ++i) {
+        const int r = (i * PM_THREADS + threadIdx.x) / CH, ch = (i * PM_THREADS + threadIdx.x) % CH;
+        const int64_t off = offs[k & 1][r], from = (off < 0 ? 0 : off) + ch * 8;
+        const uint32_t at = st + uint32_t(r * D * 2 + ((ch ^ (r & 7)) << 4)), n = off < 0 ? 0u : 16u;
+        cp_async16(at, static_cast<const T*>(a.k_cache) + from, n);
+        cp_async16(at + N * D * 2, static_cast<const T*>(a.v_cache) + from, n);
+      }
+    }
+    cp_async_commit();
+  };
+
+  // this thread's two rows
+  const int f0 = t.f0 + warp * 16 + (lane >> 2), f1 = f0 + 8;
+  const int t0 = fast_div(f0, p.group_div), t1 = fast_div(f1, p.group_div);
+  const int i0 = t.past + t0, i1 = t.past + t1;
+  const int h0 = kvh * p.group + f0 - t0 * p.group, h1 = kvh * p.group + f1 - t1 * p.group;
+  const int last = t.f0 + t.rows;
+  const float s0 = a.slopes && f0 < last ? a.slopes[h0] * kLog2e : 0.f, s1 = a.slopes && f1 < last ? a.slopes[h1] * kLog2e : 0.f;
+  const int least = t.past + fast_div(t.f0, p.group_div), most = t.past + fast_div(last - 1, p.group_div);
+  float o[NT][4] = {}, m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+  bool special = false;  // an infinite or NaN value in a block that is not seen by all rows
+
+  look_up(0);
+  __syncthreads();
+  issue(0);
+  look_up(1);
+#pragma unroll 1
+  for (int k = 0; k < blocks.count; ++k) {
+    __syncthreads();  // the lookups of block k + 1 are there, its stage is free
+    issue(k + 1);
+    look_up(k + 2);
+    cp_async_wait<1>();
+    __syncthreads();
+    const uint32_t ks = ring + (k & 1) * STAGE, vs = ks + N * D * 2;
+    const int base = blocks.base(k, N);
+    float c[N / 8][4] = {};
+    const int qr = warp * 16 + (lane & 15), qc = lane >> 4;
+    const int kr = (lane & 7) + ((lane >> 4) << 3), kc = (lane >> 3) & 1;
+#pragma unroll
+    for (int s = 0; s < D / 16; ++s) {
+      uint32_t q[4];
+      ldmatrix4(q, qs + uint32_t(qr * D * 2 + (((2 * s + qc) ^ (qr & 7)) << 4)));
+#pragma unroll
+      for (int n = 0; n < N / 16; ++n) {
+        uint32_t b[4];
+        ldmatrix4(b, ks + uint32_t((n * 16 + kr) * D * 2 + (((2 * s + kc) ^ (kr & 7)) << 4)));
+        mma_16816<DT>(c[2 * n], q, b[0], b[1]);
+        mma_16816<DT>(c[2 * n + 1], q, b[2], b[3]);
+      }
+    }
+    const bool all = base + N <= t.prefix || (base + N <= least + 1 && (a.window == 0 || base > most - a.window));
+    if (!all) {
+      for (int i = threadIdx.x; i < N * CH; i += PM_THREADS) special |= any_special<DT>(*reinterpret_cast<const uint4*>(smem + (vs - qs) + i * 16));
+    }
+    float mx0 = -INFINITY, mx1 = -INFINITY;
+#pragma unroll
+    for (int n = 0; n < N / 8; ++n)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int j = base + n * 8 + 2 * (lane & 3) + e;
+        float x0 = score_log2<CAP>(c[n][e], p), x1 = score_log2<CAP>(c[n][2 + e], p);
+        if (a.slopes) {
+          x0 -= s0 * fabsf(float(i0 - j));
+          x1 -= s1 * fabsf(float(i1 - j));
+        }
+        if (!all) {
+          x0 = j < t.len && row_sees(p, t, i0, j) ? x0 : -INFINITY;
+          x1 = j < t.len && row_sees(p, t, i1, j) ? x1 : -INFINITY;
+        }
+        c[n][e] = x0;
+        c[n][2 + e] = x1;
+        mx0 = fmaxf(mx0, x0);
+        mx1 = fmaxf(mx1, x1);
+      }
+#pragma unroll
+    for (int w = 1; w < 4; w <<= 1) {
+      mx0 = fmaxf(mx0, __shfl_xor_sync(~0u, mx0, w));
+      mx1 = fmaxf(mx1, __shfl_xor_sync(~0u, mx1, w));
+    }
+    if (__any_sync(~0u, mx0 > m0 || mx1 > m1)) {
+      const float n0 = fmaxf(m0, mx0), n1 = fmaxf(m1, mx1);
+      const float g0 = m0 == -INFINITY ? 0.f : ex2(m0 - n0), g1 = m1 == -INFINITY ? 0.f : ex2(m1 - n1);
+      m0 = n0;
+      m1 = n1;
+      l0 *= g0;
+      l1 *= g1;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        o[n][0] *= g0;
+        o[n][1] *= g0;
+        o[n][2] *= g1;
+        o[n][3] *= g1;
+      }
+    }
+    const float z0 = m0 == -INFINITY ? 0.f : m0, z1 = m1 == -INFINITY ? 0.f : m1;
+    const int vr = (lane & 7) + (((lane >> 3) & 1) << 3), vc = lane >> 4;
+#pragma unroll
+    for (int s = 0; s < N / 16; ++s) {
+      uint32_t w[4];
+#pragma unroll
+      for (int n = 0; n < 2; ++n) {
+        const float* x = c[2 * s + n];
+        const float p00 = ex2(x[0] - z0), p01 = ex2(x[1] - z0), p10 = ex2(x[2] - z1), p11 = ex2(x[3] - z1);
+        l0 += p00 + p01;
+        l1 += p10 + p11;
+        w[2 * n] = pack2<DT>(p00, p01);
+        w[2 * n + 1] = pack2<DT>(p10, p11);
+      }
+#pragma unroll
+      for (int n = 0; n < NT / 2; ++n) {
+        uint32_t b[4];
+        ldmatrix4_trans(b, vs + uint32_t((s * 16 + vr) * D * 2 + (((2 * n + vc) ^ (vr & 7)) << 4)));
+        mma_16816<DT>(o[2 * n], w, b[0], b[1]);
+        mma_16816<DT>(o[2 * n + 1], w, b[2], b[3]);
+      }
+    }
+  }
+  cp_async_wait<0>();
+  l0 += __shfl_xor_sync(~0u, l0, 1);
+  l1 += __shfl_xor_sync(~0u, l1, 1);
+  l0 += __shfl_xor_sync(~0u, l0, 2);
+  l1 += __shfl_xor_sync(~0u, l1, 2);
+  const float v0 = l0 == 0.f ? 0.f : 1.0f / l0, v1 = l1 == 0.f ? 0.f : 1.0f / l1;
+  T* out = static_cast<T*>(a.out) + 2 * (lane & 3);
+  T* o0 = out + (t.first + t0) * a.o_stride_t + h0 * a.o_stride_h;
+  T* o1 = out + (t.first + t1) * a.o_stride_t + h1 * a.o_stride_h;
+  float fine0 = 0.f, fine1 = 0.f;  // zero, or NaN where an output is not finite
+#pragma unroll
+  for (int n = 0; n < NT; ++n) {
+    const float x0 = o[n][0] * v0, x1 = o[n][1] * v0, y0 = o[n][2] * v1, y1 = o[n][3] * v1;
+    if (f0 < last) *reinterpret_cast<uint32_t*>(o0 + n * 8) = pack2<DT>(x0, x1);
+    if (f1 < last) *reinterpret_cast<uint32_t*>(o1 + n * 8) = pack2<DT>(y0, y1);
+    fine0 += (x0 + x1) * 0.f;
+    fine1 += (y0 + y1) * 0.f;
+  }
+  if (a.lse && (lane & 3) == 0) {
+    if (f0 < last) a.lse[int64_t(t.first + t0) * a.n_q_heads + h0] = (m0 + log2f(l0)) * kLn2;
+    if (f1 < last) a.lse[int64_t(t.first + t1) * a.n_q_heads + h1] = (m1 + log2f(l1)) * kLn2;
+  }
+  if (__syncthreads_or(special)) {
+    const uint32_t redo0 = __ballot_sync(~0u, fine0 != 0.f && l0 == l0), redo1 = __ballot_sync(~0u, fine1 != 0.f && l1 == l1);
+    for (int r = 0; r < 16; ++r) {
+      const int f = t.f0 + warp * 16 + r;
+      if (((r < 8 ? redo0 : redo1) >> (4 * (r & 7)) & 15u) && f < last) exact_row(p, t, kvh, f);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- other types, head dims and alignments
+constexpr int PX_ROWS = 4;
+
+template <class DT, int NI, bool VEC>
+__global__ void __launch_bounds__(PM_THREADS) prefill_simt_kernel(const __grid_constant__ PagedParams p) {
+  using T = typename DT::T;
+  constexpr int GROUPS = PM_THREADS / 8, WARPS = PM_THREADS / 32;
+  __shared__ __align__(16) float qs[PX_ROWS][32 * NI];
+  __shared__ float acc[WARPS][PX_ROWS][32 * NI + 2];
+  __shared__ int sums[WARPS], found[2];
+  const smaq_paged_args& a = p.a;
+  const int D = a.head_dim, l = threadIdx.x & 7, grp = threadIdx.x >> 3, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, kvh = blockIdx.y;
+  write_padding(p, kvh, blockIdx.x, gridDim.x);
+  const PrefillTile t = find_tile<PM_THREADS>(p, blockIdx.x, PX_ROWS, true, sums, found);
+  if (t.rows == 0) return;
+  for (int i = threadIdx.x; i < PX_ROWS * 32 * NI; i += PM_THREADS) {
+    const int r = i / (32 * NI), e = i % (32 * NI), f = t.f0 + r, tok = f / p.group;
+    qs[r][e] = r < t.rows && e < D ? load_elem(a.q, a.dtype, (t.first + tok) * a.q_stride_t + (kvh * p.group + f % p.group) * a.q_stride_h + e) : 0.f;
+  }
+  __syncthreads();
+  float o[PX_ROWS][NI][4] = {}, m[PX_ROWS], s[PX_ROWS], slope[PX_ROWS];
+  int pos[PX_ROWS];
+#pragma unroll
+  for (int r = 0; r < PX_ROWS; ++r) {
+    const int f = t.f0 + r;
+    m[r] = -INFINITY;
+    s[r] = 0.f;
+    pos[r] = r < t.rows ? t.past + f / p.group : -1;
+    slope[r] = a.slopes && r < t.rows ? a.slopes[kvh * p.group + f % p.group] : 0.f;
+  }
+  const PrefillBlocks blocks(t, GROUPS);
+  const int32_t* table = a.block_table + t.b * a.table_stride;
+  const T* kc = static_cast<const T*>(a.k_cache) + kvh * a.c_stride_h;
+  const T* vc = static_cast<const T*>(a.v_cache) + kvh * a.c_stride_h;
+  for (int b = 0; b < blocks.count; ++b) {
+    const int j = blocks.base(b, GROUPS) + grp;
+    const bool seen = tile_sees(t, j);
+    float k[NI][4], v[NI][4];
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int e = 4 * (l + 8 * i);
+#pragma unroll
+      for (int x = 0; x < 4; ++x) k[i][x] = v[i][x] = 0.f;
+      if (!seen) continue;
+      const int64_t off = token_offset(p, table, j);
+      if constexpr (VEC) {
+        if (e < D) {
+          load_vec<DT, 4>(kc + off + e, k[i]);
+          load_vec<DT, 4>(vc + off + e, v[i]);
+        }
+      } else {
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          if (e + x < D) {
+            k[i][x] = to_f(kc[off + e + x]);
+            v[i][x] = to_f(vc[off + e + x]);
+          }
+      }
+    }
+#pragma unroll
+    for (int r = 0; r < PX_ROWS; ++r) {
+      float x = 0.f;
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const float4 q = *reinterpret_cast<const float4*>(&qs[r][4 * (l + 8 * i)]);
+        x = fmaf(q.x, k[i][0], fmaf(q.y, k[i][1], fmaf(q.z, k[i][2], fmaf(q.w, k[i][3], x))));
+      }
+#pragma unroll
+      for (int w = 1; w < 8; w <<= 1) x += __shfl_xor_sync(~0u, x, w);
+      x *= a.scale;
+      if (a.softcap > 0.f) x = a.softcap * tanhf(x / a.softcap);
+      x = (x - slope[r] * fabsf(float(pos[r] - j))) * kLog2e;
+      if (!seen || !row_sees(p, t, pos[r], j)) continue;
+      if (x > m[r]) {
+        const float f = ex2(m[r] - x);
+        m[r] = x;
+        s[r] *= f;
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[r][i][e] *= f;
+      }
+      const float w = ex2(x - (m[r] == -INFINITY ? 0.f : m[r]));
+      s[r] += w;
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[r][i][e] = fmaf(w, v[i][e], o[r][i][e]);
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < PX_ROWS; ++r) {
+#pragma unroll
+    for (int w = 8; w < 32; w <<= 1) {
+      const float om = __shfl_xor_sync(~0u, m[r], w), os = __shfl_xor_sync(~0u, s[r], w);
+      const float nm = fmaxf(m[r], om), z = nm == -INFINITY ? 0.f : nm, f = ex2(m[r] - z), g = ex2(om - z);
+      m[r] = nm;
+      s[r] = s[r] * f + os * g;
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[r][i][e] = o[r][i][e] * f + __shfl_xor_sync(~0u, o[r][i][e], w) * g;
+    }
+    if (lane < 8) {
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[warp][r][4 * (l + 8 * i) + e] = o[r][i][e];
+      if (l == 0) {
+        acc[warp][r][32 * NI] = m[r];
+        acc[warp][r][32 * NI + 1] = s[r];
+      }
+    }
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < t.rows * D; i += PM_THREADS) {
+    const int r = i / D, e = i - r * D, f = t.f0 + r, tok = f / p.group, h = kvh * p.group + f % p.group;
+    float mm = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) mm = fmaxf(mm, acc[w][r][32 * NI]);
+    const float z = mm == -INFINITY ? 0.f : mm;
+    float x = 0.f, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const float g = ex2(acc[w][r][32 * NI] - z);
+      x += g * acc[w][r][e];
+      sum += g * acc[w][r][32 * NI + 1];
+    }
+    store_elem(a.out, a.dtype, int64_t(t.first + tok) * a.o_stride_t + h * a.o_stride_h + e, sum == 0.f ? 0.f : x / sum);
+    if (a.lse && e == 0) a.lse[int64_t(t.first + tok) * a.n_q_heads + h] = (mm + log2f(sum)) * kLn2;
+  }
+}
+
+// Tiles that any cu_query of this many rows and requests can have.
+int64_t most_tiles(const PagedParams& p, int size) {
+  return (p.a.n_rows * p.group + size - 1) / size + p.a.batch;
+}
+
+template <class DT, int D>
+int launch_mma(const PagedParams& p, cudaStream_t st) {
+  auto kern = p.a.softcap > 0.f ? prefill_mma_kernel<DT, D, true> : prefill_mma_kernel<DT, D, false>;
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PmCfg<D>::SMEM);
+  if (e != cudaSuccess) return cuda_status(e, "paged_prefill attr");
+  kern<<<dim3(unsigned(most_tiles(p, PmCfg<D>::ROWS)), p.a.n_kv_heads), PM_THREADS, PmCfg<D>::SMEM, st>>>(p);
+  return cuda_status(cudaGetLastError(), "paged_prefill");
+}
+template <class DT>
+int launch_mma_dim(const PagedParams& p, cudaStream_t st) {
+  switch (p.a.head_dim) {
+    case 64: return launch_mma<DT, 64>(p, st);
+    case 128: return launch_mma<DT, 128>(p, st);
+    default: return launch_mma<DT, 256>(p, st);
+  }
+}
+template <class DT>
+int launch_simt(const PagedParams& p, cudaStream_t st) {
+  const int D = p.a.head_dim;
+  const bool vec = D % 4 == 0 && paged_aligned(p.a);
+  auto go = [&](auto kern) {
+    kern<<<dim3(unsigned(most_tiles(p, PX_ROWS)), p.a.n_kv_heads), PM_THREADS, 0, st>>>(p);
+    return cuda_status(cudaGetLastError(), "paged_prefill");
+  };
+  if (D <= 64) return vec ? go(prefill_simt_kernel<DT, 2, true>) : go(prefill_simt_kernel<DT, 2, false>);
+  if (D <= 128) return vec ? go(prefill_simt_kernel<DT, 4, true>) : go(prefill_simt_kernel<DT, 4, false>);
+  return vec ? go(prefill_simt_kernel<DT, 8, true>) : go(prefill_simt_kernel<DT, 8, false>);
+}
+
+}  // namespace
+
+}  // namespace smaq
+
+extern "C" int smaq_paged_prefill(const smaq_paged_args* args, void* stream) {
+  using namespace smaq;
+  PagedParams p;
+  if (const int st = paged_check(args, true, p)) return st;
+  const smaq_paged_args& a = p.a;
+  if (a.n_rows == 0) return SMAQ_OK;
+  if (a.n_kv_heads > 65535) return fail(SMAQ_ERR_UNSUPPORTED, "paged_prefill: %d KV heads above 65535", a.n_kv_heads);
+  if (most_tiles(p, PX_ROWS) >= (int64_t(1) << 31)) return fail(SMAQ_ERR_UNSUPPORTED, "paged_prefill: too many rows");
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (a.dtype != SMAQ_F32 && (a.head_dim == 64 || a.head_dim == 128 || a.head_dim == 256) && paged_aligned(a))
+    return a.dtype == SMAQ_BF16 ? launch_mma_dim<BF16>(p, st) : launch_mma_dim<F16>(p, st);
+  return a.dtype == SMAQ_F32 ? launch_simt<F32>(p, st) : a.dtype == SMAQ_BF16 ? launch_simt<BF16>(p, st) : launch_simt<F16>(p, st);
+}

@@ -9,7 +9,7 @@ CPU implementation.
 from __future__ import annotations
 
 import math
-from typing import Optional
+from typing import NamedTuple, Optional
 
 import torch
 
@@ -469,6 +469,306 @@ def merge_partials(partials: torch.Tensor, out_dtype: torch.dtype) -> torch.Tens
     _lib.check(lib.smaq_merge_partials(p.data_ptr(), R, B, Hq, D, out.data_ptr(), dtype_code(out_dtype),
                                        out.stride(0), out.stride(1), _stream()), "smaq_merge_partials")
     return out
+
+
+# --------------------------------------------------------------------- exact paged step
+class StepTables(NamedTuple):
+    """What ``step_tables`` builds (smaq_tables_args in include/smaq_b200.h)."""
+    cu_query: torch.Tensor      # [B + 1] int32, prefix sums of the query lengths
+    seq_lens: torch.Tensor      # [B] int32, context + query; 0: finished or not admitted
+    positions: torch.Tensor     # [num_tokens] int32
+    slots: torch.Tensor         # [num_tokens] int64, page * block_size + offset; -1: no slot
+    free_count: torch.Tensor    # [1] int32
+    admitted: torch.Tensor      # [B] bool
+
+
+def _same_device(dev: torch.device, **ts: Optional[torch.Tensor]) -> int:
+    """Every given tensor is on ``dev``, the current CUDA device; returns the current stream there."""
+    for name, t in ts.items():
+        if t is not None and t.device != dev:
+            if not t.is_cuda:
+                _cuda(t)
+            raise ValueError(f"{name} is on {t.device}, expected {dev}")
+    if dev.type != "cuda":
+        raise RuntimeError(f"smaq_b200 kernels need CUDA tensors (there is no CPU fallback); got a tensor on {dev}")
+    if dev.index != torch.cuda.current_device():
+        raise ValueError(f"tensors are on {dev}, but the current device is cuda:{torch.cuda.current_device()}")
+    return torch.cuda.current_stream().cuda_stream
+
+
+def _int32(name: str, t: torch.Tensor, n: int) -> torch.Tensor:
+    if t.dim() != 1 or t.shape[0] != n:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected ({n},)")
+    if t.dtype != torch.int32:
+        if t.dtype.is_floating_point or t.dtype == torch.bool:
+            raise ValueError(f"{name} must be an integer tensor, got {t.dtype}")
+        t = t.to(torch.int32)
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def step_tables(free_blocks: torch.Tensor, free_count: torch.Tensor, context_lens: torch.Tensor,
+                query_lens: torch.Tensor, block_table: torch.Tensor, *, block_size: int, num_tokens: int,
+                finished: Optional[torch.Tensor] = None) -> StepTables:
+    """Block bookkeeping of one step in one launch (smaq_step_tables).
+
+    ``free_blocks[:free_count]`` is the stack of free pages.  Requests marked in ``finished [B]`` give
+    their pages back; then request ``b`` grows from ``context_lens[b]`` by ``query_lens[b]`` tokens and
+    takes the pages it lacks, in request order while the stack lasts.  A request whose pages run out or
+    that outgrows its row of ``block_table [B, M]`` is not admitted: its slots are -1 and its sequence
+    length is 0.  ``free_blocks`` (int32) and ``block_table`` (int32) are updated in place, the
+    new ``free_count`` is returned.  ``num_tokens``: length of ``positions`` and ``slots``; entries past
+    the step's tokens get position 0 and slot -1.  Nothing is read back to the host."""
+    dev = free_blocks.device
+    stream = _same_device(dev, free_blocks=free_blocks, free_count=free_count, context_lens=context_lens,
+                          query_lens=query_lens, block_table=block_table, finished=finished)
+    B = context_lens.shape[0]
+    if free_blocks.dtype != torch.int32 or free_blocks.dim() != 1 or not free_blocks.is_contiguous():
+        raise ValueError("free_blocks must be a contiguous int32 vector (it is updated in place)")
+    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B or (
+            block_table.shape[1] > 1 and block_table.stride(1) != 1):
+        raise ValueError(f"block_table must be int32 [{B}, M] with contiguous rows (it is updated in place)")
+    if num_tokens < 0 or block_size < 1:
+        raise ValueError(f"num_tokens {num_tokens} or block_size {block_size} out of range")
+    free_count = _int32("free_count", free_count, 1)
+    context_lens, query_lens = _int32("context_lens", context_lens, B), _int32("query_lens", query_lens, B)
+    if finished is not None:
+        if finished.shape != (B,) or finished.dtype not in (torch.bool, torch.uint8):
+            raise ValueError(f"finished must be a bool vector of length {B}")
+        finished = finished.contiguous()
+    # one buffer: slots (8 bytes) first, then the int32 outputs, positions on a 16-byte boundary
+    pad = (num_tokens + 3) // 4 * 4
+    buf = torch.empty((3 * pad + 2 * B + 2,), dtype=torch.int32, device=dev)
+    slots = buf[:2 * num_tokens].view(torch.int64)
+    positions = buf[2 * pad:2 * pad + num_tokens]
+    cu, lens, left = buf[3 * pad:3 * pad + B + 1], buf[3 * pad + B + 1:3 * pad + 2 * B + 1], buf[3 * pad + 2 * B + 1:]
+    admitted = torch.empty((B,), dtype=torch.bool, device=dev)
+    M = block_table.shape[1]
+    at = buf.data_ptr()
+    a = _lib.TablesArgs(free_blocks.data_ptr(), free_count.data_ptr(), context_lens.data_ptr(), query_lens.data_ptr(),
+                        _ptr(finished), block_table.data_ptr(), max(block_table.stride(0), M), free_blocks.shape[0],
+                        num_tokens, B, M, block_size, at + 12 * pad, at + 12 * pad + 4 * (B + 1), at + 8 * pad, at,
+                        admitted.data_ptr(), at + 12 * pad + 4 * (2 * B + 1))
+    st = _lib.load().smaq_step_tables(a, stream)
+    if st:
+        _lib.check(st, "smaq_step_tables")
+    return StepTables(cu, lens, positions, slots, left, admitted)
+
+
+def rope_table(max_positions: int, rotary_dim: int, base: float = 10000.0, *, linear: float = 1.0,
+               ntk: float = 1.0, yarn: Optional[dict] = None, device="cuda") -> torch.Tensor:
+    """``[max_positions, rotary_dim]`` fp32 rows ``cos | sin`` for ``norm_rope``, computed in fp64.
+
+    Long contexts: ``linear`` divides positions; ``ntk`` raises the base to
+    ``base * ntk ** (R / (R - 2))``; ``yarn = dict(factor, original, beta_fast=32, beta_slow=1,
+    attention=None)`` interpolates between the plain and the divided frequency of each pair by the
+    number of turns it makes over ``original`` positions, and multiplies the rows by
+    ``attention`` (default ``0.1 ln(factor) + 1``)."""
+    R = rotary_dim
+    if max_positions < 1 or R < 2 or R % 2:
+        raise ValueError(f"rope_table: max_positions {max_positions} or rotary_dim {rotary_dim} out of range")
+    if linear <= 0 or ntk <= 0 or base <= 0:
+        raise ValueError("rope_table: base and scaling factors must be positive")
+    if ntk != 1.0:
+        if R == 2:
+            raise ValueError("rope_table: ntk scaling needs a rotary_dim above 2")
+        base = base * ntk ** (R / (R - 2))
+    exps = torch.arange(0, R, 2, dtype=torch.float64, device=device) / R
+    freq = base ** -exps
+    gain = 1.0
+    if yarn is not None:
+        factor, original = float(yarn["factor"]), float(yarn["original"])
+        fast, slow = float(yarn.get("beta_fast", 32.0)), float(yarn.get("beta_slow", 1.0))
+        if factor <= 0 or original <= 0 or fast <= slow:
+            raise ValueError("rope_table: yarn needs factor, original > 0 and beta_fast > beta_slow")
+
+        def pair(turns):  # index of the pair that makes this many turns over `original` positions
+            return R * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(base))
+        lo, hi = max(math.floor(pair(fast)), 0), min(math.ceil(pair(slow)), R - 1)
+        ramp = ((torch.arange(R // 2, dtype=torch.float64, device=device) - lo) / max(hi - lo, 1e-3)).clamp(0, 1)
+        freq = freq * (1 - ramp) + freq / factor * ramp
+        gain = yarn.get("attention")
+        if gain is None:
+            gain = 0.1 * math.log(factor) + 1.0 if factor > 1 else 1.0
+    angle = torch.arange(max_positions, dtype=torch.float64, device=device)[:, None] / linear * freq
+    return (torch.cat([angle.cos(), angle.sin()], 1) * gain).to(torch.float32)
+
+
+def _head_rows(name: str, x: torch.Tensor, dtype: torch.dtype, T: int, D: int) -> torch.Tensor:
+    if x.dim() != 3 or x.shape[0] != T or x.shape[2] != D or x.dtype != dtype:
+        raise ValueError(f"{name} must be {dtype} [{T}, heads, {D}], got {x.dtype} {tuple(x.shape)}")
+    return x if x.stride(2) == 1 or D == 1 else x.contiguous()
+
+
+def _cache_pair(k_cache: torch.Tensor, v_cache: torch.Tensor, dtype: torch.dtype, D: int) -> None:
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[3] != D:
+        raise ValueError(f"caches must be [pages, page_size, kv_heads, {D}], got {tuple(k_cache.shape)} and "
+                         f"{tuple(v_cache.shape)}")
+    if k_cache.dtype != dtype or v_cache.dtype != dtype:
+        raise ValueError(f"caches must be {dtype} like the queries, got {k_cache.dtype} and {v_cache.dtype}")
+    if k_cache.stride() != v_cache.stride() or (D > 1 and k_cache.stride(3) != 1):
+        raise ValueError("caches must have the same strides and a contiguous head_dim")
+
+
+def norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, *,
+              q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+              interleaved: bool = False, v: Optional[torch.Tensor] = None, k_cache: Optional[torch.Tensor] = None,
+              v_cache: Optional[torch.Tensor] = None, slots: Optional[torch.Tensor] = None):
+    """Per-head RMS norm and rotation of ``q [T, Hq, D]`` and ``k [T, Hkv, D]`` in one pass
+    (smaq_norm_rope); returns ``(q_out, k_out)``.
+
+    ``table [P, R]``: rows ``cos | sin`` (``rope_table``) read at ``positions [T]``; the first ``R``
+    channels turn in pairs ``(i, i + R/2)``, or ``(2i, 2i + 1)`` with ``interleaved``, the others pass.
+    ``q_weight / k_weight [D]``: norm weights, None: no norm.  Heads may be views of a fused
+    projection (any token and head stride).  With ``v, k_cache, v_cache, slots`` the keys and values go
+    straight to the exact cache ``[pages, page_size, Hkv, D]`` at ``slots [T]`` (a slot outside the
+    cache is skipped) and ``k_out`` is None."""
+    T, Hq, D = q.shape
+    dt = q.dtype
+    code = dtype_code(dt)
+    stream = _same_device(q.device, q=q, k=k, positions=positions, table=table, q_weight=q_weight, k_weight=k_weight,
+                          v=v, k_cache=k_cache, v_cache=v_cache, slots=slots)
+    q, k = _head_rows("q", q, dt, T, D), _head_rows("k", k, dt, T, D)
+    Hk = k.shape[1]
+    positions = _int32("positions", positions, T)
+    if table.dim() != 2 or table.dtype != torch.float32 or table.shape[1] > D or table.shape[1] % 2:
+        raise ValueError(f"table must be float32 [positions, R] with an even R <= {D}, got {table.dtype} "
+                         f"{tuple(table.shape)}")
+    table = table.contiguous()
+
+    def weight(name, w):
+        if w is None:
+            return None
+        if w.shape != (D,):
+            raise ValueError(f"{name} must have shape ({D},), got {tuple(w.shape)}")
+        return w if w.dtype == torch.float32 and w.is_contiguous() else w.to(torch.float32).contiguous()
+    q_weight, k_weight = weight("q_weight", q_weight), weight("k_weight", k_weight)
+    given = [x is not None for x in (v, k_cache, v_cache, slots)]
+    if any(given) and not all(given):
+        raise ValueError("a cache write needs v, k_cache, v_cache and slots together")
+    q_out = torch.empty((T, Hq, D), dtype=dt, device=q.device)
+    k_out = None
+    vs = cs = (0, 0, 0)
+    pages = page_size = 0
+    if k_cache is not None:
+        v = _head_rows("v", v, dt, T, D)
+        _cache_pair(k_cache, v_cache, dt, D)
+        if v.shape[1] != Hk or k_cache.shape[2] != Hk:
+            raise ValueError(f"v has {v.shape[1]} heads and the cache {k_cache.shape[2]}, k has {Hk}")
+        if slots.shape != (T,):
+            raise ValueError(f"slots has shape {tuple(slots.shape)}, expected ({T},)")
+        slots = slots if slots.dtype == torch.int64 and slots.is_contiguous() else slots.to(torch.int64).contiguous()
+        vs, cs, pages, page_size = v.stride(), k_cache.stride(), k_cache.shape[0], k_cache.shape[1]
+    else:
+        k_out = torch.empty((T, Hk, D), dtype=dt, device=q.device)
+    qs, ks = q.stride(), k.stride()
+    a = _lib.NormRopeArgs(q.data_ptr(), k.data_ptr(), _ptr(v), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1],
+                          positions.data_ptr(), table.data_ptr(), _ptr(q_weight), _ptr(k_weight), _ptr(slots),
+                          q_out.data_ptr(), _ptr(k_out), _ptr(k_cache), _ptr(v_cache), cs[0], cs[1], cs[2], T,
+                          table.shape[0], pages, code, Hq, Hk, D, table.shape[1], int(interleaved), page_size, eps)
+    st = _lib.load().smaq_norm_rope(a, stream)
+    if st:
+        _lib.check(st, "smaq_norm_rope")
+    return q_out, k_out
+
+
+def paged_decode_workspace_bytes(batch: int, n_q_heads: int, n_kv_heads: int, head_dim: int) -> int:
+    return int(_lib.load().smaq_paged_decode_workspace_size(batch, n_q_heads, n_kv_heads, head_dim))
+
+
+def _paged(name, q, k_cache, v_cache, block_table, seq_lens, cu_query, prefix_lens, scale, window, softcap, slopes,
+           out, return_lse, workspace):
+    if q.dim() != 3:
+        raise ValueError(f"q must be [rows, heads, head_dim], got {tuple(q.shape)}")
+    T, Hq, D = q.shape
+    dt = q.dtype
+    code = dtype_code(dt)
+    stream = _same_device(q.device, q=q, k_cache=k_cache, v_cache=v_cache, block_table=block_table, seq_lens=seq_lens,
+                          cu_query=cu_query, prefix_lens=prefix_lens, slopes=slopes, out=out, workspace=workspace)
+    if q.stride(2) != 1 and D > 1:
+        q = q.contiguous()
+    _cache_pair(k_cache, v_cache, dt, D)
+    P, page_size, Hk, _ = k_cache.shape
+    if block_table.dim() != 2:
+        raise ValueError(f"block_table must be [batch, blocks], got {tuple(block_table.shape)}")
+    B, M = block_table.shape
+    if block_table.dtype != torch.int32:
+        block_table = block_table.to(torch.int32)
+    if M > 1 and block_table.stride(1) != 1:
+        block_table = block_table.contiguous()
+    seq_lens = _int32("seq_lens", seq_lens, B)
+    if Hk == 0 or Hq % Hk:
+        raise ValueError(f"{Hq} query heads do not divide over {Hk} KV heads")
+    if window is not None and window < 1:
+        raise ValueError(f"window must be at least 1, got {window}")
+    if softcap is not None and not softcap > 0:
+        raise ValueError(f"softcap must be positive, got {softcap}")
+    if prefix_lens is not None:
+        prefix_lens = _int32("prefix_lens", prefix_lens, B)
+    if slopes is not None:
+        if slopes.shape != (Hq,):
+            raise ValueError(f"slopes has shape {tuple(slopes.shape)}, expected ({Hq},)")
+        if slopes.dtype != torch.float32 or not slopes.is_contiguous():
+            slopes = slopes.to(torch.float32).contiguous()
+    if out is None:
+        out = torch.empty((T, Hq, D), dtype=dt, device=q.device)
+    elif out.shape != q.shape or out.dtype != dt or (D > 1 and out.stride(2) != 1):
+        raise ValueError(f"out must be {dt} {tuple(q.shape)} with a contiguous head_dim")
+    lse = torch.empty((T, Hq), dtype=torch.float32, device=q.device) if return_lse else None
+    qs, cs, os = q.stride(), k_cache.stride(), out.stride()
+    lib = _lib.load()
+    if cu_query is None:
+        if T != B:
+            raise ValueError(f"q has {T} rows for {B} requests; one row a request")
+        need = lib.smaq_paged_decode_workspace_size(B, Hq, Hk, D)
+        if workspace is None:
+            workspace = torch.empty((need,), dtype=torch.uint8, device=q.device)
+        ws, ws_bytes, call = workspace.data_ptr(), workspace.numel() * workspace.element_size(), lib.smaq_paged_decode
+    else:
+        cu_query = _int32("cu_query", cu_query, B + 1)
+        ws, ws_bytes, call = None, 0, lib.smaq_paged_prefill
+    a = _lib.PagedArgs(q.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2],
+                       block_table.data_ptr(), max(block_table.stride(0), M), seq_lens.data_ptr(), _ptr(cu_query),
+                       _ptr(prefix_lens), _ptr(slopes), out.data_ptr(), os[0], os[1], _ptr(lse), ws, ws_bytes, P, T, B,
+                       M, page_size, Hq, Hk, D, code, window or 0, 1.0 / math.sqrt(D) if scale is None else scale,
+                       softcap or 0.0)
+    st = call(a, stream)
+    if st:
+        _lib.check(st, name)
+    return (out, lse) if return_lse else out
+
+
+def paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                 seq_lens: torch.Tensor, *, scale: Optional[float] = None, window: Optional[int] = None,
+                 softcap: Optional[float] = None, slopes: Optional[torch.Tensor] = None,
+                 out: Optional[torch.Tensor] = None, return_lse: bool = False,
+                 workspace: Optional[torch.Tensor] = None):
+    """Attention of one new token per request over the exact paged cache (smaq_paged_decode).
+
+    ``q [B, Hq, D]``; caches ``[pages, page_size, Hkv, D]`` of the query dtype; ``block_table [B, M]``;
+    ``seq_lens [B]`` count the new token, already written.  ``window``: the last tokens that are seen;
+    ``softcap``: scores become ``c * tanh(x / c)``; ``slopes [Hq]``: ``slope * distance`` is taken off.
+    A request of length 0 gives zeros.  Returns ``out [B, Hq, D]``, with ``return_lse`` also the
+    natural log-sum-exp ``[B, Hq]`` (fp32).  ``workspace``: ``paged_decode_workspace_bytes`` bytes (uint8),
+    allocated per call when None."""
+    return _paged("smaq_paged_decode", q, k_cache, v_cache, block_table, seq_lens, None, None, scale, window, softcap,
+                  slopes, out, return_lse, workspace)
+
+
+def paged_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                  seq_lens: torch.Tensor, cu_query: torch.Tensor, *, prefix_lens: Optional[torch.Tensor] = None,
+                  scale: Optional[float] = None, window: Optional[int] = None, softcap: Optional[float] = None,
+                  slopes: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+                  return_lse: bool = False):
+    """Attention of prompt chunks over the exact paged cache (smaq_paged_prefill).
+
+    Rows ``cu_query[b] .. cu_query[b + 1]`` of ``q [T, Hq, D]`` are request ``b``'s newest tokens (the
+    last ones of its ``seq_lens[b]``, already written): row ``i`` sees tokens up to its own, the last
+    ``window`` of them if given, and the first ``prefix_lens[b]`` in any case.  Requests never see one
+    another.  Other arguments as ``paged_decode``; rows past ``cu_query[B]`` give zeros."""
+    if cu_query is None:
+        raise ValueError("paged_prefill needs cu_query")
+    return _paged("smaq_paged_prefill", q, k_cache, v_cache, block_table, seq_lens, cu_query, prefix_lens, scale,
+                  window, softcap, slopes, out, return_lse, None)
 
 
 # --------------------------------------------------------------------- failure detection
