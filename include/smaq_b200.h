@@ -487,6 +487,9 @@ typedef struct smaq_paged_args {
 size_t smaq_paged_decode_workspace_size(int batch, int n_q_heads, int n_kv_heads, int head_dim);
 int smaq_paged_decode(const smaq_paged_args* args, void* stream);
 int smaq_paged_prefill(const smaq_paged_args* args, void* stream);
+/* SMAQ_ERR_DEVICE if a bounded wait of the tensor-core prefill kernel ran out since the last check
+ * (clears it).  Synchronises the stream. */
+int smaq_prefill_status(void* stream);
 /* sizeof(smaq_tables_args), smaq_norm_rope_args, smaq_paged_args for which = 0, 1, 2, else 0. */
 size_t smaq_paged_args_size(int which);
 

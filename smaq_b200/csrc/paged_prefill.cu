@@ -11,6 +11,7 @@
 // prefill_simt_kernel (fp32, other head dims and alignments): tiles of four rows, 16 lane groups with a token
 //   each; all arithmetic in 32 bits.
 #include "paged_prefill.cuh"
+#include "prefill_tc.cuh"
 
 namespace smaq {
 
@@ -386,6 +387,7 @@ extern "C" int smaq_paged_prefill(const smaq_paged_args* args, void* stream) {
   if (a.n_kv_heads > 65535) return fail(SMAQ_ERR_UNSUPPORTED, "paged_prefill: %d KV heads above 65535", a.n_kv_heads);
   if (most_tiles(p, PX_ROWS) >= (int64_t(1) << 31)) return fail(SMAQ_ERR_UNSUPPORTED, "paged_prefill: too many rows");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (prefill_tc_eligible(a)) return launch_prefill_tc(p, st);
   if (a.dtype != SMAQ_F32 && (a.head_dim == 64 || a.head_dim == 128 || a.head_dim == 256) && paged_aligned(a))
     return a.dtype == SMAQ_BF16 ? launch_mma_dim<BF16>(p, st) : launch_mma_dim<F16>(p, st);
   return a.dtype == SMAQ_F32 ? launch_simt<F32>(p, st) : a.dtype == SMAQ_BF16 ? launch_simt<BF16>(p, st) : launch_simt<F16>(p, st);

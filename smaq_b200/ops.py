@@ -785,6 +785,11 @@ def append_status() -> None:
     _lib.check(_lib.load().smaq_append_status(_stream()), "smaq_append_status")
 
 
+def prefill_status() -> None:
+    """Raise if a bounded device wait of ``paged_prefill`` ran out since the last check (clears it)."""
+    _lib.check(_lib.load().smaq_prefill_status(_stream()), "smaq_prefill_status")
+
+
 def selftest_wait_timeout(spin_limit: int = 1 << 12) -> int:
     """Run a kernel whose mbarrier wait can never complete with a ``spin_limit`` poll bound;
     returns the library status (``5`` = SMAQ_ERR_DEVICE when the timeout path works)."""
