@@ -14,6 +14,11 @@
 // lags by at most that, so weights stay below 2^8 in either type).
 // Weights are rounded once, to the cache's type; the sums are of the unrounded ones.
 // Every wait is bounded; one that runs out sets g_prefill_fault and the CTA drains.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <mutex>
+
 #include "paged_prefill.cuh"
 #include "prefill_tc.cuh"
 #include "tcgen05.cuh"
@@ -44,6 +49,13 @@ struct PtCfg {
   static constexpr int SMEM = 2 * TILE + 2 * STAGES * TILE + 1024;
 };
 
+struct PtParams {
+  PagedParams p;
+  int tma;         // keys and values come through the tensor maps where every token of a block is seen
+  int box;         // slots a box: page_size, at most PT_N
+  CUtensorMap k, v;
+};
+
 struct PtBars {
   uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready[2], o_full[2];
   uint32_t tmem;
@@ -51,8 +63,9 @@ struct PtBars {
 };
 
 template <class DT, int D, bool MOD>
-__global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_constant__ PagedParams p) {
+__global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_constant__ PtParams pt) {
   using T = typename DT::T;
+  const PagedParams& p = pt.p;
   constexpr int TILE = PtCfg<D>::TILE, STAGES = PtCfg<D>::STAGES, CH = D / 8, ATOM = 128 * 128;
   constexpr uint32_t ID_S = idesc(DT::code == SMAQ_BF16, PT_N, false), ID_O = idesc(DT::code == SMAQ_BF16, D, true);
   extern __shared__ uint8_t smem_raw[];
@@ -62,10 +75,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
   const uint32_t base_raw = smem_u32(smem_raw), pad = (1024u - (base_raw & 1023u)) & 1023u;
   uint8_t* smem = smem_raw + pad;
   const uint32_t qs = base_raw + pad, ks = qs + 2 * TILE, vs = ks + STAGES * TILE;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kvh = blockIdx.y;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kvh = int(blockIdx.x % unsigned(a.n_kv_heads)), tile = int(blockIdx.x / unsigned(a.n_kv_heads));
 
-  write_padding(p, kvh, blockIdx.x, gridDim.x);
-  const PrefillTile t = find_tile<PT_THREADS>(p, blockIdx.x, PT_ROWS, true, sums, found);
+  write_padding(p, kvh, tile, int(gridDim.x / unsigned(a.n_kv_heads)));
+  const PrefillTile t = find_tile<PT_THREADS>(p, tile, PT_ROWS, true, sums, found);
   if (t.rows == 0) return;
   const PrefillBlocks blocks(t, PT_N);
   const int n = blocks.count, tiles = t.rows > 128 ? 2 : 1;
@@ -88,7 +101,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
   fence_before();
   __syncthreads();
   fence_after();
-  const uint32_t tmem = bars.tmem;
+  constexpr uint32_t tmem = 0;  // all 512 columns are this CTA's: the allocation starts at 0
   const uint32_t s_col = 0, o_col = 256;  // S of tile i at s_col + 128 i, O at o_col + D i
   bool failed = false;
 
@@ -130,23 +143,80 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
         cp_async_commit();
       };
       // copy g = 2 j brings keys of block j, 2 j + 1 its values; a copy is announced two copies later
+      // values of a block that some rows see in part: look for infinities and NaN where this thread copies
+      auto look_for_special = [&](int s) {
+        bool odd_value = false;
+        constexpr int PER = 32 / CH;
+        for (int i = 0; i < 32 / PER; ++i) {
+          const int ch = lane % CH, r = 32 * w + i * PER + lane / CH;
+          odd_value |= any_special<DT>(*reinterpret_cast<const uint4*>(smem + (vs - qs) + s * TILE + (ch >> 3) * ATOM + r * 128 + (((ch & 7) ^ (r & 7)) << 4)));
+        }
+        if (odd_value) bars.special = 1;
+      };
       auto announce = [&](int g) {
         const int j = g >> 1, s = j % STAGES;
-        if ((g & 1) && !seen_by_all(blocks.base(j, PT_N))) {
-          // values of a block that some rows see in part: look for infinities and NaN among this thread's own copies
-          bool odd_value = false;
-          constexpr int PER = 32 / CH;
-          for (int i = 0; i < 32 / PER; ++i) {
-            const int ch = lane % CH, r = 32 * w + i * PER + lane / CH;
-            odd_value |= any_special<DT>(*reinterpret_cast<const uint4*>(smem + (vs - qs) + s * TILE + (ch >> 3) * ATOM + r * 128 + (((ch & 7) ^ (r & 7)) << 4)));
-          }
-          if (odd_value) bars.special = 1;
-        }
+        if ((g & 1) && !seen_by_all(blocks.base(j, PT_N))) look_for_special(s);
         fence_proxy_async_smem();
         mbar_arrive((g & 1) ? &bars.v_full[s] : &bars.k_full[s]);
       };
-      int64_t off = look_up(0);
-      for (int j = 0; j < n && !failed; ++j) {
+      if (pt.tma) {
+        // A block whose every token is seen by some row comes in boxes of one page (or 128 slots of it) by 64
+        // channels, a lane of warp 0 each; the others as below, announced at once.
+        const int per = PT_N / pt.box, boxes = per * (D / 64);
+        auto whole = [&](int k) {
+          const int b = blocks.base(k, PT_N);
+          return b + PT_N <= t.prefix || (b >= t.lo && b + PT_N <= t.hi);
+        };
+        auto page_of = [&](int k) {
+          if (k >= n || lane >= boxes || !whole(k)) return 0;
+          const int64_t blk = fast_div(blocks.base(k, PT_N) + (lane % per) * pt.box, p.page_div);
+          return int(min(max(int64_t(__ldg(table + blk)), int64_t(0)), a.n_pages - 1));
+        };
+        auto fetch = [&](int j, int s, bool values, int page, int64_t off) {
+          uint64_t* bar = values ? &bars.v_full[s] : &bars.k_full[s];
+          const uint32_t dst = (values ? vs : ks) + s * TILE;
+          if (whole(j)) {
+            if (w == 0) {
+              if (lane == 0) mbar_arrive_expect_tx(bar, TILE);
+              __syncwarp();
+              if (lane < boxes) {
+                const int half = lane / per, b = lane % per, slot = blocks.base(j, PT_N) + b * pt.box;
+                tma_4d(dst + half * ATOM + b * pt.box * 128, values ? &pt.v : &pt.k, half * 64, kvh, slot - fast_div(slot, p.page_div) * a.page_size, page, bar);
+              }
+              if (lane != 0) mbar_arrive(bar);
+            } else {
+              mbar_arrive(bar);
+            }
+            if (values && !seen_by_all(blocks.base(j, PT_N))) {
+              if (!warp_wait(bar, (j / STAGES) & 1)) failed = true;
+              look_for_special(s);
+              fence_proxy_async_smem();  // before the stage is filled again
+            }
+            return;
+          }
+          bring(values ? a.v_cache : a.k_cache, dst, off);
+          cp_async_wait<0>();
+          announce(2 * j + values);
+        };
+        cp_async_wait<0>();
+        fence_proxy_async_smem();
+        mbar_arrive(&bars.q_full);
+        int page = page_of(0);
+        for (int j = 0; j < n; ++j) {
+          const int s = j % STAGES;
+          const uint32_t ph = uint32_t((j / STAGES) & 1) ^ 1u;
+          const int next = page_of(j + 1);
+          const int64_t off = whole(j) ? 0 : look_up(j);
+          if (!warp_wait(&bars.k_empty[s], ph)) { failed = true; break; }
+          fetch(j, s, false, page, off);
+          if (!warp_wait(&bars.v_empty[s], ph)) { failed = true; break; }
+          fetch(j, s, true, page, off);
+          if (failed) break;
+          page = next;
+        }
+      }
+      int64_t off = pt.tma ? -1 : look_up(0);
+      for (int j = 0; j < n && !failed && !pt.tma; ++j) {
         const int s = j % STAGES;
         const uint32_t ph = uint32_t((j / STAGES) & 1) ^ 1u;
         const int64_t next = look_up(j + 1);
@@ -166,49 +236,50 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
         off = next;
       }
       cp_async_wait<0>();
-      if (!failed && n > 0) {
+      if (!failed && n > 0 && !pt.tma) {
         announce(2 * n - 2);
         announce(2 * n - 1);
       }
-    } else if (warp == PT_MMA_WARP && lane == 0 && n > 0) {
+    } else if (warp == PT_MMA_WARP && n > 0) {
       // ---- products
+      const uint32_t lead = elect_one();
       auto scores = [&](int i, int j) {
         const uint32_t q = qs + i * TILE, k = ks + (j % STAGES) * TILE;
 #pragma unroll
         for (int c = 0; c < D / 16; ++c) {
           const uint32_t at = uint32_t((c >> 2) * ATOM + (c & 3) * 32);
-          mma_ss(tmem + s_col + 128 * i, desc(q + at, 16), desc(k + at, 16), ID_S, c > 0);
+          mma_ss(lead, tmem + s_col + 128 * i, desc(q + at, 16), desc(k + at, 16), ID_S, c > 0);
         }
-        commit(&bars.s_full[i]);
+        commit(lead, &bars.s_full[i]);
       };
-      bool ok = mbar_wait(&bars.q_full, 0, PT_SPIN) && mbar_wait(&bars.k_full[0], 0, PT_SPIN);
+      bool ok = warp_wait(&bars.q_full, 0) && warp_wait(&bars.k_full[0], 0);
       if (ok) {
         fence_after();
         for (int i = 0; i < tiles; ++i) scores(i, 0);
-        commit(&bars.k_empty[0]);
+        commit(lead, &bars.k_empty[0]);
       }
       for (int j = 0; ok && j < n; ++j) {
         const int s = j % STAGES, s1 = (j + 1) % STAGES;
-        ok = mbar_wait(&bars.v_full[s], (j / STAGES) & 1, PT_SPIN);
+        ok = warp_wait(&bars.v_full[s], (j / STAGES) & 1);
         for (int i = 0; ok && i < tiles; ++i) {
-          ok = mbar_wait(&bars.p_ready[i], j & 1, PT_SPIN);
+          ok = warp_wait(&bars.p_ready[i], j & 1);
           if (!ok) break;
           fence_after();
 #pragma unroll
           for (int c = 0; c < PT_N / 16; ++c)
-            mma_ts(tmem + o_col + D * i, tmem + s_col + 128 * i + 8 * c, desc(vs + s * TILE + c * 2048, ATOM), ID_O, (j > 0) | (c > 0));
+            mma_ts(lead, tmem + o_col + D * i, tmem + s_col + 128 * i + 8 * c, desc(vs + s * TILE + c * 2048, ATOM), ID_O, (j > 0) | (c > 0));
           if (j + 1 < n) {
-            if (i == 0) ok = mbar_wait(&bars.k_full[s1], ((j + 1) / STAGES) & 1, PT_SPIN);
+            if (i == 0) ok = warp_wait(&bars.k_full[s1], ((j + 1) / STAGES) & 1);
             if (!ok) break;
             fence_after();
             scores(i, j + 1);
           } else {
-            commit(&bars.o_full[i]);
+            commit(lead, &bars.o_full[i]);
           }
         }
         if (ok) {
-          commit(&bars.v_empty[s]);
-          if (j + 1 < n) commit(&bars.k_empty[s1]);
+          commit(lead, &bars.v_empty[s]);
+          if (j + 1 < n) commit(lead, &bars.k_empty[s1]);
         }
       }
       failed = !ok;
@@ -252,9 +323,14 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
             if (!(jj < t.len && row_sees(p, t, pos, jj))) x[c] = -INFINITY;
           }
         }
-        float mx = x[0];
+        float mxs[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-        for (int c = 1; c < PT_N; ++c) mx = fmaxf(mx, x[c]);
+        for (int c = 4; c < PT_N - 4; c += 8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mxs[e] = max3(mxs[e], x[c + e], x[c + 4 + e]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mxs[e] = fmaxf(mxs[e], x[PT_N - 4 + e]);
+        float mx = fmaxf(max3(mxs[0], mxs[1], mxs[2]), mxs[3]);
         if constexpr (!MOD) mx *= p.scale_log2;  // positive: rounding keeps the order
         float factor = 1.f;
         if (mx > m + PT_LAG || (j == 0 && mx > m)) {
@@ -277,22 +353,20 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
         }
         const float z = m == -INFINITY ? 0.f : -m;
         uint32_t w[PT_N / 2];
-        float part[4] = {0.f, 0.f, 0.f, 0.f};
+        uint64_t part[2] = {pair(l, 0.f), pair(0.f, 0.f)};
+        const uint64_t z2 = pair(z, z), scale2 = pair(p.scale_log2, p.scale_log2);
 #pragma unroll
         for (int c = 0; c < PT_N; c += 2) {
-          float u, v;
-          if constexpr (MOD) {
-            u = ex2(x[c] + z);
-            v = ex2(x[c + 1] + z);
-          } else {
-            u = ex2(fmaf(x[c], p.scale_log2, z));
-            v = ex2(fmaf(x[c + 1], p.scale_log2, z));
-          }
-          part[c & 2] += u;
-          part[(c & 2) + 1] += v;
-          w[c / 2] = pack2<DT>(u, v);
+          float2 y;
+          if constexpr (MOD) y = split(add2(pair(x[c], x[c + 1]), z2));
+          else y = split(fma2(pair(x[c], x[c + 1]), scale2, z2));
+          y.x = ex2(y.x);
+          y.y = ex2(y.y);
+          part[(c >> 1) & 1] = add2(part[(c >> 1) & 1], pair(y.x, y.y));
+          w[c / 2] = pack2<DT>(y.x, y.y);
         }
-        l += (part[0] + part[1]) + (part[2] + part[3]);
+        const float2 sum = split(add2(part[0], part[1]));
+        l = sum.x + sum.y;
         st32(ts, w);
         st32(ts + 32, w + 32);
         st_wait();
@@ -332,7 +406,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
   __syncthreads();
   if (warp == PT_MMA_WARP) {
     fence_after();
-    dealloc(tmem, PT_COLS);
+    dealloc(bars.tmem, PT_COLS);
   }
   if (warp < PT_LOAD_WARP && bars.special && (warp >> 2) < tiles) {
     uint32_t redo = __ballot_sync(~0u, odd != 0.f && l == l && f < last);
@@ -340,14 +414,49 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
   }
 }
 
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &ptr, 12000, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+  });
+  return fn;
+}
+
+// A cache as [pages][slots][heads][channels] for boxes of 64 channels by one head by `box` slots of a page.
+bool encode(CUtensorMap* map, const smaq_paged_args& a, const void* cache, int box) {
+  auto fn = encode_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[4] = {cuuint64_t(a.head_dim), cuuint64_t(a.n_kv_heads), cuuint64_t(a.page_size), cuuint64_t(a.n_pages)};
+  auto bytes = [](int64_t stride, int64_t n) { return cuuint64_t(n > 1 ? stride * 2 : 16); };  // of one element: not used
+  const cuuint64_t strides[3] = {bytes(a.c_stride_h, a.n_kv_heads), bytes(a.c_stride_slot, a.page_size), bytes(a.c_stride_page, a.n_pages)};
+  for (const cuuint64_t s : strides)
+    if (s == 0 || s >= (cuuint64_t(1) << 40)) return false;
+  const cuuint32_t shape[4] = {64u, 1u, cuuint32_t(box), 1u}, step[4] = {1u, 1u, 1u, 1u};
+  return fn(map, a.dtype == SMAQ_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(cache), dims,
+            strides, shape, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <class DT, int D>
 int launch(const PagedParams& p, cudaStream_t st) {
+  PtParams pt;
+  pt.p = p;
+  const smaq_paged_args& a = p.a;
+  // boxes tile a block of 128 tokens when a page is 8 to 128 slots and divides it, or is a multiple of it
+  pt.box = a.page_size < PT_N ? a.page_size : PT_N;
+  pt.tma = a.page_size >= 8 && (a.page_size < PT_N ? PT_N % a.page_size : a.page_size % PT_N) == 0 && a.n_pages > 0 && a.n_pages < (int64_t(1) << 31) &&
+           encode(&pt.k, a, a.k_cache, pt.box) && encode(&pt.v, a, a.v_cache, pt.box);
   const bool mod = p.a.softcap > 0.f || p.a.slopes || !(p.a.scale > 0.f);
   auto kern = mod ? prefill_tc_kernel<DT, D, true> : prefill_tc_kernel<DT, D, false>;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PtCfg<D>::SMEM);
   if (e != cudaSuccess) return cuda_status(e, "paged_prefill attr");
   const int64_t tiles = (p.a.n_rows * p.group + PT_ROWS - 1) / PT_ROWS + p.a.batch;
-  kern<<<dim3(unsigned(tiles), p.a.n_kv_heads), PT_THREADS, PtCfg<D>::SMEM, st>>>(p);
+  if (tiles * a.n_kv_heads >= (int64_t(1) << 31)) return fail(SMAQ_ERR_UNSUPPORTED, "paged_prefill: too many rows");
+  kern<<<unsigned(tiles * a.n_kv_heads), PT_THREADS, PtCfg<D>::SMEM, st>>>(pt);
   return cuda_status(cudaGetLastError(), "paged_prefill");
 }
 
