@@ -90,6 +90,7 @@ __device__ __forceinline__ bool row_sees(const PagedParams& p, const PrefillTile
 // Blocks of N tokens that a tile walks: those of the prefix, then those of [lo, hi).
 struct PrefillBlocks {
   int head, jump, count;
+  PrefillBlocks() = default;
   __device__ __forceinline__ PrefillBlocks(const PrefillTile& t, int N) {
     head = (t.prefix + N - 1) / N;
     const int from = max(head, t.lo / N), to = (t.hi + N - 1) / N;

@@ -4,10 +4,12 @@
 // tokens.  For each tile and block S = Q K^T goes to tensor memory, a warpgroup turns it into weights P there, and
 // O += P V reads P from tensor memory.  The two tiles take turns: while one is in its softmax the tensor cores work for
 // the other.
-//   warps 0-3, 4-7   softmax of tile 0, 1: thread = row, so maximum and sum need no exchange;
-//   warps 8-11       copies: queries once, then keys and values (cp.async of 16 bytes through the block table, written in the
-//                    128-byte swizzled operand layout; tokens that no row sees are written as zeros);
-//   warp 12          one thread issues all products (warps 13-15 only lend their registers).
+//   warps 0-7, 8-15  softmax of tile 0, 1: a thread has one half of a row's scores; the two halves' maxima meet in shared memory.
+//                    (One thread a row needs twice the registers, so half the warps: 632 us against 589 at 8192 tokens.)
+//   warps 16-18      copies: queries once, then keys and values, whole blocks by TMA in boxes of a page, the blocks with tokens
+//                    that no row sees, and page sizes that do not fit the block, by cp.async of 16 bytes (such tokens are written
+//                    as zeros), both in the 128-byte swizzled operand layout;
+//   warp 19          issues all products.
 // Tensor memory: S0 S1 (128 columns each), O0 O1 (head_dim each); P overwrites its S.  The product for the next S of a tile is
 // issued right behind the product that reads its P, and its completion also says that O is at rest: a softmax warp may
 // then rescale O, which it does only when a row's maximum grew by more than 2^8 (the reference maximum of a row
@@ -31,10 +33,11 @@ using namespace tc5;
 
 __device__ unsigned int g_prefill_fault;
 
-constexpr int PT_THREADS = 512;
+constexpr int PT_THREADS = 640;
 constexpr int PT_N = 128;                 // tokens a block
 constexpr int PT_ROWS = 256;
-constexpr int PT_LOAD_WARP = 8, PT_MMA_WARP = 12;
+constexpr int PT_LOAD_WARP = 16, PT_MMA_WARP = 19;
+constexpr int PT_LOADERS = 32 * (PT_MMA_WARP - PT_LOAD_WARP);
 constexpr uint32_t PT_COLS = 512;
 constexpr float PT_LAG = 8.0f;            // log2
 constexpr uint32_t PT_SPIN = 1u << 24;    // polls before a wait gives up
@@ -60,13 +63,31 @@ struct PtBars {
   uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready[2], o_full[2];
   uint32_t tmem;
   int special;
+  // the tile and its walk: read from here where needed, the softmax has no registers for them
+  PrefillTile t;
+  PrefillBlocks blocks;
+  int least, most;          // first and last row's position
+  float row[2][2][2][128];  // [turn][tile][half]: row maxima, at the end row sums
+  int fail[2][4];           // a wait of one of the two warps that share rows ran out: both stop at their next meeting
 };
 
-template <class DT, int D, bool MOD>
+__device__ __forceinline__ void named_bar(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+
+enum { PT_PLAIN = 0, PT_CAP = 1, PT_ANY = 2 };  // scores: scaled by a positive factor; capped; everything else
+// Of every PT_OF pairs of weights so many come from the polynomial, the others from the special-function unit.
+#ifndef PT_POLY
+#define PT_POLY 0
+#endif
+#ifndef PT_POLY_CAP
+#define PT_POLY_CAP 2
+#endif
+constexpr int PT_OF = 4;
+
+template <class DT, int D, int MODE>
 __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_constant__ PtParams pt) {
   using T = typename DT::T;
   const PagedParams& p = pt.p;
-  constexpr int TILE = PtCfg<D>::TILE, STAGES = PtCfg<D>::STAGES, CH = D / 8, ATOM = 128 * 128;
+  constexpr int TILE = PtCfg<D>::TILE, STAGES = PtCfg<D>::STAGES, CH = D / 8, GROUP = 8 * D * 2;  // GROUP: 8 rows, 64-channel atoms side by side
   constexpr uint32_t ID_S = idesc(DT::code == SMAQ_BF16, PT_N, false), ID_O = idesc(DT::code == SMAQ_BF16, D, true);
   extern __shared__ uint8_t smem_raw[];
   __shared__ PtBars bars;
@@ -78,23 +99,37 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kvh = int(blockIdx.x % unsigned(a.n_kv_heads)), tile = int(blockIdx.x / unsigned(a.n_kv_heads));
 
   write_padding(p, kvh, tile, int(gridDim.x / unsigned(a.n_kv_heads)));
-  const PrefillTile t = find_tile<PT_THREADS>(p, tile, PT_ROWS, true, sums, found);
-  if (t.rows == 0) return;
-  const PrefillBlocks blocks(t, PT_N);
-  const int n = blocks.count, tiles = t.rows > 128 ? 2 : 1;
+  int n, tiles, last;
+  {
+    const PrefillTile t = find_tile<PT_THREADS>(p, tile, PT_ROWS, true, sums, found);
+    if (t.rows == 0) return;
+    const PrefillBlocks blocks(t, PT_N);
+    n = blocks.count;
+    tiles = t.rows > 128 ? 2 : 1;
+    last = t.f0 + t.rows;
+    if (threadIdx.x == 0) {
+      bars.t = t;
+      bars.blocks = blocks;
+      bars.least = t.past + fast_div(t.f0, p.group_div);
+      bars.most = t.past + fast_div(last - 1, p.group_div);
+    }
+  }
+  const PrefillTile& t = bars.t;
+  const PrefillBlocks& blocks = bars.blocks;
 
   if (threadIdx.x == 0) {
-    mbar_init(&bars.q_full, 128);
+    mbar_init(&bars.q_full, PT_LOADERS);
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&bars.k_full[s], 128);
-      mbar_init(&bars.v_full[s], 128);
+      mbar_init(&bars.k_full[s], PT_LOADERS);
+      mbar_init(&bars.v_full[s], PT_LOADERS);
       mbar_init(&bars.k_empty[s], 1);
       mbar_init(&bars.v_empty[s], 1);
       mbar_init(&bars.s_full[s], 1);
-      mbar_init(&bars.p_ready[s], 128);
+      mbar_init(&bars.p_ready[s], 8);
       mbar_init(&bars.o_full[s], 1);
     }
     bars.special = 0;
+    for (int i = 0; i < 8; ++i) bars.fail[i >> 2][i & 3] = 0;
     fence_mbar_init();
   }
   if (warp == PT_MMA_WARP) alloc(&bars.tmem, PT_COLS);
@@ -105,140 +140,100 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
   const uint32_t s_col = 0, o_col = 256;  // S of tile i at s_col + 128 i, O at o_col + D i
   bool failed = false;
 
-  const int last = t.f0 + t.rows;
-  const int least = t.past + fast_div(t.f0, p.group_div), most = t.past + fast_div(last - 1, p.group_div);
   auto seen_by_all = [&](int base) {
-    return base + PT_N <= t.prefix || (base + PT_N <= least + 1 && (a.window == 0 || base > most - a.window));
+    return base + PT_N <= t.prefix || (base + PT_N <= bars.least + 1 && (a.window == 0 || base > bars.most - a.window));
   };
   float odd = 0.f, l = 0.f;  // softmax threads: NaN where an output is not finite; sum of weights
   int f = 0;
 
   if (warp >= PT_LOAD_WARP) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     if (warp < PT_MMA_WARP) {
-      // ---- copies: warp w brings rows 32w .. 32w + 31 of every operand
+      // ---- copies
       const int w = warp - PT_LOAD_WARP, tid = threadIdx.x - PT_LOAD_WARP * 32;
-      for (int i = tid; i < tiles * 128 * CH; i += 128) {
+      const uint32_t lead = elect_one();
+      auto at = [&](int r, int ch) { return uint32_t((r >> 3) * GROUP + (ch >> 3) * 1024 + (r & 7) * 128 + (((ch & 7) ^ (r & 7)) << 4)); };
+      for (int i = tid; i < tiles * 128 * CH; i += PT_LOADERS) {
         const int r = i / CH, ch = i % CH, fr = t.f0 + r, tok = fast_div(fr, p.group_div);
         const bool live = r < t.rows;
         const T* src = static_cast<const T*>(a.q) + (live ? (t.first + tok) * a.q_stride_t + (kvh * p.group + fr - tok * p.group) * a.q_stride_h + ch * 8 : 0);
-        cp_async16(qs + uint32_t((r >> 7) * TILE + (ch >> 3) * ATOM + (r & 127) * 128 + (((ch & 7) ^ (r & 7)) << 4)), src, live ? 16u : 0u);
+        cp_async16(qs + at(r, ch), src, live ? 16u : 0u);
       }
       cp_async_commit();
+      cp_async_wait<0>();
+      fence_proxy_async_smem();
+      mbar_arrive(&bars.q_full);
       const int32_t* table = a.block_table + t.b * a.table_stride;
-      auto look_up = [&](int k) {
-        if (k >= n) return int64_t(-1);
-        const int j = blocks.base(k, PT_N) + 32 * w + lane;
-        return tile_sees(t, j) ? token_offset(p, table, j) + kvh * a.c_stride_h : int64_t(-1);
+      // Blocks whose every token is seen by some row come by TMA, in boxes of one page (or 128 slots of it), the warps in
+      // turn.  (Issued by the lanes of one warp side by side, boxes cost about 150 cycles each, 5000 a block.)
+      const int per = PT_N / pt.box;
+      auto whole = [&](int k) {
+        const int b = blocks.base(k, PT_N);
+        return pt.tma && (b + PT_N <= t.prefix || (b >= t.lo && b + PT_N <= t.hi));
       };
-      auto bring = [&](const void* cache, uint32_t dst, int64_t off) {
-        constexpr int PER = 32 / CH;  // rows a pass
-#pragma unroll
-        for (int i = 0; i < 32 / PER; ++i) {
-          const int rr = i * PER + lane / CH, ch = lane % CH, r = 32 * w + rr;
-          const int64_t o = __shfl_sync(~0u, off, rr);
-          cp_async16(dst + uint32_t((ch >> 3) * ATOM + r * 128 + (((ch & 7) ^ (r & 7)) << 4)),
-                     static_cast<const T*>(cache) + (o < 0 ? 0 : o) + ch * 8, o < 0 ? 0u : 16u);
-        }
-        cp_async_commit();
+      auto page_of = [&](int k) {
+        if (k >= n || lane >= per || !whole(k)) return 0;
+        const int64_t blk = fast_div(blocks.base(k, PT_N) + lane * pt.box, p.page_div);
+        return int(min(max(int64_t(__ldg(table + blk)), int64_t(0)), a.n_pages - 1));
       };
-      // copy g = 2 j brings keys of block j, 2 j + 1 its values; a copy is announced two copies later
-      // values of a block that some rows see in part: look for infinities and NaN where this thread copies
+      // Blocks that come by cp.async: warp w brings rows r0 .. r0 + rows of every operand.
+      const int r0 = w * 43, rows = min(43, PT_N - r0);
+      // values of a block that some rows see in part: look for infinities and NaN in this warp's rows
       auto look_for_special = [&](int s) {
         bool odd_value = false;
-        constexpr int PER = 32 / CH;
-        for (int i = 0; i < 32 / PER; ++i) {
-          const int ch = lane % CH, r = 32 * w + i * PER + lane / CH;
-          odd_value |= any_special<DT>(*reinterpret_cast<const uint4*>(smem + (vs - qs) + s * TILE + (ch >> 3) * ATOM + r * 128 + (((ch & 7) ^ (r & 7)) << 4)));
-        }
+        for (int i = lane; i < rows * CH; i += 32) odd_value |= any_special<DT>(*reinterpret_cast<const uint4*>(smem + (vs - qs) + s * TILE + at(r0 + i / CH, i % CH)));
         if (odd_value) bars.special = 1;
       };
-      auto announce = [&](int g) {
-        const int j = g >> 1, s = j % STAGES;
-        if ((g & 1) && !seen_by_all(blocks.base(j, PT_N))) look_for_special(s);
-        fence_proxy_async_smem();
-        mbar_arrive((g & 1) ? &bars.v_full[s] : &bars.k_full[s]);
-      };
-      if (pt.tma) {
-        // A block whose every token is seen by some row comes in boxes of one page (or 128 slots of it) by 64
-        // channels, a lane of warp 0 each; the others as below, announced at once.
-        const int per = PT_N / pt.box, boxes = per * (D / 64);
-        auto whole = [&](int k) {
-          const int b = blocks.base(k, PT_N);
-          return b + PT_N <= t.prefix || (b >= t.lo && b + PT_N <= t.hi);
-        };
-        auto page_of = [&](int k) {
-          if (k >= n || lane >= boxes || !whole(k)) return 0;
-          const int64_t blk = fast_div(blocks.base(k, PT_N) + (lane % per) * pt.box, p.page_div);
-          return int(min(max(int64_t(__ldg(table + blk)), int64_t(0)), a.n_pages - 1));
-        };
-        auto fetch = [&](int j, int s, bool values, int page, int64_t off) {
-          uint64_t* bar = values ? &bars.v_full[s] : &bars.k_full[s];
-          const uint32_t dst = (values ? vs : ks) + s * TILE;
-          if (whole(j)) {
-            if (w == 0) {
-              if (lane == 0) mbar_arrive_expect_tx(bar, TILE);
-              __syncwarp();
-              if (lane < boxes) {
-                const int half = lane / per, b = lane % per, slot = blocks.base(j, PT_N) + b * pt.box;
-                tma_4d(dst + half * ATOM + b * pt.box * 128, values ? &pt.v : &pt.k, half * 64, kvh, slot - fast_div(slot, p.page_div) * a.page_size, page, bar);
-              }
-              if (lane != 0) mbar_arrive(bar);
-            } else {
-              mbar_arrive(bar);
-            }
-            if (values && !seen_by_all(blocks.base(j, PT_N))) {
-              if (!warp_wait(bar, (j / STAGES) & 1)) failed = true;
-              look_for_special(s);
-              fence_proxy_async_smem();  // before the stage is filled again
-            }
-            return;
+      auto fetch = [&](int j, int s, bool values, int page) {
+        uint64_t* bar = values ? &bars.v_full[s] : &bars.k_full[s];
+        const uint32_t dst = (values ? vs : ks) + s * TILE;
+        const bool part = values && !seen_by_all(blocks.base(j, PT_N));
+        if (whole(j)) {
+          if (tid == 0) mbar_arrive_expect_tx(bar, TILE);
+          const int first = blocks.base(j, PT_N), slot = per > 1 ? 0 : first - fast_div(first, p.page_div) * a.page_size;
+          for (int b = w; b < per; b += PT_MMA_WARP - PT_LOAD_WARP)
+            tma_5d(lead, dst + b * pt.box * (D * 2), values ? &pt.v : &pt.k, kvh * int(a.c_stride_h), 0, 0, slot >> 3, __shfl_sync(~0u, page, b), bar);
+          if (tid != 0) mbar_arrive(bar);
+          if (part) {
+            if (!warp_wait(bar, (j / STAGES) & 1)) failed = true;
+            look_for_special(s);
+            fence_proxy_async_smem();  // before the stage is filled again
           }
-          bring(values ? a.v_cache : a.k_cache, dst, off);
-          cp_async_wait<0>();
-          announce(2 * j + values);
-        };
-        cp_async_wait<0>();
-        fence_proxy_async_smem();
-        mbar_arrive(&bars.q_full);
-        int page = page_of(0);
-        for (int j = 0; j < n; ++j) {
-          const int s = j % STAGES;
-          const uint32_t ph = uint32_t((j / STAGES) & 1) ^ 1u;
-          const int next = page_of(j + 1);
-          const int64_t off = whole(j) ? 0 : look_up(j);
-          if (!warp_wait(&bars.k_empty[s], ph)) { failed = true; break; }
-          fetch(j, s, false, page, off);
-          if (!warp_wait(&bars.v_empty[s], ph)) { failed = true; break; }
-          fetch(j, s, true, page, off);
-          if (failed) break;
-          page = next;
+          return;
         }
-      }
-      int64_t off = pt.tma ? -1 : look_up(0);
-      for (int j = 0; j < n && !failed && !pt.tma; ++j) {
+        const T* cache = static_cast<const T*>(values ? a.v_cache : a.k_cache);
+        auto offset = [&](int r) {
+          const int tok = blocks.base(j, PT_N) + r0 + r;
+          return r < rows && tile_sees(t, tok) ? token_offset(p, table, tok) + kvh * a.c_stride_h : int64_t(-1);
+        };
+        const int64_t off0 = offset(lane), off1 = offset(lane + 32);
+#pragma unroll 4
+        for (int i0 = 0; i0 < 44 * CH; i0 += 32) {
+          const int r = (i0 + lane) / CH, ch = (i0 + lane) % CH;
+          const int64_t lo = __shfl_sync(~0u, off0, r & 31), hi = __shfl_sync(~0u, off1, r & 31);
+          const int64_t off = r < 32 ? lo : hi;
+          if (r < rows) cp_async16(dst + at(r0 + r, ch), cache + (off < 0 ? 0 : off) + ch * 8, off < 0 ? 0u : 16u);
+        }
+        cp_async_commit();
+        cp_async_wait<0>();
+        if (part) {
+          __syncwarp();  // the other lanes' copies too
+          look_for_special(s);
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(bar);
+      };
+      int page = page_of(0);
+      for (int j = 0; j < n; ++j) {
         const int s = j % STAGES;
         const uint32_t ph = uint32_t((j / STAGES) & 1) ^ 1u;
-        const int64_t next = look_up(j + 1);
+        const int next = page_of(j + 1);
         if (!warp_wait(&bars.k_empty[s], ph)) { failed = true; break; }
-        bring(a.k_cache, ks + s * TILE, off);
-        cp_async_wait<2>();
-        if (j > 0) announce(2 * j - 2);
+        fetch(j, s, false, page);
         if (!warp_wait(&bars.v_empty[s], ph)) { failed = true; break; }
-        bring(a.v_cache, vs + s * TILE, off);
-        cp_async_wait<2>();
-        if (j == 0) {  // the queries were the group before the first keys
-          fence_proxy_async_smem();
-          mbar_arrive(&bars.q_full);
-        } else {
-          announce(2 * j - 1);
-        }
-        off = next;
-      }
-      cp_async_wait<0>();
-      if (!failed && n > 0 && !pt.tma) {
-        announce(2 * n - 2);
-        announce(2 * n - 1);
+        fetch(j, s, true, page);
+        if (failed) break;
+        page = next;
       }
     } else if (warp == PT_MMA_WARP && n > 0) {
       // ---- products
@@ -247,8 +242,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
         const uint32_t q = qs + i * TILE, k = ks + (j % STAGES) * TILE;
 #pragma unroll
         for (int c = 0; c < D / 16; ++c) {
-          const uint32_t at = uint32_t((c >> 2) * ATOM + (c & 3) * 32);
-          mma_ss(lead, tmem + s_col + 128 * i, desc(q + at, 16), desc(k + at, 16), ID_S, c > 0);
+          const uint32_t at = uint32_t((c >> 2) * 1024 + (c & 3) * 32);
+          mma_ss(lead, tmem + s_col + 128 * i, desc(q + at, GROUP, 16), desc(k + at, GROUP, 16), ID_S, c > 0);
         }
         commit(lead, &bars.s_full[i]);
       };
@@ -267,7 +262,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
           fence_after();
 #pragma unroll
           for (int c = 0; c < PT_N / 16; ++c)
-            mma_ts(lead, tmem + o_col + D * i, tmem + s_col + 128 * i + 8 * c, desc(vs + s * TILE + c * 2048, ATOM), ID_O, (j > 0) | (c > 0));
+            mma_ts(lead, tmem + o_col + D * i, tmem + s_col + 128 * i + 64 * (c >> 2) + 8 * (c & 3), desc(vs + s * TILE + c * 2 * GROUP, GROUP, 1024), ID_O, (j > 0) | (c > 0));
           if (j + 1 < n) {
             if (i == 0) ok = warp_wait(&bars.k_full[s1], ((j + 1) / STAGES) & 1);
             if (!ok) break;
@@ -285,53 +280,88 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
       failed = !ok;
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
-    const int i = warp >> 2;  // tile
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    constexpr int C = PT_N / 2;                   // columns a thread
+    const int i = warp >> 3, half = (warp >> 2) & 1;  // tile, half of the columns
     if (i < tiles) {
-      const int row = threadIdx.x & 127;
+      const int row = 32 * (warp & 3) + lane, meet = 2 + i * 4 + (warp & 3);  // barrier of the two warps that share these rows
       f = t.f0 + 128 * i + row;
       const int tok = fast_div(f, p.group_div), h = kvh * p.group + f - tok * p.group, pos = t.past + tok;
       const float slope = a.slopes && f < last ? a.slopes[h] * kLog2e : 0.f;
       const uint32_t lanes = uint32_t(32 * (warp & 3)) << 16;
-      const uint32_t ts = tmem + lanes + s_col + 128 * i, to = tmem + lanes + o_col + D * i;
+      const uint32_t ts = tmem + lanes + s_col + 128 * i, to = tmem + lanes + o_col + D * i + half * (D / 2);
       float m = -INFINITY;  // reference maximum of the row, log2
       for (int j = 0; j < n; ++j) {
-        if (!warp_wait(&bars.s_full[i], j & 1)) { failed = true; break; }
+        if (!warp_wait(&bars.s_full[i], j & 1)) bars.fail[i][warp & 3] = 1;
         fence_after();
-        float x[PT_N];
+        // Two passes over the scores, 32 columns at a time, so that they need not stay in registers: the first
+        // finds the maximum and puts capped, biased or masked scores back, the second makes the weights.
+        const int base = blocks.base(j, PT_N) + half * C;
+        const bool part = !seen_by_all(base - half * C);
+        float mx = -INFINITY;
 #pragma unroll
-        for (int c = 0; c < PT_N / 32; ++c) ld32(ts + 32 * c, reinterpret_cast<uint32_t*>(x) + 32 * c);
-        ld_wait();
-        const int base = blocks.base(j, PT_N);
-        if constexpr (MOD) {
-          if (p.a.softcap > 0.f) {
+        for (int q = 0; q < C / 32; ++q) {
+          float x[32];
+          ld32(ts + half * C + 32 * q, reinterpret_cast<uint32_t*>(x));
+          ld_wait();
+          const int b = base + 32 * q;
+          if constexpr (MODE == PT_CAP) {
+            const uint64_t in2 = pair(p.cap_in, p.cap_in), out2 = pair(-2.0f * p.cap_log2, -2.0f * p.cap_log2), cap2 = pair(p.cap_log2, p.cap_log2);
 #pragma unroll
-            for (int c = 0; c < PT_N; ++c) x[c] = score_log2<true>(x[c], p);
-          } else {
+            for (int c = 0; c < 32; c += 2) {  // cap tanh, as score_log2
+              float2 y = split(mul2(pair(x[c], x[c + 1]), in2));
+              if ((c >> 1) % PT_OF < PT_POLY_CAP) {
+                asm("min.NaN.f32 %0, %0, %1;" : "+f"(y.x) : "f"(126.0f));
+                asm("min.NaN.f32 %0, %0, %1;" : "+f"(y.y) : "f"(126.0f));
+                y = split(exp2_poly<5>(pair(y.x, y.y)));
+              } else {
+                y.x = ex2(y.x);
+                y.y = ex2(y.y);
+              }
+              y = split(add2(pair(y.x, y.y), pair(1.0f, 1.0f)));
+              y = split(fma2(pair(rcp_approx(y.x), rcp_approx(y.y)), out2, cap2));
+              x[c] = y.x;
+              x[c + 1] = y.y;
+            }
+          } else if constexpr (MODE == PT_ANY) {
+            if (p.a.softcap > 0.f) {
 #pragma unroll
-            for (int c = 0; c < PT_N; ++c) x[c] *= p.scale_log2;
+              for (int c = 0; c < 32; ++c) x[c] = score_log2<true>(x[c], p);
+            } else {
+#pragma unroll
+              for (int c = 0; c < 32; ++c) x[c] *= p.scale_log2;
+            }
+            if (a.slopes) {
+#pragma unroll
+              for (int c = 0; c < 32; ++c) x[c] -= slope * fabsf(float(pos - b - c));
+            }
           }
-          if (a.slopes) {
+          if (part) {
+            const int upper = min(pos + 1, t.len) - b;
+            if (t.prefix <= base && (a.window == 0 || base - half * C > bars.most - a.window)) {  // cut by the row's own position alone
 #pragma unroll
-            for (int c = 0; c < PT_N; ++c) x[c] -= slope * fabsf(float(pos - base - c));
+              for (int c = 0; c < 32; ++c) x[c] = c < upper ? x[c] : -INFINITY;
+            } else {
+              const int lower = a.window ? pos - a.window + 1 - b : 0, pre = t.prefix - b;
+#pragma unroll
+              for (int c = 0; c < 32; ++c) x[c] = c < pre || (c >= lower && c < upper) ? x[c] : -INFINITY;
+            }
           }
+          if (MODE != PT_PLAIN || part) st32(ts + half * C + 32 * q, reinterpret_cast<const uint32_t*>(x));
+          float mxs[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+          for (int c = 4; c < 28; c += 8)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mxs[e] = max3(mxs[e], x[c + e], x[c + 4 + e]);
+          mx = max3(mx, max3(mxs[0], mxs[1], mxs[2]), max3(mxs[3], x[28], x[29]));
+          mx = max3(mx, x[30], x[31]);
         }
-        if (!seen_by_all(base)) {
-#pragma unroll
-          for (int c = 0; c < PT_N; ++c) {
-            const int jj = base + c;
-            if (!(jj < t.len && row_sees(p, t, pos, jj))) x[c] = -INFINITY;
-          }
-        }
-        float mxs[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-        for (int c = 4; c < PT_N - 4; c += 8)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) mxs[e] = max3(mxs[e], x[c + e], x[c + 4 + e]);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) mxs[e] = fmaxf(mxs[e], x[PT_N - 4 + e]);
-        float mx = fmaxf(max3(mxs[0], mxs[1], mxs[2]), mxs[3]);
-        if constexpr (!MOD) mx *= p.scale_log2;  // positive: rounding keeps the order
+        if constexpr (MODE == PT_PLAIN) mx *= p.scale_log2;  // positive: rounding keeps the order
+        if (MODE != PT_PLAIN || part) st_wait();
+        bars.row[j & 1][i][half][row] = mx;
+        named_bar(meet, 64);
+        mx = fmaxf(mx, bars.row[j & 1][i][half ^ 1][row]);
+        if (*reinterpret_cast<volatile int*>(&bars.fail[i][warp & 3])) { failed = true; break; }
         float factor = 1.f;
         if (mx > m + PT_LAG || (j == 0 && mx > m)) {
           factor = m == -INFINITY ? 0.f : ex2(m - mx);
@@ -341,7 +371,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
           l *= factor;
           if (j > 0) {
 #pragma unroll
-            for (int c = 0; c < D / 32; ++c) {
+            for (int c = 0; c < D / 64; ++c) {
               uint32_t o[32];
               ld32(to + 32 * c, o);
               ld_wait();
@@ -352,33 +382,48 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
           }
         }
         const float z = m == -INFINITY ? 0.f : -m;
-        uint32_t w[PT_N / 2];
-        uint64_t part[2] = {pair(l, 0.f), pair(0.f, 0.f)};
+        uint64_t part2[2] = {pair(l, 0.f), pair(0.f, 0.f)};
         const uint64_t z2 = pair(z, z), scale2 = pair(p.scale_log2, p.scale_log2);
 #pragma unroll
-        for (int c = 0; c < PT_N; c += 2) {
-          float2 y;
-          if constexpr (MOD) y = split(add2(pair(x[c], x[c + 1]), z2));
-          else y = split(fma2(pair(x[c], x[c + 1]), scale2, z2));
-          y.x = ex2(y.x);
-          y.y = ex2(y.y);
-          part[(c >> 1) & 1] = add2(part[(c >> 1) & 1], pair(y.x, y.y));
-          w[c / 2] = pack2<DT>(y.x, y.y);
+        for (int q = 0; q < C / 32; ++q) {
+          float x[32];
+          uint32_t w[16];
+          ld32(ts + half * C + 32 * q, reinterpret_cast<uint32_t*>(x));
+          ld_wait();
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) {
+            constexpr int POLY = MODE == PT_CAP ? PT_OF : PT_POLY;
+            uint64_t y2;
+            if constexpr (MODE == PT_PLAIN) y2 = fma2(pair(x[c], x[c + 1]), scale2, z2);
+            else y2 = add2(pair(x[c], x[c + 1]), z2);
+            float2 y = split(y2);
+            if ((c >> 1) % PT_OF < POLY) {
+              y = split(exp2_poly<4>(y2));
+            } else {
+              y.x = ex2(y.x);
+              y.y = ex2(y.y);
+            }
+            part2[(c >> 1) & 1] = add2(part2[(c >> 1) & 1], pair(y.x, y.y));
+            w[c / 2] = pack2<DT>(y.x, y.y);
+          }
+          st16(ts + half * C + 16 * q, w);  // over scores that this thread has read
         }
-        const float2 sum = split(add2(part[0], part[1]));
+        const float2 sum = split(add2(part2[0], part2[1]));
         l = sum.x + sum.y;
-        st32(ts, w);
-        st32(ts + 32, w + 32);
         st_wait();
         fence_before();
-        mbar_arrive(&bars.p_ready[i]);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&bars.p_ready[i]);
       }
       if (n > 0 && !failed && !warp_wait(&bars.o_full[i], 0)) failed = true;
       fence_after();
+      bars.row[n & 1][i][half][row] = l;
+      named_bar(meet, 64);
+      l += bars.row[n & 1][i][half ^ 1][row];
       const float inv = l == 0.f ? 0.f : 1.0f / l;
-      T* out = static_cast<T*>(a.out) + int64_t(t.first + tok) * a.o_stride_t + h * a.o_stride_h;
+      T* out = static_cast<T*>(a.out) + int64_t(t.first + tok) * a.o_stride_t + h * a.o_stride_h + half * (D / 2);
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
+      for (int c = 0; c < D / 64; ++c) {
         uint32_t o[32], w[16];
         if (n > 0) {
           ld32(to + 32 * c, o);
@@ -398,7 +443,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
           for (int e = 0; e < 4; ++e) reinterpret_cast<uint4*>(out + 32 * c)[e] = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
         }
       }
-      if (a.lse && f < last) a.lse[int64_t(t.first + tok) * a.n_q_heads + h] = (m + log2f(l)) * kLn2;
+      if (a.lse && half == 0 && f < last) a.lse[int64_t(t.first + tok) * a.n_q_heads + h] = (m + log2f(l)) * kLn2;
     }
   }
   if (failed) atomicOr(&g_prefill_fault, 1u);
@@ -408,7 +453,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
     fence_after();
     dealloc(bars.tmem, PT_COLS);
   }
-  if (warp < PT_LOAD_WARP && bars.special && (warp >> 2) < tiles) {
+  if (warp < PT_LOAD_WARP && bars.special && (warp >> 3) < tiles) {
     uint32_t redo = __ballot_sync(~0u, odd != 0.f && l == l && f < last);
     for (; redo; redo &= redo - 1) exact_row(p, t, kvh, __shfl_sync(~0u, f, __ffs(redo) - 1));
   }
@@ -426,17 +471,20 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
-// A cache as [pages][slots][heads][channels] for boxes of 64 channels by one head by `box` slots of a page.
+// A cache for boxes of `box` slots of a page by one head: channels of all heads in a row (a head begins at kvh *
+// stride), eight slots, the 64-channel parts of a head, groups of eight slots, pages.  A box lands as it is
+// multiplied: 8-row atoms, the parts of a head side by side.
 bool encode(CUtensorMap* map, const smaq_paged_args& a, const void* cache, int box) {
   auto fn = encode_fn();
   if (!fn) return false;
-  const cuuint64_t dims[4] = {cuuint64_t(a.head_dim), cuuint64_t(a.n_kv_heads), cuuint64_t(a.page_size), cuuint64_t(a.n_pages)};
-  auto bytes = [](int64_t stride, int64_t n) { return cuuint64_t(n > 1 ? stride * 2 : 16); };  // of one element: not used
-  const cuuint64_t strides[3] = {bytes(a.c_stride_h, a.n_kv_heads), bytes(a.c_stride_slot, a.page_size), bytes(a.c_stride_page, a.n_pages)};
+  const int64_t row = (a.n_kv_heads - 1) * a.c_stride_h + 64;
+  if (row < 64 || row >= (int64_t(1) << 31) || a.c_stride_slot <= 0 || (a.n_pages > 1 && a.c_stride_page <= 0)) return false;
+  const cuuint64_t dims[5] = {cuuint64_t(row), 8, cuuint64_t(a.head_dim / 64), cuuint64_t(a.page_size / 8), cuuint64_t(a.n_pages)};
+  const cuuint64_t strides[4] = {cuuint64_t(a.c_stride_slot) * 2, 128, cuuint64_t(a.c_stride_slot) * 16, cuuint64_t(a.n_pages > 1 ? a.c_stride_page * 2 : 16)};
   for (const cuuint64_t s : strides)
-    if (s == 0 || s >= (cuuint64_t(1) << 40)) return false;
-  const cuuint32_t shape[4] = {64u, 1u, cuuint32_t(box), 1u}, step[4] = {1u, 1u, 1u, 1u};
-  return fn(map, a.dtype == SMAQ_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(cache), dims,
+    if (s >= (cuuint64_t(1) << 40)) return false;
+  const cuuint32_t shape[5] = {64u, 8u, cuuint32_t(a.head_dim / 64), cuuint32_t(box / 8), 1u}, step[5] = {1u, 1u, 1u, 1u, 1u};
+  return fn(map, a.dtype == SMAQ_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, const_cast<void*>(cache), dims,
             strides, shape, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -449,9 +497,10 @@ int launch(const PagedParams& p, cudaStream_t st) {
   // boxes tile a block of 128 tokens when a page is 8 to 128 slots and divides it, or is a multiple of it
   pt.box = a.page_size < PT_N ? a.page_size : PT_N;
   pt.tma = a.page_size >= 8 && (a.page_size < PT_N ? PT_N % a.page_size : a.page_size % PT_N) == 0 && a.n_pages > 0 && a.n_pages < (int64_t(1) << 31) &&
-           encode(&pt.k, a, a.k_cache, pt.box) && encode(&pt.v, a, a.v_cache, pt.box);
-  const bool mod = p.a.softcap > 0.f || p.a.slopes || !(p.a.scale > 0.f);
-  auto kern = mod ? prefill_tc_kernel<DT, D, true> : prefill_tc_kernel<DT, D, false>;
+           a.n_kv_heads * a.c_stride_h < (int64_t(1) << 31) && encode(&pt.k, a, a.k_cache, pt.box) && encode(&pt.v, a, a.v_cache, pt.box);
+  auto kern = a.slopes || !(a.scale > 0.f) ? prefill_tc_kernel<DT, D, PT_ANY>
+              : a.softcap > 0.f            ? prefill_tc_kernel<DT, D, PT_CAP>
+                                           : prefill_tc_kernel<DT, D, PT_PLAIN>;
   const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PtCfg<D>::SMEM);
   if (e != cudaSuccess) return cuda_status(e, "paged_prefill attr");
   const int64_t tiles = (p.a.n_rows * p.group + PT_ROWS - 1) / PT_ROWS + p.a.batch;

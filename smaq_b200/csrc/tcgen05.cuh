@@ -18,13 +18,11 @@ __device__ __forceinline__ void dealloc(uint32_t tmem, uint32_t cols) {
   asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(cols) : "memory");
 }
 
-// Shared-memory operand in 128-byte swizzled atoms of 64 16-bit elements by 8 rows (1024 bytes).  K-major (64
-// elements of the contraction a row): rows of atoms 1024 bytes apart (stride field).  MN-major (64 output elements a
-// row, one row a contraction index): groups of 8 contraction indices 1024 bytes apart (stride field), the next 64
-// output elements `next` bytes on (leading field).
-__device__ __forceinline__ uint64_t desc(uint32_t saddr, uint32_t next) {
-  return uint64_t((saddr & 0x3FFFFu) >> 4) | (uint64_t(next >> 4) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) |
-         (uint64_t(2) << 61);
+// Shared-memory operand in 128-byte swizzled atoms: 8 rows of 128 bytes (64 16-bit elements), 1024 bytes.  `group`: bytes from
+// one 8-row group to the next.  K-major: rows are output rows, 64 contraction elements each.  MN-major: rows are
+// contraction indices, 64 output elements each, and `next` is the way to the next 64 output elements.
+__device__ __forceinline__ uint64_t desc(uint32_t saddr, uint32_t group, uint32_t next) {
+  return uint64_t((saddr & 0x3FFFFu) >> 4) | (uint64_t(next >> 4) << 16) | (uint64_t(group >> 4) << 32) | (uint64_t(1) << 46) | (uint64_t(2) << 61);
 }
 // kind::f16 instruction descriptor: fp32 accumulators, both operands bf16 or fp16, M = 128; B K-major or MN-major.
 constexpr uint32_t idesc(bool bf16, uint32_t n, bool b_mn_major) {
@@ -85,13 +83,21 @@ __device__ __forceinline__ void st32(uint32_t taddr, const uint32_t* r) {
       "r"(r[31])
       : "memory");
 }
+__device__ __forceinline__ void st16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]),
+      "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
 __device__ __forceinline__ void st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Box of a 4-D tensor map to shared memory (no multicast).
-__device__ __forceinline__ void tma_4d(uint32_t dst, const void* map, int x, int y, int z, int w, uint64_t* bar) {
+// Box of a 5-D tensor map to shared memory (no multicast), issued by the lane with `lead`.
+__device__ __forceinline__ void tma_5d(uint32_t lead, uint32_t dst, const void* map, int c0, int c1, int c2, int c3, int c4, uint64_t* bar) {
   asm volatile(
-      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(smem_u32(bar))
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %8, 0;\n\t"
+      "@q cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];\n\t}" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4), "r"(smem_u32(bar)), "r"(lead)
       : "memory");
 }
 
@@ -125,6 +131,36 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
   float r;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
   return r;
+}
+
+// 2^x for two x <= 126 on the FMA pipes, whose throughput the special-function unit's exponential lacks: x = n + r
+// with n the nearest integer (added to 1.5 2^23 + 127, whose low bits then hold n + 127), 2^n from those bits, 2^r
+// by a polynomial with p(0) = 1 of least relative error on [-1/2, 1/2] (fitted by linear programming on
+// Chebyshev points): 2.9e-6 for degree 4, 1.9e-7 for 5.  x below -126.5 gives 0 exactly, -infinity
+// too; NaN stays NaN.
+template <int DEG>
+__device__ __forceinline__ uint64_t exp2_poly(uint64_t x) {
+  float2 v = split(x);
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(v.x) : "f"(-127.0f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(v.y) : "f"(-127.0f));
+  constexpr float kMagic = 12582912.0f + 127.0f;
+  x = pair(v.x, v.y);
+  const uint64_t t = add2(x, pair(kMagic, kMagic));
+  const uint64_t r = fma2(add2(t, pair(-kMagic, -kMagic)), pair(-1.0f, -1.0f), x);
+  uint64_t y;
+  if constexpr (DEG == 4) {
+    y = fma2(pair(0.009582852944731712f, 0.009582852944731712f), r, pair(0.055906426161527634f, 0.055906426161527634f));
+    y = fma2(y, r, pair(0.24024099111557007f, 0.24024099111557007f));
+    y = fma2(y, r, pair(0.6931241750717163f, 0.6931241750717163f));
+  } else {
+    y = fma2(pair(0.001326465280726552f, 0.001326465280726552f), r, pair(0.009671511128544807f, 0.009671511128544807f));
+    y = fma2(y, r, pair(0.05550733953714371f, 0.05550733953714371f));
+    y = fma2(y, r, pair(0.24022242426872253f, 0.24022242426872253f));
+    y = fma2(y, r, pair(0.6931470036506653f, 0.6931470036506653f));
+  }
+  y = fma2(y, r, pair(1.0f, 1.0f));
+  const float2 n = split(t);
+  return mul2(y, pair(__uint_as_float(__float_as_uint(n.x) << 23), __uint_as_float(__float_as_uint(n.y) << 23)));
 }
 
 }  // namespace tc5
