@@ -4,8 +4,10 @@
 // tokens.  For each tile and block S = Q K^T goes to tensor memory, a warpgroup turns it into weights P there, and
 // O += P V reads P from tensor memory.  The two tiles take turns: while one is in its softmax the tensor cores work for
 // the other.
-//   warps 0-7, 8-15  softmax of tile 0, 1: a thread has one half of a row's scores; the two halves' maxima meet in shared memory.
-//                    (One thread a row needs twice the registers, so half the warps: 632 us against 589 at 8192 tokens.)
+//   warps 0-7, 8-15  softmax of tile 0, 1: a thread has one half of a row's scores and goes over them twice, 32 columns at a time
+//                    (maximum, weights); the halves' maxima meet in shared memory.  (One thread a row with its 128 scores in
+//                    registers has half the warps to hide latencies with: 541 us against 539 at 8192 tokens, 728 against 712
+//                    capped.)
 //   warps 16-18      copies: queries once, then keys and values, whole blocks by TMA in boxes of a page, the blocks with tokens
 //                    that no row sees, and page sizes that do not fit the block, by cp.async of 16 bytes (such tokens are written
 //                    as zeros), both in the 128-byte swizzled operand layout;
@@ -33,10 +35,12 @@ using namespace tc5;
 
 __device__ unsigned int g_prefill_fault;
 
-constexpr int PT_THREADS = 640;
+constexpr int PT_SPLIT = 2;               // softmax threads a row
+constexpr int PT_TW = 4 * PT_SPLIT;       // softmax warps a tile
+constexpr int PT_THREADS = 32 * (2 * PT_TW + 4);
 constexpr int PT_N = 128;                 // tokens a block
 constexpr int PT_ROWS = 256;
-constexpr int PT_LOAD_WARP = 16, PT_MMA_WARP = 19;
+constexpr int PT_LOAD_WARP = 2 * PT_TW, PT_MMA_WARP = PT_LOAD_WARP + 3;
 constexpr int PT_LOADERS = 32 * (PT_MMA_WARP - PT_LOAD_WARP);
 constexpr uint32_t PT_COLS = 512;
 constexpr float PT_LAG = 8.0f;            // log2
@@ -74,14 +78,30 @@ struct PtBars {
 __device__ __forceinline__ void named_bar(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
 enum { PT_PLAIN = 0, PT_CAP = 1, PT_ANY = 2 };  // scores: scaled by a positive factor; capped; everything else
-// Of every PT_OF pairs of weights so many come from the polynomial, the others from the special-function unit.
-#ifndef PT_POLY
-#define PT_POLY 0
-#endif
-#ifndef PT_POLY_CAP
-#define PT_POLY_CAP 2
-#endif
-constexpr int PT_OF = 4;
+// Of every PT_OF pairs of exponentials so many come from the polynomial, the others from the special-function unit,
+// which alone would need as long as the products.  At 8192 tokens and 32/8 heads 0, 1, 2, 3 of 8 took 578, 539, 557,
+// 558 us; a capped score takes two exponentials and a reciprocal: (4, 2), (2, 2), (6, 2), (4, 4) of 8 for (tanh, weight)
+// took 712, 725, 726, 735 us on chunks of 64/8 heads behind 8K tokens.
+constexpr int PT_POLY = 1, PT_POLY_CAP = 4, PT_POLY_EXP = 2;
+constexpr int PT_OF = 8;
+
+// 2^x of PT_OF pairs, POLY of them by the polynomial.
+template <int DEG, int POLY>
+__device__ __forceinline__ void exp2_group(uint64_t (&x)[PT_OF]) {
+  if constexpr (POLY > 0) {
+    uint64_t y[POLY];
+#pragma unroll
+    for (int i = 0; i < POLY; ++i) y[i] = x[i];
+    exp2_poly<DEG>(y);
+#pragma unroll
+    for (int i = 0; i < POLY; ++i) x[i] = y[i];
+  }
+#pragma unroll
+  for (int i = POLY; i < PT_OF; ++i) {
+    const float2 v = split(x[i]);
+    x[i] = pair(ex2(v.x), ex2(v.y));
+  }
+}
 
 template <class DT, int D, int MODE>
 __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_constant__ PtParams pt) {
@@ -125,7 +145,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
       mbar_init(&bars.k_empty[s], 1);
       mbar_init(&bars.v_empty[s], 1);
       mbar_init(&bars.s_full[s], 1);
-      mbar_init(&bars.p_ready[s], 8);
+      mbar_init(&bars.p_ready[s], PT_TW);
       mbar_init(&bars.o_full[s], 1);
     }
     bars.special = 0;
@@ -147,7 +167,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
   int f = 0;
 
   if (warp >= PT_LOAD_WARP) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");  // 128 x 64 + 512 x 104 = 640 x 96, the launch's
     if (warp < PT_MMA_WARP) {
       // ---- copies
       const int w = warp - PT_LOAD_WARP, tid = threadIdx.x - PT_LOAD_WARP * 32;
@@ -281,47 +301,53 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
-    constexpr int C = PT_N / 2;                   // columns a thread
-    const int i = warp >> 3, half = (warp >> 2) & 1;  // tile, half of the columns
+    constexpr int C = PT_N / PT_SPLIT;                  // columns a thread
+    const int i = warp / PT_TW, half = (warp >> 2) & 1;  // tile, half of the columns
     if (i < tiles) {
       const int row = 32 * (warp & 3) + lane, meet = 2 + i * 4 + (warp & 3);  // barrier of the two warps that share these rows
       f = t.f0 + 128 * i + row;
       const int tok = fast_div(f, p.group_div), h = kvh * p.group + f - tok * p.group, pos = t.past + tok;
       const float slope = a.slopes && f < last ? a.slopes[h] * kLog2e : 0.f;
       const uint32_t lanes = uint32_t(32 * (warp & 3)) << 16;
-      const uint32_t ts = tmem + lanes + s_col + 128 * i, to = tmem + lanes + o_col + D * i + half * (D / 2);
+      const uint32_t ts = tmem + lanes + s_col + 128 * i, to = tmem + lanes + o_col + D * i + half * (D / PT_SPLIT);
       float m = -INFINITY;  // reference maximum of the row, log2
       for (int j = 0; j < n; ++j) {
+        const int base = blocks.base(j, PT_N) + half * C;
+        const bool part = !seen_by_all(base - half * C);
         if (!warp_wait(&bars.s_full[i], j & 1)) bars.fail[i][warp & 3] = 1;
         fence_after();
         // Two passes over the scores, 32 columns at a time, so that they need not stay in registers: the first
         // finds the maximum and puts capped, biased or masked scores back, the second makes the weights.
-        const int base = blocks.base(j, PT_N) + half * C;
-        const bool part = !seen_by_all(base - half * C);
         float mx = -INFINITY;
+        float x[32];
 #pragma unroll
         for (int q = 0; q < C / 32; ++q) {
-          float x[32];
           ld32(ts + half * C + 32 * q, reinterpret_cast<uint32_t*>(x));
           ld_wait();
           const int b = base + 32 * q;
           if constexpr (MODE == PT_CAP) {
             const uint64_t in2 = pair(p.cap_in, p.cap_in), out2 = pair(-2.0f * p.cap_log2, -2.0f * p.cap_log2), cap2 = pair(p.cap_log2, p.cap_log2);
 #pragma unroll
-            for (int c = 0; c < 32; c += 2) {  // cap tanh, as score_log2
-              float2 y = split(mul2(pair(x[c], x[c + 1]), in2));
-              if ((c >> 1) % PT_OF < PT_POLY_CAP) {
-                asm("min.NaN.f32 %0, %0, %1;" : "+f"(y.x) : "f"(126.0f));
-                asm("min.NaN.f32 %0, %0, %1;" : "+f"(y.y) : "f"(126.0f));
-                y = split(exp2_poly<5>(pair(y.x, y.y)));
-              } else {
-                y.x = ex2(y.x);
-                y.y = ex2(y.y);
+            for (int c = 0; c < 32; c += 2 * PT_OF) {  // cap tanh, as score_log2
+              uint64_t y[PT_OF];
+#pragma unroll
+              for (int e = 0; e < PT_OF; ++e) {
+                y[e] = mul2(pair(x[c + 2 * e], x[c + 2 * e + 1]), in2);
+                if (e < PT_POLY_CAP) {  // the polynomial's range: tanh is 1 long before
+                  float2 v = split(y[e]);
+                  asm("min.NaN.f32 %0, %0, %1;" : "+f"(v.x) : "f"(126.0f));
+                  asm("min.NaN.f32 %0, %0, %1;" : "+f"(v.y) : "f"(126.0f));
+                  y[e] = pair(v.x, v.y);
+                }
               }
-              y = split(add2(pair(y.x, y.y), pair(1.0f, 1.0f)));
-              y = split(fma2(pair(rcp_approx(y.x), rcp_approx(y.y)), out2, cap2));
-              x[c] = y.x;
-              x[c + 1] = y.y;
+              exp2_group<5, PT_POLY_CAP>(y);
+#pragma unroll
+              for (int e = 0; e < PT_OF; ++e) {
+                const float2 v = split(add2(y[e], pair(1.0f, 1.0f)));
+                const float2 u = split(fma2(pair(rcp_approx(v.x), rcp_approx(v.y)), out2, cap2));
+                x[c + 2 * e] = u.x;
+                x[c + 2 * e + 1] = u.y;
+              }
             }
           } else if constexpr (MODE == PT_ANY) {
             if (p.a.softcap > 0.f) {
@@ -371,7 +397,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
           l *= factor;
           if (j > 0) {
 #pragma unroll
-            for (int c = 0; c < D / 64; ++c) {
+            for (int c = 0; c < D / PT_SPLIT / 32; ++c) {
               uint32_t o[32];
               ld32(to + 32 * c, o);
               ld_wait();
@@ -386,25 +412,24 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
         const uint64_t z2 = pair(z, z), scale2 = pair(p.scale_log2, p.scale_log2);
 #pragma unroll
         for (int q = 0; q < C / 32; ++q) {
-          float x[32];
           uint32_t w[16];
           ld32(ts + half * C + 32 * q, reinterpret_cast<uint32_t*>(x));
           ld_wait();
 #pragma unroll
-          for (int c = 0; c < 32; c += 2) {
-            constexpr int POLY = MODE == PT_CAP ? PT_OF : PT_POLY;
-            uint64_t y2;
-            if constexpr (MODE == PT_PLAIN) y2 = fma2(pair(x[c], x[c + 1]), scale2, z2);
-            else y2 = add2(pair(x[c], x[c + 1]), z2);
-            float2 y = split(y2);
-            if ((c >> 1) % PT_OF < POLY) {
-              y = split(exp2_poly<4>(y2));
-            } else {
-              y.x = ex2(y.x);
-              y.y = ex2(y.y);
+          for (int c = 0; c < 32; c += 2 * PT_OF) {
+            uint64_t y[PT_OF];
+#pragma unroll
+            for (int e = 0; e < PT_OF; ++e) {
+              const uint64_t v = pair(x[c + 2 * e], x[c + 2 * e + 1]);
+              y[e] = MODE == PT_PLAIN ? fma2(v, scale2, z2) : add2(v, z2);
             }
-            part2[(c >> 1) & 1] = add2(part2[(c >> 1) & 1], pair(y.x, y.y));
-            w[c / 2] = pack2<DT>(y.x, y.y);
+            exp2_group<4, MODE == PT_CAP ? PT_POLY_EXP : PT_POLY>(y);
+#pragma unroll
+            for (int e = 0; e < PT_OF; ++e) {
+              part2[e & 1] = add2(part2[e & 1], y[e]);
+              const float2 v = split(y[e]);
+              w[c / 2 + e] = pack2<DT>(v.x, v.y);
+            }
           }
           st16(ts + half * C + 16 * q, w);  // over scores that this thread has read
         }
@@ -421,9 +446,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
       named_bar(meet, 64);
       l += bars.row[n & 1][i][half ^ 1][row];
       const float inv = l == 0.f ? 0.f : 1.0f / l;
-      T* out = static_cast<T*>(a.out) + int64_t(t.first + tok) * a.o_stride_t + h * a.o_stride_h + half * (D / 2);
+      T* out = static_cast<T*>(a.out) + int64_t(t.first + tok) * a.o_stride_t + h * a.o_stride_h + half * (D / PT_SPLIT);
 #pragma unroll
-      for (int c = 0; c < D / 64; ++c) {
+      for (int c = 0; c < D / PT_SPLIT / 32; ++c) {
         uint32_t o[32], w[16];
         if (n > 0) {
           ld32(to + 32 * c, o);
@@ -453,7 +478,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
     fence_after();
     dealloc(bars.tmem, PT_COLS);
   }
-  if (warp < PT_LOAD_WARP && bars.special && (warp >> 3) < tiles) {
+  if (warp < PT_LOAD_WARP && bars.special && warp / PT_TW < tiles) {
     uint32_t redo = __ballot_sync(~0u, odd != 0.f && l == l && f < last);
     for (; redo; redo &= redo - 1) exact_row(p, t, kvh, __shfl_sync(~0u, f, __ffs(redo) - 1));
   }

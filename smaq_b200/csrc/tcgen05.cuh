@@ -138,29 +138,45 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 // by a polynomial with p(0) = 1 of least relative error on [-1/2, 1/2] (fitted by linear programming on
 // Chebyshev points): 2.9e-6 for degree 4, 1.9e-7 for 5.  x below -126.5 gives 0 exactly, -infinity
 // too; NaN stays NaN.
-template <int DEG>
-__device__ __forceinline__ uint64_t exp2_poly(uint64_t x) {
-  float2 v = split(x);
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(v.x) : "f"(-127.0f));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(v.y) : "f"(-127.0f));
+__device__ constexpr float exp2_coef(int deg, int power) {
+  return deg == 4 ? (power == 1 ? 0.6931241750717163f : power == 2 ? 0.24024099111557007f : power == 3 ? 0.055906426161527634f : 0.009582852944731712f)
+                  : (power == 1   ? 0.6931470036506653f
+                     : power == 2 ? 0.24022242426872253f
+                     : power == 3 ? 0.05550733953714371f
+                     : power == 4 ? 0.009671511128544807f
+                                  : 0.001326465280726552f);
+}
+// N pairs step by step side by side: one pair alone is a chain of eleven dependent operations.
+template <int DEG, int N>
+__device__ __forceinline__ void exp2_poly(uint64_t (&x)[N]) {
   constexpr float kMagic = 12582912.0f + 127.0f;
-  x = pair(v.x, v.y);
-  const uint64_t t = add2(x, pair(kMagic, kMagic));
-  const uint64_t r = fma2(add2(t, pair(-kMagic, -kMagic)), pair(-1.0f, -1.0f), x);
-  uint64_t y;
-  if constexpr (DEG == 4) {
-    y = fma2(pair(0.009582852944731712f, 0.009582852944731712f), r, pair(0.055906426161527634f, 0.055906426161527634f));
-    y = fma2(y, r, pair(0.24024099111557007f, 0.24024099111557007f));
-    y = fma2(y, r, pair(0.6931241750717163f, 0.6931241750717163f));
-  } else {
-    y = fma2(pair(0.001326465280726552f, 0.001326465280726552f), r, pair(0.009671511128544807f, 0.009671511128544807f));
-    y = fma2(y, r, pair(0.05550733953714371f, 0.05550733953714371f));
-    y = fma2(y, r, pair(0.24022242426872253f, 0.24022242426872253f));
-    y = fma2(y, r, pair(0.6931470036506653f, 0.6931470036506653f));
+  uint64_t t[N], r[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    float2 v = split(x[i]);
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(v.x) : "f"(-127.0f));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(v.y) : "f"(-127.0f));
+    x[i] = pair(v.x, v.y);
   }
-  y = fma2(y, r, pair(1.0f, 1.0f));
-  const float2 n = split(t);
-  return mul2(y, pair(__uint_as_float(__float_as_uint(n.x) << 23), __uint_as_float(__float_as_uint(n.y) << 23)));
+#pragma unroll
+  for (int i = 0; i < N; ++i) t[i] = add2(x[i], pair(kMagic, kMagic));
+#pragma unroll
+  for (int i = 0; i < N; ++i) r[i] = add2(t[i], pair(-kMagic, -kMagic));
+#pragma unroll
+  for (int i = 0; i < N; ++i) r[i] = fma2(r[i], pair(-1.0f, -1.0f), x[i]);
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = fma2(pair(exp2_coef(DEG, DEG), exp2_coef(DEG, DEG)), r[i], pair(exp2_coef(DEG, DEG - 1), exp2_coef(DEG, DEG - 1)));
+#pragma unroll
+  for (int d = DEG - 2; d >= 1; --d)
+#pragma unroll
+    for (int i = 0; i < N; ++i) x[i] = fma2(x[i], r[i], pair(exp2_coef(DEG, d), exp2_coef(DEG, d)));
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = fma2(x[i], r[i], pair(1.0f, 1.0f));
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const float2 n = split(t[i]);
+    x[i] = mul2(x[i], pair(__uint_as_float(__float_as_uint(n.x) << 23), __uint_as_float(__float_as_uint(n.y) << 23)));
+  }
 }
 
 }  // namespace tc5
