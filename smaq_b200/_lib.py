@@ -8,6 +8,8 @@ from __future__ import annotations
 
 import ctypes as C
 import os
+import struct
+from typing import Callable
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libsmaq_b200.so")
@@ -135,6 +137,20 @@ class PagedArgs(C.Structure):
     ]
 
 
+_CODES = {vp: "P", i64: "q", i32: "i", C.c_size_t: "N", C.c_float: "f"}
+
+
+def packer(mirror) -> Callable[..., bytes]:
+    """``struct`` packer of a mirror's fields, in order (pointers as integers, 0 for NULL): the small
+    serving calls fill their arguments in one go, which costs a third of setting ctypes fields."""
+    s = struct.Struct("@" + "".join(_CODES[t] for _, t in mirror._fields_) + "0q")
+    if s.size != C.sizeof(mirror):
+        raise RuntimeError(f"{mirror.__name__}: packed size {s.size}, mirror {C.sizeof(mirror)}")
+    return s.pack
+
+
+pack_tables, pack_norm_rope, pack_paged = packer(TablesArgs), packer(NormRopeArgs), packer(PagedArgs)
+
 _lib = None
 
 
@@ -162,15 +178,15 @@ def load() -> C.CDLL:
         if lib.smaq_paged_args_size(which) != C.sizeof(mirror):
             raise RuntimeError(f"{path}: {mirror.__name__} is {C.sizeof(mirror)} bytes here but "
                                f"{lib.smaq_paged_args_size(which)} in the library (stale build or ABI mismatch)")
-    lib.smaq_step_tables.argtypes = [C.POINTER(TablesArgs), vp]
+    lib.smaq_step_tables.argtypes = [C.c_char_p, vp]  # packed arguments
     lib.smaq_step_tables.restype = i32
-    lib.smaq_norm_rope.argtypes = [C.POINTER(NormRopeArgs), vp]
+    lib.smaq_norm_rope.argtypes = [C.c_char_p, vp]
     lib.smaq_norm_rope.restype = i32
     lib.smaq_paged_decode_workspace_size.argtypes = [i32, i32, i32, i32]
     lib.smaq_paged_decode_workspace_size.restype = C.c_size_t
-    lib.smaq_paged_decode.argtypes = [C.POINTER(PagedArgs), vp]
+    lib.smaq_paged_decode.argtypes = [C.c_char_p, vp]
     lib.smaq_paged_decode.restype = i32
-    lib.smaq_paged_prefill.argtypes = [C.POINTER(PagedArgs), vp]
+    lib.smaq_paged_prefill.argtypes = [C.c_char_p, vp]
     lib.smaq_paged_prefill.restype = i32
     lib.smaq_prefill_status.argtypes = [vp]
     lib.smaq_prefill_status.restype = i32

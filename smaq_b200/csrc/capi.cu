@@ -2,6 +2,8 @@
 #include <stdarg.h>
 #include <stdio.h>
 
+#include <atomic>
+
 #include "common.cuh"
 
 namespace smaq {
@@ -29,9 +31,12 @@ int cuda_status(cudaError_t e, const char* where) {
 }
 
 int num_sms() {
+  static std::atomic<int> known[64];  // by device: the count does not change
   int dev = 0, n = 0;
   if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+  if (dev < 64 && (n = known[dev].load(std::memory_order_relaxed)) > 0) return n;
   if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || n <= 0) return 148;
+  if (dev < 64) known[dev].store(n, std::memory_order_relaxed);
   return n;
 }
 

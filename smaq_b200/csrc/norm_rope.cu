@@ -8,7 +8,7 @@
 // half, so both partners of every pair, (i, i + R/2) as well as (2i, 2i + 1), are in one lane and the
 // rotation needs no exchange; only the sum of squares crosses lanes.  The cosines and sines of a token
 // are read once into registers and serve all heads that the lane group walks; it walks more heads a token
-// when there are enough tokens to fill the GPU, and loads two heads ahead.  Values are copied by the same
+// when there are enough tokens to fill the GPU, and loads a head ahead.  Values are copied by the same
 // walk.  Bound by HBM bytes for prompts, by latency for decode steps.
 // norm_rope_any_kernel: any head_dim and alignment, one warp a head, element by element.
 #include "common.cuh"
@@ -21,11 +21,17 @@ struct NrParams {
   smaq_norm_rope_args a;
   int heads;            // q + k (+ v with a cache)
   int per;              // heads that a lane group walks
-  int groups;           // ceil(heads / per)
+  int groups, q_groups, k_groups;  // lane groups a token, of its queries and of its keys (and values)
   FastDiv page_div;
 };
 
 constexpr int NR_THREADS = 256;
+#ifndef NR_CTAS
+#define NR_CTAS 3
+#endif
+#ifndef NR_PER
+#define NR_PER 8
+#endif
 
 // Element offset of slot `s` in the cache, < 0 for one outside it.
 __device__ __forceinline__ int64_t slot_offset(const NrParams& p, int64_t s) {
@@ -84,9 +90,10 @@ __device__ __forceinline__ void load8f(const float* p, float* x) {
   x[4] = w.x; x[5] = w.y; x[6] = w.z; x[7] = w.w;
 }
 
-// LANES lanes a head (a power of two >= head_dim / 16).
+// LANES lanes a head (a power of two >= head_dim / 16).  A lane group walks `per` heads of one kind (queries, keys
+// or values) of one token.
 template <class DT, int LANES, bool INTERLEAVED>
-__global__ void __launch_bounds__(NR_THREADS) norm_rope_kernel(const __grid_constant__ NrParams p) {
+__global__ void __launch_bounds__(NR_THREADS, NR_CTAS) norm_rope_kernel(const __grid_constant__ NrParams p) {
   using T = typename DT::T;
   const smaq_norm_rope_args& a = p.a;
   const int lane = threadIdx.x % LANES;
@@ -94,21 +101,63 @@ __global__ void __launch_bounds__(NR_THREADS) norm_rope_kernel(const __grid_cons
   const int64_t t = job / p.groups;
   if (t >= a.n_tokens) return;  // whole lane groups leave; the shuffles below name the group's lanes
   const unsigned mask = (LANES == 32 ? ~0u : ((1u << LANES) - 1u) << ((threadIdx.x & 31) / LANES * LANES));
-  const int h0 = int(job - t * p.groups) * p.per, h1 = min(h0 + p.per, p.heads);
-  const int D = a.head_dim, R = a.rotary_dim, Hq = a.n_q_heads, Hk = a.n_kv_heads;
+  const int D = a.head_dim, R = a.rotary_dim;
+  int g = int(job - t * p.groups), kind = 0;
+  if (g >= p.q_groups) {
+    g -= p.q_groups;
+    kind = 1 + (g >= p.k_groups);
+    if (kind == 2) g -= p.k_groups;
+  }
+  const int h0 = g * p.per;
+  int left = min(p.per, (kind ? a.n_kv_heads : a.n_q_heads) - h0);
   const bool live = lane < D / 16, turned = lane < R / 16;
   // this lane's two vectors
-  const int ea = turned ? 8 * lane : R + 16 * (lane - R / 16), eb = turned ? R / 2 + 8 * lane : ea + 8;
+  const int ea = turned ? 8 * lane : R + 16 * (lane - R / 16), ahead = turned ? R / 2 : 8;
 
-  float c[16], s[16];
-  if (turned && h0 < Hq + Hk) {
+  const int64_t in_step = kind == 0 ? a.q_stride_h : kind == 1 ? a.k_stride_h : a.v_stride_h;
+  const T* src = static_cast<const T*>(kind == 0 ? a.q : kind == 1 ? a.k : a.v) +
+                 t * (kind == 0 ? a.q_stride_t : kind == 1 ? a.k_stride_t : a.v_stride_t) + h0 * in_step + ea;
+  T *dst, *also = nullptr;  // also: keys may go to the cache and to k_out
+  int64_t step = D;
+  if (kind == 0) {
+    dst = static_cast<T*>(a.q_out) + (t * a.n_q_heads + h0) * D + ea;
+  } else {
+    if (kind == 1 && a.k_out) also = static_cast<T*>(a.k_out) + (t * a.n_kv_heads + h0) * D + ea;
+    const int64_t at = a.k_cache ? slot_offset(p, a.slots[t]) : -1;
+    dst = at < 0 ? nullptr : static_cast<T*>(kind == 1 ? a.k_cache : a.v_cache) + at + h0 * a.c_stride_h + ea;
+    step = a.c_stride_h;
+  }
+  Vec8<DT> na = {}, nb = {};  // the next head's
+  if (live) {
+    na = load8<DT>(src);
+    nb = load8<DT>(src + ahead);
+  }
+  if (kind == 2) {
+    while (left-- > 0) {
+      const Vec8<DT> va = na, vb = nb;
+      if (!live) continue;
+      if (left > 0) {
+        src += in_step;
+        na = load8<DT>(src);
+        nb = load8<DT>(src + ahead);
+      }
+      if (dst) {
+        store8<DT>(dst, va);
+        store8<DT>(dst + ahead, vb);
+        dst += step;
+      }
+    }
+    return;
+  }
+  float c[8], s[8], w[16];
+  if (turned) {
     const int pos = a.positions[t];
     if (pos >= 0 && pos < a.n_positions) {
       const float* row = a.table + int64_t(pos) * R;
-      if constexpr (INTERLEAVED) {
-        // pair i of vector a (b) is pair ea / 2 + i (eb / 2 + i)
-        const float4 ca = __ldg(reinterpret_cast<const float4*>(row + ea / 2)), cb = __ldg(reinterpret_cast<const float4*>(row + eb / 2));
-        const float4 sa = __ldg(reinterpret_cast<const float4*>(row + R / 2 + ea / 2)), sb = __ldg(reinterpret_cast<const float4*>(row + R / 2 + eb / 2));
+      if constexpr (INTERLEAVED) {  // pair i of either vector is pair (its first element) / 2 + i
+        const float4 ca = __ldg(reinterpret_cast<const float4*>(row + ea / 2)), cb = __ldg(reinterpret_cast<const float4*>(row + (ea + ahead) / 2));
+        row += R / 2;
+        const float4 sa = __ldg(reinterpret_cast<const float4*>(row + ea / 2)), sb = __ldg(reinterpret_cast<const float4*>(row + (ea + ahead) / 2));
         c[0] = ca.x; c[1] = ca.y; c[2] = ca.z; c[3] = ca.w; c[4] = cb.x; c[5] = cb.y; c[6] = cb.z; c[7] = cb.w;
         s[0] = sa.x; s[1] = sa.y; s[2] = sa.z; s[3] = sa.w; s[4] = sb.x; s[5] = sb.y; s[6] = sb.z; s[7] = sb.w;
       } else {
@@ -120,90 +169,54 @@ __global__ void __launch_bounds__(NR_THREADS) norm_rope_kernel(const __grid_cons
       for (int i = 0; i < 8; ++i) c[i] = s[i] = __int_as_float(0x7FC00000);
     }
   }
-  const int64_t dst = a.k_cache ? slot_offset(p, a.slots[t]) : 0;
-  float w[16];
-  int weighted = -1;  // whose weights w holds: 0 queries, 1 keys
-
-  auto source = [&](int h) {
-    return h < Hq        ? static_cast<const T*>(a.q) + t * a.q_stride_t + h * a.q_stride_h
-           : h < Hq + Hk ? static_cast<const T*>(a.k) + t * a.k_stride_t + (h - Hq) * a.k_stride_h
-                         : static_cast<const T*>(a.v) + t * a.v_stride_t + (h - Hq - Hk) * a.v_stride_h;
-  };
-  auto finish = [&](int h, Vec8<DT> va, Vec8<DT> vb) {
-    if (h < Hq + Hk) {
-      const int kind = h >= Hq;
-      const float* weight = kind ? a.k_weight : a.q_weight;
-      float x[16];
-      unpack8(va, x);
-      unpack8(vb, x + 8);
-      if (weight) {
-        if (weighted != kind) {
-          weighted = kind;
-          if (live) {
-            load8f(weight + ea, w);
-            load8f(weight + eb, w + 8);
-          }
-        }
-        float ss = 0.f;
-        if (live) {
+  const float* weight = kind ? a.k_weight : a.q_weight;
+  if (weight && live) {
+    load8f(weight + ea, w);
+    load8f(weight + ea + ahead, w + 8);
+  }
+  while (left-- > 0) {
+    float x[16];
+    unpack8(na, x);
+    unpack8(nb, x + 8);
+    if (left > 0 && live) {
+      src += in_step;
+      na = load8<DT>(src);
+      nb = load8<DT>(src + ahead);
+    }
+    if (weight) {
+      float ss = 0.f;
+      if (live) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) ss = fmaf(x[i], x[i], ss);
-        }
-#pragma unroll
-        for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
-        const float r = 1.0f / sqrtf(ss / float(D) + a.eps);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] *= r * w[i];
+        for (int i = 0; i < 16; ++i) ss = fmaf(x[i], x[i], ss);
       }
-      if (turned) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          // pair i: (i, i + 8) of this lane's sixteen, or its neighbours (2i, 2i + 1)
-          const int ia = INTERLEAVED ? 2 * i : i, ib = INTERLEAVED ? 2 * i + 1 : i + 8;
-          const float u = x[ia], v = x[ib];
-          x[ia] = u * c[i] - v * s[i];
-          x[ib] = v * c[i] + u * s[i];
-        }
-      }
-      va = pack8<DT>(x);
-      vb = pack8<DT>(x + 8);
+      for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
+      const float r = 1.0f / sqrtf(ss / float(D) + a.eps);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] *= r * w[i];
     }
-    if (!live) return;
-    if (h < Hq) {
-      T* o = static_cast<T*>(a.q_out) + (t * Hq + h) * D;
-      store8<DT>(o + ea, va);
-      store8<DT>(o + eb, vb);
-      return;
-    }
-    const int hk = h < Hq + Hk ? h - Hq : h - Hq - Hk;
-    if (h < Hq + Hk && a.k_out) {
-      T* o = static_cast<T*>(a.k_out) + (t * Hk + hk) * D;
-      store8<DT>(o + ea, va);
-      store8<DT>(o + eb, vb);
-    }
-    if (a.k_cache && dst >= 0) {
-      T* o = static_cast<T*>(h < Hq + Hk ? a.k_cache : a.v_cache) + dst + hk * a.c_stride_h;
-      store8<DT>(o + ea, va);
-      store8<DT>(o + eb, vb);
-    }
-  };
-
-  Vec8<DT> zero = {};
-  for (int h = h0; h < h1; h += 2) {
-    const bool two = h + 1 < h1;
-    Vec8<DT> a0 = zero, b0 = zero, a1 = zero, b1 = zero;
-    if (live) {
-      const T* s0 = source(h);
-      a0 = load8<DT>(s0 + ea);
-      b0 = load8<DT>(s0 + eb);
-      if (two) {
-        const T* s1 = source(h + 1);
-        a1 = load8<DT>(s1 + ea);
-        b1 = load8<DT>(s1 + eb);
+    if (turned) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        // pair i: (i, i + 8) of this lane's sixteen, or its neighbours (2i, 2i + 1)
+        const int ia = INTERLEAVED ? 2 * i : i, ib = INTERLEAVED ? 2 * i + 1 : i + 8;
+        const float u = x[ia], v = x[ib];
+        x[ia] = u * c[i] - v * s[i];
+        x[ib] = v * c[i] + u * s[i];
       }
     }
-    finish(h, a0, b0);
-    if (two) finish(h + 1, a1, b1);
+    if (!live) continue;
+    const Vec8<DT> va = pack8<DT>(x), vb = pack8<DT>(x + 8);
+    if (dst) {
+      store8<DT>(dst, va);
+      store8<DT>(dst + ahead, vb);
+      dst += step;
+    }
+    if (also) {
+      store8<DT>(also, va);
+      store8<DT>(also + ahead, vb);
+      also += D;
+    }
   }
 }
 
@@ -272,9 +285,10 @@ int launch_dtype(NrParams& p, cudaStream_t st) {
   // spread over the GPU; aim at four CTAs of threads an SM
   const int64_t want = int64_t(num_sms()) * 4 * NR_THREADS / lanes;  // lane groups
   int64_t per = p.a.n_tokens * p.heads / want;
-  per = per < 1 ? 1 : per > 8 ? 8 : per;
-  p.groups = int((p.heads + per - 1) / per);
-  p.per = (p.heads + p.groups - 1) / p.groups;
+  p.per = int(per < 1 ? 1 : per > NR_PER ? NR_PER : per);
+  p.q_groups = (p.a.n_q_heads + p.per - 1) / p.per;
+  p.k_groups = (p.a.n_kv_heads + p.per - 1) / p.per;
+  p.groups = p.q_groups + p.k_groups * (p.a.k_cache ? 2 : 1);
   switch (lanes) {
     case 4: return launch_lanes<DT, 4>(p, st);
     case 8: return launch_lanes<DT, 8>(p, st);

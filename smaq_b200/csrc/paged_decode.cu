@@ -579,20 +579,40 @@ __global__ void __launch_bounds__(PD_THREADS) paged_simt_kernel(const __grid_con
     const int32_t* table = a.block_table + at.b * a.table_stride;
     const T* kc = static_cast<const T*>(a.k_cache) + kvh * a.c_stride_h;
     const T* vc = static_cast<const T*>(a.v_cache) + kvh * a.c_stride_h;
+    // keys and values a step ahead where registers allow, addresses two
+    constexpr bool AHEAD = NI <= 4;
+    float nk[NI][4], nv[NI][4];
+    auto offset = [&](int j) { return j < hi ? token_offset(p, table, j) : int64_t(-1); };
+    auto fetch = [&](int64_t off) {
+      if (off >= 0) {
+        load_row<DT, NI, VEC>(kc + off, l, D, nk);
+        load_row<DT, NI, VEC>(vc + off, l, D, nv);
+        return;
+      }
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) nk[i][e] = nv[i][e] = 0.f;
+    };
+    int64_t next = offset(lo + grp);
+    if (AHEAD) {
+      fetch(next);
+      next = offset(lo + GROUPS + grp);
+    }
     for (int j0 = lo; j0 < hi; j0 += GROUPS) {  // the same number of steps for every group: whole warps shuffle
       const int j = j0 + grp;
       const bool seen = j < hi;
       float k[NI][4], v[NI][4];
-      if (seen) {
-        const int64_t off = token_offset(p, table, j);
-        load_row<DT, NI, VEC>(kc + off, l, D, k);
-        load_row<DT, NI, VEC>(vc + off, l, D, v);
-      } else {
+      if (!AHEAD) fetch(next);
 #pragma unroll
-        for (int i = 0; i < NI; ++i)
+      for (int i = 0; i < NI; ++i)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) k[i][e] = v[i][e] = 0.f;
-      }
+        for (int e = 0; e < 4; ++e) {
+          k[i][e] = nk[i][e];
+          v[i][e] = nv[i][e];
+        }
+      if (AHEAD) fetch(next);
+      next = offset(j + (AHEAD ? 2 : 1) * GROUPS);
 #pragma unroll
       for (int r = 0; r < PS_ROWS; ++r) {
         float x = 0.f;
@@ -689,6 +709,9 @@ __global__ void __launch_bounds__(PD_THREADS) paged_simt_kernel(const __grid_con
 __global__ void __launch_bounds__(PD_THREADS) paged_join_kernel(const __grid_constant__ DecodeParamsX d, int tile_rows) {
   __shared__ int64_t warp_sums[PD_THREADS / 32];
   __shared__ int64_t my_first;
+  __shared__ float reduce[PD_THREADS / 32];
+  extern __shared__ float slots_of[];  // [2][grid]
+  float *factor = slots_of, *part = slots_of + d.grid;
   const PagedParams& p = d.p;
   const smaq_paged_args& a = p.a;
   const int b = blockIdx.x / a.n_q_heads, h = blockIdx.x - b * a.n_q_heads, D = a.head_dim, LD = D + 2;
@@ -712,17 +735,31 @@ __global__ void __launch_bounds__(PD_THREADS) paged_join_kernel(const __grid_con
   if (c0 == c1) return;
   const int64_t step = int64_t(d.rows) * LD;
   const float* slot = d.slots + (int64_t(c0) + int64_t(b) * d.segs + s) * step + r * LD;
-  const int n = c1 - c0 + 1;
+  const int n = c1 - c0 + 1;  // at most the grid
+  // every slot's maximum and sum at once, then its factor
   float m = -INFINITY;
-  for (int i = 0; i < n; ++i) m = fmaxf(m, slot[i * step + D]);
+  for (int i = threadIdx.x; i < n; i += PD_THREADS) {
+    const float2 ml = *reinterpret_cast<const float2*>(slot + i * step + D);
+    factor[i] = ml.x;
+    part[i] = ml.y;
+    m = fmaxf(m, ml.x);
+  }
+  m = warp_max(m);
+  if ((threadIdx.x & 31) == 0) reduce[threadIdx.x >> 5] = m;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < PD_THREADS / 32; ++i) m = fmaxf(m, reduce[i]);
   const float z = m == -INFINITY ? 0.f : m;
   float sum = 0.f;
-  for (int i = 0; i < n; ++i) sum += ex2(slot[i * step + D] - z) * slot[i * step + D + 1];
+  for (int i = 0; i < n; ++i) sum += ex2(factor[i] - z) * part[i];  // in slot order, by every thread alike
+  __syncthreads();
+  for (int i = threadIdx.x; i < n; i += PD_THREADS) factor[i] = ex2(factor[i] - z);
+  __syncthreads();
   const float inv = sum == 0.f ? 0.f : 1.0f / sum;
   for (int c = threadIdx.x; c < D; c += PD_THREADS) {
     float x = 0.f;
-#pragma unroll 4
-    for (int i = 0; i < n; ++i) x += ex2(slot[i * step + D] - z) * slot[i * step + c];
+#pragma unroll 8
+    for (int i = 0; i < n; ++i) x += factor[i] * slot[i * step + c];
     store_elem(a.out, a.dtype, b * a.o_stride_t + h * a.o_stride_h + c, x * inv);
   }
   if (a.lse && threadIdx.x == 0) a.lse[int64_t(b) * a.n_q_heads + h] = (m + log2f(sum)) * kLn2;
@@ -809,6 +846,7 @@ extern "C" int smaq_paged_decode(const smaq_paged_args* args, void* stream) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(a.batch) * unsigned(a.n_q_heads));
   cfg.blockDim = dim3(PD_THREADS);
+  cfg.dynamicSmemBytes = size_t(d.grid) * 2 * sizeof(float);
   cfg.stream = st;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -482,18 +482,22 @@ class StepTables(NamedTuple):
     admitted: torch.Tensor      # [B] bool
 
 
-def _same_device(dev: torch.device, **ts: Optional[torch.Tensor]) -> int:
-    """Every given tensor is on ``dev``, the current CUDA device; returns the current stream there."""
-    for name, t in ts.items():
-        if t is not None and t.device != dev:
-            if not t.is_cuda:
-                _cuda(t)
-            raise ValueError(f"{name} is on {t.device}, expected {dev}")
-    if dev.type != "cuda":
-        raise RuntimeError(f"smaq_b200 kernels need CUDA tensors (there is no CPU fallback); got a tensor on {dev}")
-    if dev.index != torch.cuda.current_device():
-        raise ValueError(f"tensors are on {dev}, but the current device is cuda:{torch.cuda.current_device()}")
-    return torch.cuda.current_stream().cuda_stream
+def _stream_for(ref: torch.Tensor, others: tuple) -> int:
+    """The current stream of ``ref``'s device, on which every other tensor (or None) must be too."""
+    dev = ref.get_device()
+    for t in others:
+        if t is not None and t.get_device() != dev:
+            _cuda(ref, *others)
+            raise ValueError(f"tensors are on {ref.device} and {t.device}")
+    if dev < 0:
+        _cuda(ref)
+    if dev != torch._C._cuda_getDevice():
+        raise ValueError(f"tensors are on {ref.device}, but the current device is cuda:{torch.cuda.current_device()}")
+    return torch._C._cuda_getCurrentRawStream(dev)
+
+
+def _addr(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
 
 
 def _int32(name: str, t: torch.Tensor, n: int) -> torch.Tensor:
@@ -518,9 +522,7 @@ def step_tables(free_blocks: torch.Tensor, free_count: torch.Tensor, context_len
     length is 0.  ``free_blocks`` (int32) and ``block_table`` (int32) are updated in place, the
     new ``free_count`` is returned.  ``num_tokens``: length of ``positions`` and ``slots``; entries past
     the step's tokens get position 0 and slot -1.  Nothing is read back to the host."""
-    dev = free_blocks.device
-    stream = _same_device(dev, free_blocks=free_blocks, free_count=free_count, context_lens=context_lens,
-                          query_lens=query_lens, block_table=block_table, finished=finished)
+    stream = _stream_for(free_blocks, (free_count, context_lens, query_lens, block_table, finished))
     B = context_lens.shape[0]
     if free_blocks.dtype != torch.int32 or free_blocks.dim() != 1 or not free_blocks.is_contiguous():
         raise ValueError("free_blocks must be a contiguous int32 vector (it is updated in place)")
@@ -535,23 +537,22 @@ def step_tables(free_blocks: torch.Tensor, free_count: torch.Tensor, context_len
         if finished.shape != (B,) or finished.dtype not in (torch.bool, torch.uint8):
             raise ValueError(f"finished must be a bool vector of length {B}")
         finished = finished.contiguous()
-    # one buffer: slots (8 bytes) first, then the int32 outputs, positions on a 16-byte boundary
-    pad = (num_tokens + 3) // 4 * 4
-    buf = torch.empty((3 * pad + 2 * B + 2,), dtype=torch.int32, device=dev)
-    slots = buf[:2 * num_tokens].view(torch.int64)
-    positions = buf[2 * pad:2 * pad + num_tokens]
-    cu, lens, left = buf[3 * pad:3 * pad + B + 1], buf[3 * pad + B + 1:3 * pad + 2 * B + 1], buf[3 * pad + 2 * B + 1:]
-    admitted = torch.empty((B,), dtype=torch.bool, device=dev)
-    M = block_table.shape[1]
+    # one buffer: slots (8 bytes) first, positions on a 16-byte boundary, the rest
+    M, T, dev = block_table.shape[1], num_tokens, free_blocks.device
+    pad = (T + 3) // 4 * 4
+    buf = torch.empty(3 * pad + 2 * B + 2, dtype=torch.int32, device=dev)
+    slots, _, positions, _, cu, lens, left = buf.split_with_sizes([2 * T, 2 * (pad - T), T, pad - T, B + 1, B, 1])
+    admitted = torch.empty(B, dtype=torch.bool, device=dev)
     at = buf.data_ptr()
-    a = _lib.TablesArgs(free_blocks.data_ptr(), free_count.data_ptr(), context_lens.data_ptr(), query_lens.data_ptr(),
-                        _ptr(finished), block_table.data_ptr(), max(block_table.stride(0), M), free_blocks.shape[0],
-                        num_tokens, B, M, block_size, at + 12 * pad, at + 12 * pad + 4 * (B + 1), at + 8 * pad, at,
-                        admitted.data_ptr(), at + 12 * pad + 4 * (2 * B + 1))
-    st = _lib.load().smaq_step_tables(a, stream)
+    rest = at + 12 * pad
+    st = _lib.load().smaq_step_tables(
+        _lib.pack_tables(free_blocks.data_ptr(), free_count.data_ptr(), context_lens.data_ptr(), query_lens.data_ptr(),
+                         _addr(finished), block_table.data_ptr(), max(block_table.stride(0), M), free_blocks.shape[0], T,
+                         B, M, block_size, rest, rest + 4 * (B + 1), at + 8 * pad, at, admitted.data_ptr(),
+                         rest + 4 * (2 * B + 1)), stream)
     if st:
         _lib.check(st, "smaq_step_tables")
-    return StepTables(cu, lens, positions, slots, left, admitted)
+    return StepTables(cu, lens, positions, slots.view(torch.int64), left, admitted)
 
 
 def rope_table(max_positions: int, rotary_dim: int, base: float = 10000.0, *, linear: float = 1.0,
@@ -600,12 +601,13 @@ def _head_rows(name: str, x: torch.Tensor, dtype: torch.dtype, T: int, D: int) -
 
 
 def _cache_pair(k_cache: torch.Tensor, v_cache: torch.Tensor, dtype: torch.dtype, D: int) -> None:
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[3] != D:
+    shape, strides = k_cache.shape, k_cache.stride()
+    if len(shape) != 4 or shape != v_cache.shape or shape[3] != D:
         raise ValueError(f"caches must be [pages, page_size, kv_heads, {D}], got {tuple(k_cache.shape)} and "
                          f"{tuple(v_cache.shape)}")
     if k_cache.dtype != dtype or v_cache.dtype != dtype:
         raise ValueError(f"caches must be {dtype} like the queries, got {k_cache.dtype} and {v_cache.dtype}")
-    if k_cache.stride() != v_cache.stride() or (D > 1 and k_cache.stride(3) != 1):
+    if strides != v_cache.stride() or (D > 1 and strides[3] != 1):
         raise ValueError("caches must have the same strides and a contiguous head_dim")
 
 
@@ -625,8 +627,7 @@ def norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, table: 
     T, Hq, D = q.shape
     dt = q.dtype
     code = dtype_code(dt)
-    stream = _same_device(q.device, q=q, k=k, positions=positions, table=table, q_weight=q_weight, k_weight=k_weight,
-                          v=v, k_cache=k_cache, v_cache=v_cache, slots=slots)
+    stream = _stream_for(q, (k, positions, table, q_weight, k_weight, v, k_cache, v_cache, slots))
     q, k = _head_rows("q", q, dt, T, D), _head_rows("k", k, dt, T, D)
     Hk = k.shape[1]
     positions = _int32("positions", positions, T)
@@ -661,11 +662,12 @@ def norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, table: 
     else:
         k_out = torch.empty((T, Hk, D), dtype=dt, device=q.device)
     qs, ks = q.stride(), k.stride()
-    a = _lib.NormRopeArgs(q.data_ptr(), k.data_ptr(), _ptr(v), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1],
-                          positions.data_ptr(), table.data_ptr(), _ptr(q_weight), _ptr(k_weight), _ptr(slots),
-                          q_out.data_ptr(), _ptr(k_out), _ptr(k_cache), _ptr(v_cache), cs[0], cs[1], cs[2], T,
-                          table.shape[0], pages, code, Hq, Hk, D, table.shape[1], int(interleaved), page_size, eps)
-    st = _lib.load().smaq_norm_rope(a, stream)
+    st = _lib.load().smaq_norm_rope(
+        _lib.pack_norm_rope(q.data_ptr(), k.data_ptr(), _addr(v), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1],
+                            positions.data_ptr(), table.data_ptr(), _addr(q_weight), _addr(k_weight), _addr(slots),
+                            q_out.data_ptr(), _addr(k_out), _addr(k_cache), _addr(v_cache), cs[0], cs[1], cs[2], T,
+                            table.shape[0], pages, code, Hq, Hk, D, table.shape[1], int(interleaved), page_size, eps),
+        stream)
     if st:
         _lib.check(st, "smaq_norm_rope")
     return q_out, k_out
@@ -682,8 +684,7 @@ def _paged(name, q, k_cache, v_cache, block_table, seq_lens, cu_query, prefix_le
     T, Hq, D = q.shape
     dt = q.dtype
     code = dtype_code(dt)
-    stream = _same_device(q.device, q=q, k_cache=k_cache, v_cache=v_cache, block_table=block_table, seq_lens=seq_lens,
-                          cu_query=cu_query, prefix_lens=prefix_lens, slopes=slopes, out=out, workspace=workspace)
+    stream = _stream_for(q, (k_cache, v_cache, block_table, seq_lens, cu_query, prefix_lens, slopes, out, workspace))
     if q.stride(2) != 1 and D > 1:
         q = q.contiguous()
     _cache_pair(k_cache, v_cache, dt, D)
@@ -725,13 +726,13 @@ def _paged(name, q, k_cache, v_cache, block_table, seq_lens, cu_query, prefix_le
         ws, ws_bytes, call = workspace.data_ptr(), workspace.numel() * workspace.element_size(), lib.smaq_paged_decode
     else:
         cu_query = _int32("cu_query", cu_query, B + 1)
-        ws, ws_bytes, call = None, 0, lib.smaq_paged_prefill
-    a = _lib.PagedArgs(q.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2],
-                       block_table.data_ptr(), max(block_table.stride(0), M), seq_lens.data_ptr(), _ptr(cu_query),
-                       _ptr(prefix_lens), _ptr(slopes), out.data_ptr(), os[0], os[1], _ptr(lse), ws, ws_bytes, P, T, B,
-                       M, page_size, Hq, Hk, D, code, window or 0, 1.0 / math.sqrt(D) if scale is None else scale,
-                       softcap or 0.0)
-    st = call(a, stream)
+        ws, ws_bytes, call = 0, 0, lib.smaq_paged_prefill
+    st = call(
+        _lib.pack_paged(q.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2],
+                        block_table.data_ptr(), max(block_table.stride(0), M), seq_lens.data_ptr(), _addr(cu_query),
+                        _addr(prefix_lens), _addr(slopes), out.data_ptr(), os[0], os[1], _addr(lse), ws, ws_bytes, P, T,
+                        B, M, page_size, Hq, Hk, D, code, window or 0, 1.0 / math.sqrt(D) if scale is None else scale,
+                        softcap or 0.0), stream)
     if st:
         _lib.check(st, name)
     return (out, lse) if return_lse else out
