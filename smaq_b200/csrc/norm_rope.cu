@@ -12,6 +12,7 @@
 // walk.  Bound by HBM bytes for prompts, by latency for decode steps.
 // norm_rope_any_kernel: any head_dim and alignment, one warp a head, element by element.
 #include "common.cuh"
+#include "ptx.cuh"
 
 namespace smaq {
 
@@ -22,16 +23,13 @@ struct NrParams {
   int heads;            // q + k (+ v with a cache)
   int per;              // heads that a lane group walks
   int groups, q_groups, k_groups;  // lane groups a token, of its queries and of its keys (and values)
+  float inv_dim;
   FastDiv page_div;
 };
 
-constexpr int NR_THREADS = 256;
-#ifndef NR_CTAS
-#define NR_CTAS 3
-#endif
-#ifndef NR_PER
-#define NR_PER 8
-#endif
+constexpr int NR_THREADS = 128;
+constexpr int NR_CTAS = 6;  // an SM: 80 registers; 64 spill (67 us), 104 hold too few loads in flight (78 us)
+constexpr int NR_PER = 2;   // heads a lane group walks at most: 1, 2, 4, 8, 16 took 91, 54, 56, 62, 70 us at 8192 tokens
 
 // Element offset of slot `s` in the cache, < 0 for one outside it.
 __device__ __forceinline__ int64_t slot_offset(const NrParams& p, int64_t s) {
@@ -70,24 +68,48 @@ __device__ __forceinline__ void store8(typename DT::T* p, const Vec8<DT>& v) {
   *reinterpret_cast<decltype(v.u)*>(p) = v.u;
   if constexpr (DT::code == SMAQ_F32) reinterpret_cast<float4*>(p)[1] = v.w;
 }
+// Eight elements as four packed pairs of 32-bit values.
 template <class DT>
-__device__ __forceinline__ void unpack8(const Vec8<DT>& v, float* x) {
-  const typename DT::T* e = reinterpret_cast<const typename DT::T*>(&v);
+__device__ __forceinline__ void unpack8(const Vec8<DT>& v, uint64_t* x) {
+  if constexpr (DT::code == SMAQ_F32) {
+    x[0] = pair(v.u.x, v.u.y);
+    x[1] = pair(v.u.z, v.u.w);
+    x[2] = pair(v.w.x, v.w.y);
+    x[3] = pair(v.w.z, v.w.w);
+  } else {
+    const uint32_t w[4] = {v.u.x, v.u.y, v.u.z, v.u.w};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) x[i] = to_f(e[i]);
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (DT::code == SMAQ_BF16) {
+        x[i] = pair(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
+      } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        x[i] = pair(f.x, f.y);
+      }
+    }
+  }
 }
 template <class DT>
-__device__ __forceinline__ Vec8<DT> pack8(const float* x) {
+__device__ __forceinline__ Vec8<DT> pack8(const uint64_t* x) {
   Vec8<DT> v;
-  typename DT::T* e = reinterpret_cast<typename DT::T*>(&v);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) e[i] = from_f<DT>(x[i]);
+  const float2 f0 = split(x[0]), f1 = split(x[1]), f2 = split(x[2]), f3 = split(x[3]);
+  if constexpr (DT::code == SMAQ_F32) {
+    v.u = make_float4(f0.x, f0.y, f1.x, f1.y);
+    v.w = make_float4(f2.x, f2.y, f3.x, f3.y);
+  } else if constexpr (DT::code == SMAQ_BF16) {
+    auto two = [](float2 f) { uint32_t r; asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(f.y), "f"(f.x)); return r; };
+    v.u = make_uint4(two(f0), two(f1), two(f2), two(f3));
+  } else {
+    v.u = make_uint4(pack_f16x2(f0.x, f0.y), pack_f16x2(f1.x, f1.y), pack_f16x2(f2.x, f2.y), pack_f16x2(f3.x, f3.y));
+  }
   return v;
 }
-__device__ __forceinline__ void load8f(const float* p, float* x) {
+__device__ __forceinline__ void load8f(const float* p, uint64_t* x) {
   const float4 u = __ldg(reinterpret_cast<const float4*>(p)), w = __ldg(reinterpret_cast<const float4*>(p) + 1);
-  x[0] = u.x; x[1] = u.y; x[2] = u.z; x[3] = u.w;
-  x[4] = w.x; x[5] = w.y; x[6] = w.z; x[7] = w.w;
+  x[0] = pair(u.x, u.y);
+  x[1] = pair(u.z, u.w);
+  x[2] = pair(w.x, w.y);
+  x[3] = pair(w.z, w.w);
 }
 
 // LANES lanes a head (a power of two >= head_dim / 16).  A lane group walks `per` heads of one kind (queries, keys
@@ -149,7 +171,7 @@ __global__ void __launch_bounds__(NR_THREADS, NR_CTAS) norm_rope_kernel(const __
     }
     return;
   }
-  float c[8], s[8], w[16];
+  uint64_t c[4], s[4], w[8];  // interleaved: the cosines and sines of vector a's four pairs, then b's
   if (turned) {
     const int pos = a.positions[t];
     if (pos >= 0 && pos < a.n_positions) {
@@ -158,55 +180,67 @@ __global__ void __launch_bounds__(NR_THREADS, NR_CTAS) norm_rope_kernel(const __
         const float4 ca = __ldg(reinterpret_cast<const float4*>(row + ea / 2)), cb = __ldg(reinterpret_cast<const float4*>(row + (ea + ahead) / 2));
         row += R / 2;
         const float4 sa = __ldg(reinterpret_cast<const float4*>(row + ea / 2)), sb = __ldg(reinterpret_cast<const float4*>(row + (ea + ahead) / 2));
-        c[0] = ca.x; c[1] = ca.y; c[2] = ca.z; c[3] = ca.w; c[4] = cb.x; c[5] = cb.y; c[6] = cb.z; c[7] = cb.w;
-        s[0] = sa.x; s[1] = sa.y; s[2] = sa.z; s[3] = sa.w; s[4] = sb.x; s[5] = sb.y; s[6] = sb.z; s[7] = sb.w;
+        c[0] = pair(ca.x, ca.y); c[1] = pair(ca.z, ca.w); c[2] = pair(cb.x, cb.y); c[3] = pair(cb.z, cb.w);
+        s[0] = pair(sa.x, sa.y); s[1] = pair(sa.z, sa.w); s[2] = pair(sb.x, sb.y); s[3] = pair(sb.z, sb.w);
       } else {
         load8f(row + ea, c);
         load8f(row + R / 2 + ea, s);
       }
     } else {
+      const float nan = __int_as_float(0x7FC00000);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) c[i] = s[i] = __int_as_float(0x7FC00000);
+      for (int i = 0; i < 4; ++i) c[i] = s[i] = pair(nan, nan);
     }
   }
   const float* weight = kind ? a.k_weight : a.q_weight;
   if (weight && live) {
     load8f(weight + ea, w);
-    load8f(weight + ea + ahead, w + 8);
+    load8f(weight + ea + ahead, w + 4);
   }
   while (left-- > 0) {
-    float x[16];
-    unpack8(na, x);
-    unpack8(nb, x + 8);
+    uint64_t x[8];
+    unpack8<DT>(na, x);
+    unpack8<DT>(nb, x + 4);
     if (left > 0 && live) {
       src += in_step;
       na = load8<DT>(src);
       nb = load8<DT>(src + ahead);
     }
     if (weight) {
-      float ss = 0.f;
+      uint64_t sq[2] = {0, 0};
       if (live) {
 #pragma unroll
-        for (int i = 0; i < 16; ++i) ss = fmaf(x[i], x[i], ss);
+        for (int i = 0; i < 8; ++i) sq[i & 1] = fma2(x[i], x[i], sq[i & 1]);
       }
+      const float2 f = split(add2(sq[0], sq[1]));
+      float ss = f.x + f.y;
 #pragma unroll
       for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
-      const float r = 1.0f / sqrtf(ss / float(D) + a.eps);
+      const float r = rsqrtf(fmaf(ss, p.inv_dim, a.eps));
+      const uint64_t r2 = pair(r, r);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] *= r * w[i];
+      for (int i = 0; i < 8; ++i) x[i] = mul2(x[i], mul2(r2, w[i]));
     }
     if (turned) {
+      if constexpr (INTERLEAVED) {  // a packed pair is a rotated pair
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        // pair i: (i, i + 8) of this lane's sixteen, or its neighbours (2i, 2i + 1)
-        const int ia = INTERLEAVED ? 2 * i : i, ib = INTERLEAVED ? 2 * i + 1 : i + 8;
-        const float u = x[ia], v = x[ib];
-        x[ia] = u * c[i] - v * s[i];
-        x[ib] = v * c[i] + u * s[i];
+        for (int i = 0; i < 8; ++i) {
+          const float2 u = split(x[i]), c2 = split(c[i >> 1]), s2 = split(s[i >> 1]);
+          const float cc = i & 1 ? c2.y : c2.x, sn = i & 1 ? s2.y : s2.x;
+          x[i] = pair(u.x * cc - u.y * sn, u.y * cc + u.x * sn);
+        }
+      } else {  // pair i is (i, i + 8) of this lane's sixteen
+        const uint64_t minus = pair(-1.0f, -1.0f);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint64_t u = x[i], v = x[i + 4];
+          x[i] = fma2(mul2(v, s[i]), minus, mul2(u, c[i]));
+          x[i + 4] = fma2(v, c[i], mul2(u, s[i]));
+        }
       }
     }
     if (!live) continue;
-    const Vec8<DT> va = pack8<DT>(x), vb = pack8<DT>(x + 8);
+    const Vec8<DT> va = pack8<DT>(x), vb = pack8<DT>(x + 4);
     if (dst) {
       store8<DT>(dst, va);
       store8<DT>(dst + ahead, vb);
@@ -322,6 +356,7 @@ extern "C" int smaq_norm_rope(const smaq_norm_rope_args* args, void* stream) {
   p.heads = a.n_q_heads + a.n_kv_heads * (cache ? 2 : 1);
   p.per = 1;
   p.groups = p.heads;
+  p.inv_dim = 1.0f / float(a.head_dim);
   p.page_div = make_fastdiv(cache ? a.page_size : 1);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   const int64_t e = a.dtype == SMAQ_F32 ? 4 : 2;  // every vector on a 16-byte boundary
