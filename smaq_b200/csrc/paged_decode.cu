@@ -20,8 +20,10 @@
 // keeps 16-bit rounding out of the weights.  Slots past the visible range are filled with zeros by the copy and
 // their scores replaced, so what they hold never matters.
 //
-// paged_simt_kernel (fp32 caches, other head dims and alignments): 16 groups of eight lanes, one token a
-// group, up to four query rows a tile, FMA; scores and weights stay in 32 bits.
+// paged_decode_f32_kernel (fp32, head_dim 64 / 128): the same rings; FMA throughout, since tf32 products in three parts
+// left 2e-6 in the scores (rounding inside the tensor cores' sums).
+// paged_simt_kernel (other head dims and alignments): 16 groups of eight lanes, one token a group, four query
+// rows a tile.
 #include "paged.cuh"
 
 namespace smaq {
@@ -225,20 +227,83 @@ __device__ __noinline__ void redo_row(const PagedParams& p, int b, int h, int lo
     if (lane + 32 * k < D) acc[lane + 32 * k] = o[k];
 }
 
+// Stages of 16 tokens, keys then values, of ROW bytes a token: a warp's ring.
+template <int ROW>
+struct Stages {
+  static constexpr int BYTES = 16 * ROW * 2;
+  static constexpr int N = ROW == 128 ? 6 : 3;
+  static constexpr int CTAS = ROW == 512 ? 1 : 2;                // an SM
+};
+
+// A warp's copies: the walk runs ahead of the computing one by N - 1 units, its page lookups by one more.
+template <class T, int ROW>
+struct Feed {
+  using S = Stages<ROW>;
+  static constexpr int CH = ROW / 16;  // 16-byte chunks a token; chunk c of row r lies at c ^ (r % 8)
+  Walk in;
+  int count, looked = 0, issued = 0;
+  int64_t row_off = -1;  // offset of token (lane & 15) of the unit looked up last, < 0: not visible
+  uint8_t* ring;
+
+  __device__ __forceinline__ void start(const DecodeParamsX& d, int b, int64_t into, int units, uint8_t* at) {
+    in.start(d, b, into);
+    count = units;
+    ring = at;
+    look_up(d);
+#pragma unroll 1
+    for (int i = 0; i < S::N - 1; ++i) {
+      issue(d);
+      look_up(d);
+    }
+  }
+  __device__ __forceinline__ void look_up(const DecodeParamsX& d) {
+    if (looked >= count) return;
+    if (looked) in.next(d);
+    ++looked;
+    const int lane = threadIdx.x & 31, j = in.v.lo + in.t * PD_UNIT + (threadIdx.x >> 5) * 16 + (lane & 15);
+    row_off = -1;
+    if (j < in.v.hi)
+      row_off = token_offset(d.p, d.p.a.block_table + in.b * d.p.a.table_stride, j) + int64_t(in.s / d.tiles) * d.p.a.c_stride_h;
+  }
+  __device__ __forceinline__ void issue(const DecodeParamsX& d) {
+    if (issued < count) {
+      const int lane = threadIdx.x & 31;
+      const uint32_t st = smem_u32(ring + (issued % S::N) * S::BYTES);
+#pragma unroll
+      for (int i = 0; i < 16 * CH / 32; ++i) {
+        const int r = (i * 32 + lane) / CH, ch = (i * 32 + lane) % CH;
+        const int64_t off = __shfl_sync(~0u, row_off, r);
+        const uint32_t at = st + uint32_t(r * ROW + ((ch ^ (r & 7)) << 4));
+        const int64_t from = (off < 0 ? 0 : off) + ch * int(16 / sizeof(T));
+        const uint32_t n = off < 0 ? 0u : 16u;
+        cp_async16(at, static_cast<const T*>(d.p.a.k_cache) + from, n);
+        cp_async16(at + 16 * ROW, static_cast<const T*>(d.p.a.v_cache) + from, n);
+      }
+      ++issued;
+    }
+    cp_async_commit();
+  }
+  // Stage of unit i, whole; the copies of unit i + N - 1 go into the stage of the unit before it.
+  __device__ __forceinline__ uint8_t* stage(const DecodeParamsX& d, int i) {
+    cp_async_wait<S::N - 2>();
+    __syncwarp();
+    issue(d);
+    look_up(d);
+    return ring + (i % S::N) * S::BYTES;
+  }
+};
+
 template <int D>
 struct Cfg {
-  static constexpr int STAGE = 16 * D * 2 * 2;                   // bytes: 16 tokens, K and V
-  static constexpr int STAGES = D == 64 ? 6 : 3;
+  using S = Stages<2 * D>;
   static constexpr int LD = D + 2;                               // floats of a merge row: accumulator, m, sum
-  static constexpr int SMEM = 4 * STAGES * STAGE + 2 * 16 * LD * 4;
-  static constexpr int CTAS = D == 256 ? 1 : 2;                  // an SM
+  static constexpr int SMEM = 4 * S::N * S::BYTES + 2 * 16 * LD * 4;
 };
 
 template <class DT, int D, bool CAP>
-__global__ void __launch_bounds__(PD_THREADS, Cfg<D>::CTAS) paged_decode_kernel(const __grid_constant__ DecodeParamsX d) {
+__global__ void __launch_bounds__(PD_THREADS, Stages<2 * D>::CTAS) paged_decode_kernel(const __grid_constant__ DecodeParamsX d) {
   using T = typename DT::T;
-  constexpr int STAGE = Cfg<D>::STAGE, STAGES = Cfg<D>::STAGES, LD = Cfg<D>::LD;
-  constexpr int CH = D / 8;         // 16-byte chunks a row
+  constexpr int LD = Cfg<D>::LD;
   constexpr int KS = D / 16;        // contraction steps of the scores
   constexpr int NT = D / 8;         // output column tiles
   extern __shared__ __align__(128) uint8_t smem[];
@@ -255,45 +320,10 @@ __global__ void __launch_bounds__(PD_THREADS, Cfg<D>::CTAS) paged_decode_kernel(
   const int count = int(u1 - u0);
   if (count <= 0) return;
 
-  uint8_t* ring = smem + warp * STAGES * STAGE;
-  float* merge = reinterpret_cast<float*>(smem + 4 * STAGES * STAGE);
-
-  // ---- copies: the walk `in` runs ahead of the computing walk by STAGES - 1 units, its lookups by one more
-  Walk in;
-  in.start(d, run.b, run.into);
-  int looked = 0, issued = 0;
-  int64_t row_off = -1;  // offset of token (lane & 15) of the unit looked up last, < 0: not visible
-  auto look_up = [&]() {
-    if (looked >= count) return;
-    if (looked) in.next(d);
-    ++looked;
-    const int j = in.v.lo + in.t * PD_UNIT + warp * 16 + (lane & 15);
-    row_off = -1;
-    if (j < in.v.hi) row_off = token_offset(p, a.block_table + in.b * a.table_stride, j) + int64_t(in.s / d.tiles) * a.c_stride_h;
-  };
-  auto issue = [&]() {
-    if (issued < count) {
-      const uint32_t st = smem_u32(ring + (issued % STAGES) * STAGE);
-#pragma unroll
-      for (int i = 0; i < 16 * CH / 32; ++i) {
-        const int r = (i * 32 + lane) / CH, ch = (i * 32 + lane) % CH;
-        const int64_t off = __shfl_sync(~0u, row_off, r);
-        const uint32_t at = st + uint32_t(r * D * 2 + ((ch ^ (r & 7)) << 4));
-        const int64_t from = (off < 0 ? 0 : off) + ch * 8;
-        const uint32_t n = off < 0 ? 0u : 16u;
-        cp_async16(at, static_cast<const T*>(a.k_cache) + from, n);
-        cp_async16(at + 16 * D * 2, static_cast<const T*>(a.v_cache) + from, n);
-      }
-      ++issued;
-    }
-    cp_async_commit();
-  };
-  look_up();
-#pragma unroll 1
-  for (int i = 0; i < STAGES - 1; ++i) {
-    issue();
-    look_up();
-  }
+  using S = Stages<2 * D>;
+  float* merge = reinterpret_cast<float*>(smem + 4 * S::N * S::BYTES);
+  Feed<T, 2 * D> feed;
+  feed.start(d, run.b, run.into, count, smem + warp * S::N * S::BYTES);
 
   // ---- compute
   Walk at;
@@ -330,14 +360,9 @@ __global__ void __launch_bounds__(PD_THREADS, Cfg<D>::CTAS) paged_decode_kernel(
         slope1 = r1 < rows ? a.slopes[first + r1] * kLog2e : 0.f;
       }
     }
-    cp_async_wait<STAGES - 2>();
-    __syncwarp();
-    issue();
-    look_up();
-
+    const uint32_t ks = smem_u32(feed.stage(d, i)), vs = ks + 16 * D * 2;
     const int j0 = at.v.lo + at.t * PD_UNIT + warp * 16;
     if (j0 < at.v.hi) {
-      const uint32_t ks = smem_u32(ring + (i % STAGES) * STAGE), vs = ks + 16 * D * 2;
       float c[2][4] = {};
       // keys: tokens 0-7 / 8-15 (matrix pairs), channels 16k .. 16k + 15
       const int kr = (lane & 7) + ((lane >> 4) << 3), kc = (lane >> 3) & 1;
@@ -475,12 +500,10 @@ __global__ void __launch_bounds__(PD_THREADS, Cfg<D>::CTAS) paged_decode_kernel(
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
               const float2 x = *reinterpret_cast<const float2*>(merge + n * 8 + col);
-              if (r == r0) {
-                o[n][0] = x.x;
-                o[n][1] = x.y;
-              } else if (r == r1) {
-                o[n][2] = x.x;
-                o[n][3] = x.y;
+              const int e = r < 8 ? 0 : 2;
+              if (r == (e ? r1 : r0)) {  // finite elements stay as they are
+                if (!isfinite(e ? o[n][2] : o[n][0])) (e ? o[n][2] : o[n][0]) = x.x;
+                if (!isfinite(e ? o[n][3] : o[n][1])) (e ? o[n][3] : o[n][1]) = x.y;
               }
             }
             __syncwarp();
@@ -512,6 +535,187 @@ __global__ void __launch_bounds__(PD_THREADS, Cfg<D>::CTAS) paged_decode_kernel(
           }
         }
       }
+      fresh = true;
+      from = 0;
+    }
+    if (i + 1 < count) at.next(d);
+  }
+}
+
+// ---------------------------------------------------------------- fp32
+// R query heads a tile.  Scores: lane = (half of the channels, token), so that a 16-token stage takes one exchange a
+// row; weighted values: lane = D / 32 channels, the weights broadcast from shared memory.
+template <int D, int R>
+struct FCfg {
+  using S = Stages<4 * D>;
+  static constexpr int QH = D / 2 + 4;                 // floats of half a query row: the halves start four banks apart
+  static constexpr int AREA = R * 2 * QH;              // a warp's query rows, at the end of a segment its accumulators
+  static constexpr int SMEM = 4 * (S::N * S::BYTES + (AREA + 16 * R) * 4);
+};
+
+template <int D, int R, bool CAP>
+__global__ void __launch_bounds__(PD_THREADS, Stages<4 * D>::CTAS) paged_decode_f32_kernel(const __grid_constant__ DecodeParamsX d) {
+  using Q = FCfg<D, R>;
+  using S = Stages<4 * D>;
+  constexpr int E = D / 32, LD = D + 2;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int64_t warp_sums[PD_THREADS / 32], found_into;
+  __shared__ int found_b;
+  const PagedParams& p = d.p;
+  const smaq_paged_args& a = p.a;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_launch_dependents();
+  write_empty(d);
+  const RunStart run = find_run(d, warp_sums, &found_b, &found_into, [&](int64_t total) { return run_first(blockIdx.x, total, d.grid); });
+  const int64_t u0 = run_first(blockIdx.x, run.total, d.grid), u1 = run_first(int64_t(blockIdx.x) + 1, run.total, d.grid);
+  const int count = int(u1 - u0);
+  if (count <= 0) return;
+  Feed<float, 4 * D> feed;
+  feed.start(d, run.b, run.into, count, smem + warp * S::N * S::BYTES);
+  float* areas = reinterpret_cast<float*>(smem + 4 * S::N * S::BYTES);
+  float *mine = areas + warp * Q::AREA, *ps = areas + 4 * Q::AREA + warp * 16 * R;
+
+  Walk at;
+  at.start(d, run.b, run.into);
+  const int tok = lane & 15, half = lane >> 4;
+  float o[R][E], m[R], l[R], slope[R];
+  bool fresh = true;
+  int from = at.t;
+#pragma unroll 1
+  for (int i = 0; i < count; ++i) {
+    const int kvh = at.s / d.tiles, tile = at.s - kvh * d.tiles;
+    const int first = kvh * p.group + tile * R, rows = min(R, p.group - tile * R);
+    if (fresh) {
+      fresh = false;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        m[r] = -INFINITY;
+        l[r] = 0.f;
+        slope[r] = a.slopes && r < rows ? a.slopes[first + r] * kLog2e : 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[r][e] = 0.f;
+      }
+      for (int k = lane; k < R * D; k += 32) {
+        const int r = k / D, e = k % D;
+        mine[(2 * r + e / (D / 2)) * Q::QH + e % (D / 2)] =
+            r < rows ? static_cast<const float*>(a.q)[at.b * a.q_stride_t + (first + r) * a.q_stride_h + e] : 0.f;
+      }
+    }
+    const uint8_t* ks = feed.stage(d, i);  // waits for the whole warp: the query rows are there too
+    const uint8_t* vs = ks + 16 * 4 * D;
+    const int j0 = at.v.lo + at.t * PD_UNIT + warp * 16, last = at.v.hi - 1;
+    if (j0 <= last) {
+      float x[R];
+#pragma unroll
+      for (int r = 0; r < R; ++r) x[r] = 0.f;
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) {
+        const float4 k = *reinterpret_cast<const float4*>(ks + tok * 4 * D + (((half * (D / 8) + c) ^ (tok & 7)) << 4));
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const float4 q = *reinterpret_cast<const float4*>(mine + (2 * r + half) * Q::QH + 4 * c);
+          x[r] = fmaf(q.x, k.x, fmaf(q.y, k.y, fmaf(q.z, k.z, fmaf(q.w, k.w, x[r]))));
+        }
+      }
+      const int j = j0 + tok;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        float y = x[r] + __shfl_xor_sync(~0u, x[r], 16);
+        if constexpr (CAP) y = a.softcap * kLog2e * tanhf(y * a.scale / a.softcap);
+        else y *= p.scale_log2;
+        y = j <= last ? y - slope[r] * float(last - j) : -INFINITY;
+        if (__any_sync(~0u, y > m[r])) {
+          float n = fmaxf(m[r], y);
+#pragma unroll
+          for (int w = 8; w > 0; w >>= 1) n = fmaxf(n, __shfl_xor_sync(~0u, n, w));
+          const float f = m[r] == -INFINITY ? 0.f : ex2(m[r] - n);
+          m[r] = n;
+          l[r] *= f;
+#pragma unroll
+          for (int e = 0; e < E; ++e) o[r][e] *= f;
+        }
+        x[r] = ex2(y - (m[r] == -INFINITY ? 0.f : m[r]));
+        l[r] += x[r];
+      }
+      if (half == 0) {
+#pragma unroll
+        for (int r = 0; r < R; r += 4) *reinterpret_cast<float4*>(ps + tok * R + r) = make_float4(x[r], x[r + 1], x[r + 2], x[r + 3]);
+      }
+      __syncwarp();
+#pragma unroll
+      for (int t = 0; t < 16; ++t) {
+        float v[E];
+        const uint8_t* row = vs + t * 4 * D;
+        if constexpr (E == 2) {
+          const float2 u = *reinterpret_cast<const float2*>(row + (((lane >> 1) ^ (t & 7)) << 4) + (lane & 1) * 8);
+          v[0] = u.x;
+          v[1] = u.y;
+        } else {
+          const float4 u = *reinterpret_cast<const float4*>(row + ((lane ^ (t & 7)) << 4));
+          v[0] = u.x;
+          v[1] = u.y;
+          v[2] = u.z;
+          v[3] = u.w;
+        }
+#pragma unroll
+        for (int r = 0; r < R; r += 4) {
+          const float4 w = *reinterpret_cast<const float4*>(ps + t * R + r);
+#pragma unroll
+          for (int e = 0; e < E; ++e) {
+            o[r][e] = fmaf(w.x, v[e], o[r][e]);
+            o[r + 1][e] = fmaf(w.y, v[e], o[r + 1][e]);
+            o[r + 2][e] = fmaf(w.z, v[e], o[r + 2][e]);
+            o[r + 3][e] = fmaf(w.w, v[e], o[r + 3][e]);
+          }
+        }
+      }
+      __syncwarp();  // before the weights of the next stage
+    }
+
+    const bool ends = at.t + 1 == at.v.units;
+    if (ends || i + 1 == count) {
+      // ---- the four warps' states into one
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+#pragma unroll
+        for (int w = 8; w > 0; w >>= 1) l[r] += __shfl_xor_sync(~0u, l[r], w);
+#pragma unroll
+        for (int e = 0; e < E; ++e) mine[r * LD + E * lane + e] = o[r][e];
+        if (lane == 0) {
+          mine[r * LD + D] = m[r];
+          mine[r * LD + D + 1] = l[r];
+        }
+      }
+      __syncthreads();
+      const bool all = ends && from == 0;
+      float* slot = d.slots + (int64_t(blockIdx.x) + int64_t(at.b) * d.segs + at.s) * d.rows * LD;
+      for (int k = threadIdx.x; k < rows * D; k += PD_THREADS) {
+        const int r = k / D, e = k - r * D;
+        float mm = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) mm = fmaxf(mm, areas[w * Q::AREA + r * LD + D]);
+        const float z = mm == -INFINITY ? 0.f : mm;
+        float x = 0.f, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const float f = ex2(areas[w * Q::AREA + r * LD + D] - z);
+          if (f > 0.f || f != f) {  // a warp without tokens holds zeros
+            x += f * areas[w * Q::AREA + r * LD + e];
+            sum += f * areas[w * Q::AREA + r * LD + D + 1];
+          }
+        }
+        if (all) {
+          static_cast<float*>(a.out)[at.b * a.o_stride_t + (first + r) * a.o_stride_h + e] = sum == 0.f ? 0.f : x / sum;
+          if (a.lse && e == 0) a.lse[int64_t(at.b) * a.n_q_heads + first + r] = (mm + log2f(sum)) * kLn2;
+        } else {
+          slot[r * LD + e] = x;
+          if (e == 0) {
+            slot[r * LD + D] = mm;
+            slot[r * LD + D + 1] = sum;
+          }
+        }
+      }
+      __syncthreads();  // before the areas hold the next segment's queries
       fresh = true;
       from = 0;
     }
@@ -765,20 +969,31 @@ __global__ void __launch_bounds__(PD_THREADS) paged_join_kernel(const __grid_con
   if (a.lse && threadIdx.x == 0) a.lse[int64_t(b) * a.n_q_heads + h] = (m + log2f(sum)) * kLn2;
 }
 
-bool mma_eligible(const smaq_paged_args& a) {
-  return a.dtype != SMAQ_F32 && (a.head_dim == 64 || a.head_dim == 128 || a.head_dim == 256) && paged_aligned(a);
+constexpr int PS_CTAS = 4;  // CTAs an SM of the SIMT kernel
+
+// Which kernel: the ring kernels take head_dim 64, 128 and (16-bit) 256 on 16-byte boundaries.
+enum { PATH_SIMT, PATH_MMA, PATH_F32 };
+struct Shape {
+  int path, tile, ctas;  // query heads a tile, CTAs an SM
+};
+Shape shape_of(int dtype, int head_dim, int group, bool aligned) {
+  const bool ring = aligned && (head_dim == 64 || head_dim == 128 || (head_dim == 256 && dtype != SMAQ_F32));
+  if (!ring) return {PATH_SIMT, PS_ROWS, PS_CTAS};
+  if (dtype == SMAQ_F32) return {PATH_F32, group > 4 ? 8 : 4, head_dim == 64 ? 2 : 1};
+  return {PATH_MMA, 16, head_dim == 256 ? 1 : 2};
 }
 
-constexpr int PS_CTAS = 4;  // CTAs an SM of the SIMT kernel
-int tile_rows_of(bool mma) { return mma ? 16 : PS_ROWS; }
-
+template <class K>
+int launch_ring(K kern, int smem, const DecodeParamsX& d, cudaStream_t st) {
+  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (e != cudaSuccess) return cuda_status(e, "paged_decode attr");
+  kern<<<d.grid, PD_THREADS, smem, st>>>(d);
+  return cuda_status(cudaGetLastError(), "paged_decode");
+}
 template <class DT, int D>
 int launch_mma(const DecodeParamsX& d, cudaStream_t st) {
-  auto kern = d.p.a.softcap > 0.f ? paged_decode_kernel<DT, D, true> : paged_decode_kernel<DT, D, false>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM);
-  if (e != cudaSuccess) return cuda_status(e, "paged_decode attr");
-  kern<<<d.grid, PD_THREADS, Cfg<D>::SMEM, st>>>(d);
-  return cuda_status(cudaGetLastError(), "paged_decode");
+  return d.p.a.softcap > 0.f ? launch_ring(paged_decode_kernel<DT, D, true>, Cfg<D>::SMEM, d, st)
+                             : launch_ring(paged_decode_kernel<DT, D, false>, Cfg<D>::SMEM, d, st);
 }
 template <class DT>
 int launch_mma_dim(const DecodeParamsX& d, cudaStream_t st) {
@@ -787,6 +1002,11 @@ int launch_mma_dim(const DecodeParamsX& d, cudaStream_t st) {
     case 128: return launch_mma<DT, 128>(d, st);
     default: return launch_mma<DT, 256>(d, st);
   }
+}
+template <int D, int R>
+int launch_f32(const DecodeParamsX& d, cudaStream_t st) {
+  return d.p.a.softcap > 0.f ? launch_ring(paged_decode_f32_kernel<D, R, true>, FCfg<D, R>::SMEM, d, st)
+                             : launch_ring(paged_decode_f32_kernel<D, R, false>, FCfg<D, R>::SMEM, d, st);
 }
 template <class DT>
 int launch_simt(const DecodeParamsX& d, cudaStream_t st) {
@@ -808,15 +1028,16 @@ int launch_simt(const DecodeParamsX& d, cudaStream_t st) {
 extern "C" size_t smaq_paged_decode_workspace_size(int batch, int n_q_heads, int n_kv_heads, int head_dim) {
   using namespace smaq;
   if (batch <= 0 || n_kv_heads <= 0 || n_q_heads < n_kv_heads || head_dim <= 0) return 0;
-  // enough for either kernel: the one with fewer rows a tile has as many rows in all
+  // enough for whichever kernel the dtype and alignment choose
   const int group = n_q_heads / n_kv_heads;
   size_t most = 0;
-  for (const bool mma : {false, true}) {
-    const int tr = tile_rows_of(mma), tiles = (group + tr - 1) / tr, rows = group < tr ? group : tr;
-    const int ctas = num_sms() * (mma ? (head_dim == 256 ? 1 : 2) : PS_CTAS);
-    const size_t n = (size_t(ctas) + size_t(batch) * n_kv_heads * tiles) * rows * (head_dim + 2) * sizeof(float);
-    most = n > most ? n : most;
-  }
+  for (const int dtype : {SMAQ_F32, SMAQ_BF16})
+    for (const bool aligned : {false, true}) {
+      const Shape s = shape_of(dtype, head_dim, group, aligned);
+      const int tiles = (group + s.tile - 1) / s.tile, rows = group < s.tile ? group : s.tile;
+      const size_t n = (size_t(num_sms()) * s.ctas + size_t(batch) * n_kv_heads * tiles) * rows * (head_dim + 2) * sizeof(float);
+      most = n > most ? n : most;
+    }
   return most;
 }
 
@@ -831,16 +1052,18 @@ extern "C" int smaq_paged_decode(const smaq_paged_args* args, void* stream) {
   if (!a.workspace || a.workspace_bytes < need)
     return fail(SMAQ_ERR_WORKSPACE, "paged_decode: workspace %zu bytes, needs %zu", a.workspace ? a.workspace_bytes : size_t(0), need);
   if (reinterpret_cast<uintptr_t>(a.workspace) % 16) return fail(SMAQ_ERR_INVALID, "paged_decode: workspace must be 16-byte aligned");
-  const bool mma = mma_eligible(a);
-  const int tr = tile_rows_of(mma);
-  d.tiles = (d.p.group + tr - 1) / tr;
-  d.rows = d.p.group < tr ? d.p.group : tr;
+  const Shape sh = shape_of(a.dtype, a.head_dim, d.p.group, paged_aligned(a));
+  d.tiles = (d.p.group + sh.tile - 1) / sh.tile;
+  d.rows = d.p.group < sh.tile ? d.p.group : sh.tile;
   d.segs = a.n_kv_heads * d.tiles;
-  d.grid = num_sms() * (mma ? (a.head_dim == 256 ? 1 : 2) : PS_CTAS);
+  d.grid = num_sms() * sh.ctas;
   d.slots = static_cast<float*>(a.workspace);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   int rc;
-  if (mma) rc = a.dtype == SMAQ_BF16 ? launch_mma_dim<BF16>(d, st) : launch_mma_dim<F16>(d, st);
+  if (sh.path == PATH_MMA) rc = a.dtype == SMAQ_BF16 ? launch_mma_dim<BF16>(d, st) : launch_mma_dim<F16>(d, st);
+  else if (sh.path == PATH_F32)
+    rc = a.head_dim == 64 ? (sh.tile == 4 ? launch_f32<64, 4>(d, st) : launch_f32<64, 8>(d, st))
+                          : (sh.tile == 4 ? launch_f32<128, 4>(d, st) : launch_f32<128, 8>(d, st));
   else rc = a.dtype == SMAQ_F32 ? launch_simt<F32>(d, st) : a.dtype == SMAQ_BF16 ? launch_simt<BF16>(d, st) : launch_simt<F16>(d, st);
   if (rc) return rc;
   cudaLaunchConfig_t cfg = {};
@@ -853,5 +1076,5 @@ extern "C" int smaq_paged_decode(const smaq_paged_args* args, void* stream) {
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, paged_join_kernel, d, tr), "paged_decode join");
+  return cuda_status(cudaLaunchKernelEx(&cfg, paged_join_kernel, d, sh.tile), "paged_decode join");
 }
