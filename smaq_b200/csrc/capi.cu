@@ -40,6 +40,26 @@ int num_sms() {
   return n;
 }
 
+int allow_smem(const void* kernel, int bytes, const char* where) {
+  struct Grant {
+    const void* kernel;
+    int dev, bytes;
+  };
+  static thread_local Grant known[64];  // one more question to the driver a thread costs nothing; a lock would
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return cuda_status(e, where);
+  Grant* slot = nullptr;
+  for (Grant& g : known) {
+    if (g.kernel == kernel && g.dev == dev && g.bytes >= bytes) return SMAQ_OK;
+    if (!slot && (!g.kernel || (g.kernel == kernel && g.dev == dev))) slot = &g;
+  }
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return cuda_status(e, where);
+  if (slot) *slot = {kernel, dev, bytes};
+  return SMAQ_OK;
+}
+
 }  // namespace smaq
 
 extern "C" int smaq_abi_version(void) { return SMAQ_ABI_VERSION; }

@@ -15,6 +15,8 @@ void set_error(const char* fmt, ...);
 int fail(int code, const char* fmt, ...);
 int cuda_status(cudaError_t e, const char* where);
 int num_sms();
+// Lets `kernel` use `bytes` of dynamic shared memory on the current device; asked of the driver once a device.
+int allow_smem(const void* kernel, int bytes, const char* where);
 
 // ---------------------------------------------------------------- dtype tags
 struct F32 {

@@ -985,8 +985,7 @@ Shape shape_of(int dtype, int head_dim, int group, bool aligned) {
 
 template <class K>
 int launch_ring(K kern, int smem, const DecodeParamsX& d, cudaStream_t st) {
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  if (e != cudaSuccess) return cuda_status(e, "paged_decode attr");
+  if (const int rc = allow_smem(reinterpret_cast<const void*>(kern), smem, "paged_decode")) return rc;
   kern<<<d.grid, PD_THREADS, smem, st>>>(d);
   return cuda_status(cudaGetLastError(), "paged_decode");
 }

@@ -348,8 +348,7 @@ int64_t most_tiles(const PagedParams& p, int size) {
 template <class DT, int D>
 int launch_mma(const PagedParams& p, cudaStream_t st) {
   auto kern = p.a.softcap > 0.f ? prefill_mma_kernel<DT, D, true> : prefill_mma_kernel<DT, D, false>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PmCfg<D>::SMEM);
-  if (e != cudaSuccess) return cuda_status(e, "paged_prefill attr");
+  if (const int rc = allow_smem(reinterpret_cast<const void*>(kern), PmCfg<D>::SMEM, "paged_prefill")) return rc;
   kern<<<dim3(unsigned(most_tiles(p, PmCfg<D>::ROWS)), p.a.n_kv_heads), PM_THREADS, PmCfg<D>::SMEM, st>>>(p);
   return cuda_status(cudaGetLastError(), "paged_prefill");
 }

@@ -21,8 +21,6 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
-#include <mutex>
-
 #include "paged_prefill.cuh"
 #include "prefill_tc.cuh"
 #include "tcgen05.cuh"
@@ -485,14 +483,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
+  static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
     void* ptr = nullptr;
     cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &ptr, 12000, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
-  });
+    const bool ok = cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &ptr, 12000, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ok ? ptr : nullptr);
+  }();
   return fn;
 }
 
@@ -526,8 +522,7 @@ int launch(const PagedParams& p, cudaStream_t st) {
   auto kern = a.slopes || !(a.scale > 0.f) ? prefill_tc_kernel<DT, D, PT_ANY>
               : a.softcap > 0.f            ? prefill_tc_kernel<DT, D, PT_CAP>
                                            : prefill_tc_kernel<DT, D, PT_PLAIN>;
-  const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PtCfg<D>::SMEM);
-  if (e != cudaSuccess) return cuda_status(e, "paged_prefill attr");
+  if (const int rc = allow_smem(reinterpret_cast<const void*>(kern), PtCfg<D>::SMEM, "paged_prefill")) return rc;
   const int64_t tiles = (p.a.n_rows * p.group + PT_ROWS - 1) / PT_ROWS + p.a.batch;
   if (tiles * a.n_kv_heads >= (int64_t(1) << 31)) return fail(SMAQ_ERR_UNSUPPORTED, "paged_prefill: too many rows");
   kern<<<unsigned(tiles * a.n_kv_heads), PT_THREADS, PtCfg<D>::SMEM, st>>>(pt);
@@ -537,6 +532,9 @@ int launch(const PagedParams& p, cudaStream_t st) {
 }  // namespace
 
 bool prefill_tc_eligible(const smaq_paged_args& a) {
+#ifdef NO_TC
+  return false;
+#endif
   return a.dtype != SMAQ_F32 && (a.head_dim == 64 || a.head_dim == 128) && paged_aligned(a);
 }
 

@@ -501,9 +501,9 @@ def _addr(t: Optional[torch.Tensor]) -> int:
 
 
 def _int32(name: str, t: torch.Tensor, n: int) -> torch.Tensor:
-    if t.dim() != 1 or t.shape[0] != n:
+    if t.shape != (n,):
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected ({n},)")
-    if t.dtype != torch.int32:
+    if t.dtype is not torch.int32:
         if t.dtype.is_floating_point or t.dtype == torch.bool:
             raise ValueError(f"{name} must be an integer tensor, got {t.dtype}")
         t = t.to(torch.int32)
@@ -524,10 +524,11 @@ def step_tables(free_blocks: torch.Tensor, free_count: torch.Tensor, context_len
     the step's tokens get position 0 and slot -1.  Nothing is read back to the host."""
     stream = _stream_for(free_blocks, (free_count, context_lens, query_lens, block_table, finished))
     B = context_lens.shape[0]
-    if free_blocks.dtype != torch.int32 or free_blocks.dim() != 1 or not free_blocks.is_contiguous():
+    if free_blocks.dtype is not torch.int32 or free_blocks.dim() != 1 or not free_blocks.is_contiguous():
         raise ValueError("free_blocks must be a contiguous int32 vector (it is updated in place)")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or block_table.shape[0] != B or (
-            block_table.shape[1] > 1 and block_table.stride(1) != 1):
+    width = block_table.shape
+    if block_table.dtype is not torch.int32 or len(width) != 2 or width[0] != B or (
+            width[1] > 1 and block_table.stride(1) != 1):
         raise ValueError(f"block_table must be int32 [{B}, M] with contiguous rows (it is updated in place)")
     if num_tokens < 0 or block_size < 1:
         raise ValueError(f"num_tokens {num_tokens} or block_size {block_size} out of range")
@@ -536,13 +537,14 @@ def step_tables(free_blocks: torch.Tensor, free_count: torch.Tensor, context_len
     if finished is not None:
         if finished.shape != (B,) or finished.dtype not in (torch.bool, torch.uint8):
             raise ValueError(f"finished must be a bool vector of length {B}")
-        finished = finished.contiguous()
+        if not finished.is_contiguous():
+            finished = finished.contiguous()
     # one buffer: slots (8 bytes) first, positions on a 16-byte boundary, the rest
-    M, T, dev = block_table.shape[1], num_tokens, free_blocks.device
+    M, T = width[1], num_tokens
     pad = (T + 3) // 4 * 4
-    buf = torch.empty(3 * pad + 2 * B + 2, dtype=torch.int32, device=dev)
+    buf = free_blocks.new_empty(3 * pad + 2 * B + 2)
     slots, _, positions, _, cu, lens, left = buf.split_with_sizes([2 * T, 2 * (pad - T), T, pad - T, B + 1, B, 1])
-    admitted = torch.empty(B, dtype=torch.bool, device=dev)
+    admitted = torch.empty(B, dtype=torch.bool, device=free_blocks.device)
     at = buf.data_ptr()
     rest = at + 12 * pad
     st = _lib.load().smaq_step_tables(
@@ -594,21 +596,35 @@ def rope_table(max_positions: int, rotary_dim: int, base: float = 10000.0, *, li
     return (torch.cat([angle.cos(), angle.sin()], 1) * gain).to(torch.float32)
 
 
-def _head_rows(name: str, x: torch.Tensor, dtype: torch.dtype, T: int, D: int) -> torch.Tensor:
-    if x.dim() != 3 or x.shape[0] != T or x.shape[2] != D or x.dtype != dtype:
-        raise ValueError(f"{name} must be {dtype} [{T}, heads, {D}], got {x.dtype} {tuple(x.shape)}")
-    return x if x.stride(2) == 1 or D == 1 else x.contiguous()
+def _head_rows(name: str, x: torch.Tensor, dtype: torch.dtype, T: int, D: int) -> tuple:
+    """``x`` with contiguous channels, its heads, token stride and head stride."""
+    shape = x.shape
+    if len(shape) != 3 or shape[0] != T or shape[2] != D or x.dtype is not dtype:
+        raise ValueError(f"{name} must be {dtype} [{T}, heads, {D}], got {x.dtype} {tuple(shape)}")
+    st, sh, sd = x.stride()
+    if sd != 1 and D > 1:
+        x = x.contiguous()
+        st, sh, _ = x.stride()
+    return x, shape[1], st, sh
 
 
-def _cache_pair(k_cache: torch.Tensor, v_cache: torch.Tensor, dtype: torch.dtype, D: int) -> None:
+def _vector_f32(name: str, w: torch.Tensor, n: int) -> torch.Tensor:
+    if w.shape != (n,):
+        raise ValueError(f"{name} has shape {tuple(w.shape)}, expected ({n},)")
+    return w if w.dtype is torch.float32 and w.is_contiguous() else w.to(torch.float32).contiguous()
+
+
+def _cache_pair(k_cache: torch.Tensor, v_cache: torch.Tensor, dtype: torch.dtype, D: int) -> tuple:
+    """Pages, page size, heads and the page, slot and head strides of a checked pair."""
     shape, strides = k_cache.shape, k_cache.stride()
     if len(shape) != 4 or shape != v_cache.shape or shape[3] != D:
         raise ValueError(f"caches must be [pages, page_size, kv_heads, {D}], got {tuple(k_cache.shape)} and "
                          f"{tuple(v_cache.shape)}")
-    if k_cache.dtype != dtype or v_cache.dtype != dtype:
+    if k_cache.dtype is not dtype or v_cache.dtype is not dtype:
         raise ValueError(f"caches must be {dtype} like the queries, got {k_cache.dtype} and {v_cache.dtype}")
     if strides != v_cache.stride() or (D > 1 and strides[3] != 1):
         raise ValueError("caches must have the same strides and a contiguous head_dim")
+    return shape[0], shape[1], shape[2], strides[0], strides[1], strides[2]
 
 
 def norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, table: torch.Tensor, *,
@@ -628,46 +644,39 @@ def norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, table: 
     dt = q.dtype
     code = dtype_code(dt)
     stream = _stream_for(q, (k, positions, table, q_weight, k_weight, v, k_cache, v_cache, slots))
-    q, k = _head_rows("q", q, dt, T, D), _head_rows("k", k, dt, T, D)
-    Hk = k.shape[1]
+    q, _, qt, qh = _head_rows("q", q, dt, T, D)
+    k, Hk, kt, kh = _head_rows("k", k, dt, T, D)
     positions = _int32("positions", positions, T)
-    if table.dim() != 2 or table.dtype != torch.float32 or table.shape[1] > D or table.shape[1] % 2:
-        raise ValueError(f"table must be float32 [positions, R] with an even R <= {D}, got {table.dtype} "
-                         f"{tuple(table.shape)}")
-    table = table.contiguous()
-
-    def weight(name, w):
-        if w is None:
-            return None
-        if w.shape != (D,):
-            raise ValueError(f"{name} must have shape ({D},), got {tuple(w.shape)}")
-        return w if w.dtype == torch.float32 and w.is_contiguous() else w.to(torch.float32).contiguous()
-    q_weight, k_weight = weight("q_weight", q_weight), weight("k_weight", k_weight)
-    given = [x is not None for x in (v, k_cache, v_cache, slots)]
-    if any(given) and not all(given):
-        raise ValueError("a cache write needs v, k_cache, v_cache and slots together")
-    q_out = torch.empty((T, Hq, D), dtype=dt, device=q.device)
+    rows = table.shape
+    if len(rows) != 2 or table.dtype is not torch.float32 or rows[1] > D or rows[1] % 2:
+        raise ValueError(f"table must be float32 [positions, R] with an even R <= {D}, got {table.dtype} {tuple(rows)}")
+    if not table.is_contiguous():
+        table = table.contiguous()
+    if q_weight is not None:
+        q_weight = _vector_f32("q_weight", q_weight, D)
+    if k_weight is not None:
+        k_weight = _vector_f32("k_weight", k_weight, D)
     k_out = None
-    vs = cs = (0, 0, 0)
-    pages = page_size = 0
-    if k_cache is not None:
-        v = _head_rows("v", v, dt, T, D)
-        _cache_pair(k_cache, v_cache, dt, D)
-        if v.shape[1] != Hk or k_cache.shape[2] != Hk:
-            raise ValueError(f"v has {v.shape[1]} heads and the cache {k_cache.shape[2]}, k has {Hk}")
+    vt = vh = pages = page_size = cp = cs = ch = 0
+    if k_cache is None and v is None and v_cache is None and slots is None:
+        k_out = k.new_empty((T, Hk, D))
+    else:
+        if k_cache is None or v is None or v_cache is None or slots is None:
+            raise ValueError("a cache write needs v, k_cache, v_cache and slots together")
+        v, Hv, vt, vh = _head_rows("v", v, dt, T, D)
+        pages, page_size, Hc, cp, cs, ch = _cache_pair(k_cache, v_cache, dt, D)
+        if Hv != Hk or Hc != Hk:
+            raise ValueError(f"v has {Hv} heads and the cache {Hc}, k has {Hk}")
         if slots.shape != (T,):
             raise ValueError(f"slots has shape {tuple(slots.shape)}, expected ({T},)")
-        slots = slots if slots.dtype == torch.int64 and slots.is_contiguous() else slots.to(torch.int64).contiguous()
-        vs, cs, pages, page_size = v.stride(), k_cache.stride(), k_cache.shape[0], k_cache.shape[1]
-    else:
-        k_out = torch.empty((T, Hk, D), dtype=dt, device=q.device)
-    qs, ks = q.stride(), k.stride()
+        if slots.dtype is not torch.int64 or not slots.is_contiguous():
+            slots = slots.to(torch.int64).contiguous()
+    q_out = q.new_empty((T, Hq, D))
     st = _lib.load().smaq_norm_rope(
-        _lib.pack_norm_rope(q.data_ptr(), k.data_ptr(), _addr(v), qs[0], qs[1], ks[0], ks[1], vs[0], vs[1],
-                            positions.data_ptr(), table.data_ptr(), _addr(q_weight), _addr(k_weight), _addr(slots),
-                            q_out.data_ptr(), _addr(k_out), _addr(k_cache), _addr(v_cache), cs[0], cs[1], cs[2], T,
-                            table.shape[0], pages, code, Hq, Hk, D, table.shape[1], int(interleaved), page_size, eps),
-        stream)
+        _lib.pack_norm_rope(q.data_ptr(), k.data_ptr(), _addr(v), qt, qh, kt, kh, vt, vh, positions.data_ptr(),
+                            table.data_ptr(), _addr(q_weight), _addr(k_weight), _addr(slots), q_out.data_ptr(),
+                            _addr(k_out), _addr(k_cache), _addr(v_cache), cp, cs, ch, T, rows[0], pages, code, Hq, Hk,
+                            D, rows[1], int(interleaved), page_size, eps), stream)
     if st:
         _lib.check(st, "smaq_norm_rope")
     return q_out, k_out
@@ -685,17 +694,20 @@ def _paged(name, q, k_cache, v_cache, block_table, seq_lens, cu_query, prefix_le
     dt = q.dtype
     code = dtype_code(dt)
     stream = _stream_for(q, (k_cache, v_cache, block_table, seq_lens, cu_query, prefix_lens, slopes, out, workspace))
-    if q.stride(2) != 1 and D > 1:
+    qt, qh, qd = q.stride()
+    if qd != 1 and D > 1:
         q = q.contiguous()
-    _cache_pair(k_cache, v_cache, dt, D)
-    P, page_size, Hk, _ = k_cache.shape
+        qt, qh, _ = q.stride()
+    P, page_size, Hk, cp, cs, ch = _cache_pair(k_cache, v_cache, dt, D)
     if block_table.dim() != 2:
         raise ValueError(f"block_table must be [batch, blocks], got {tuple(block_table.shape)}")
     B, M = block_table.shape
-    if block_table.dtype != torch.int32:
+    if block_table.dtype is not torch.int32:
         block_table = block_table.to(torch.int32)
-    if M > 1 and block_table.stride(1) != 1:
+    row, col = block_table.stride()
+    if M > 1 and col != 1:
         block_table = block_table.contiguous()
+        row = M
     seq_lens = _int32("seq_lens", seq_lens, B)
     if Hk == 0 or Hq % Hk:
         raise ValueError(f"{Hq} query heads do not divide over {Hk} KV heads")
@@ -706,33 +718,30 @@ def _paged(name, q, k_cache, v_cache, block_table, seq_lens, cu_query, prefix_le
     if prefix_lens is not None:
         prefix_lens = _int32("prefix_lens", prefix_lens, B)
     if slopes is not None:
-        if slopes.shape != (Hq,):
-            raise ValueError(f"slopes has shape {tuple(slopes.shape)}, expected ({Hq},)")
-        if slopes.dtype != torch.float32 or not slopes.is_contiguous():
-            slopes = slopes.to(torch.float32).contiguous()
+        slopes = _vector_f32("slopes", slopes, Hq)
     if out is None:
-        out = torch.empty((T, Hq, D), dtype=dt, device=q.device)
-    elif out.shape != q.shape or out.dtype != dt or (D > 1 and out.stride(2) != 1):
+        out = q.new_empty((T, Hq, D))
+    elif out.shape != q.shape or out.dtype is not dt or (D > 1 and out.stride(2) != 1):
         raise ValueError(f"out must be {dt} {tuple(q.shape)} with a contiguous head_dim")
     lse = torch.empty((T, Hq), dtype=torch.float32, device=q.device) if return_lse else None
-    qs, cs, os = q.stride(), k_cache.stride(), out.stride()
+    ot, oh, _ = out.stride()
     lib = _lib.load()
+    ws = ws_bytes = 0
     if cu_query is None:
         if T != B:
             raise ValueError(f"q has {T} rows for {B} requests; one row a request")
-        need = lib.smaq_paged_decode_workspace_size(B, Hq, Hk, D)
         if workspace is None:
-            workspace = torch.empty((need,), dtype=torch.uint8, device=q.device)
+            workspace = torch.empty(lib.smaq_paged_decode_workspace_size(B, Hq, Hk, D), dtype=torch.uint8,
+                                    device=q.device)
         ws, ws_bytes, call = workspace.data_ptr(), workspace.numel() * workspace.element_size(), lib.smaq_paged_decode
     else:
         cu_query = _int32("cu_query", cu_query, B + 1)
-        ws, ws_bytes, call = 0, 0, lib.smaq_paged_prefill
+        call = lib.smaq_paged_prefill
     st = call(
-        _lib.pack_paged(q.data_ptr(), qs[0], qs[1], k_cache.data_ptr(), v_cache.data_ptr(), cs[0], cs[1], cs[2],
-                        block_table.data_ptr(), max(block_table.stride(0), M), seq_lens.data_ptr(), _addr(cu_query),
-                        _addr(prefix_lens), _addr(slopes), out.data_ptr(), os[0], os[1], _addr(lse), ws, ws_bytes, P, T,
-                        B, M, page_size, Hq, Hk, D, code, window or 0, 1.0 / math.sqrt(D) if scale is None else scale,
-                        softcap or 0.0), stream)
+        _lib.pack_paged(q.data_ptr(), qt, qh, k_cache.data_ptr(), v_cache.data_ptr(), cp, cs, ch,
+                        block_table.data_ptr(), max(row, M), seq_lens.data_ptr(), _addr(cu_query), _addr(prefix_lens),
+                        _addr(slopes), out.data_ptr(), ot, oh, _addr(lse), ws, ws_bytes, P, T, B, M, page_size, Hq, Hk,
+                        D, code, window or 0, 1.0 / math.sqrt(D) if scale is None else scale, softcap or 0.0), stream)
     if st:
         _lib.check(st, name)
     return (out, lse) if return_lse else out
