@@ -462,7 +462,8 @@ int smaq_norm_rope(const smaq_norm_rope_args* args, void* stream);
  * read leaves the cache.  lse: natural log of the sum of exp(score), [rows, n_q_heads].
  *   smaq_paged_decode: one row per request (cu_query, prefix_lens unused), the cache split over the
  *     GPU by length and joined; needs smaq_paged_decode_workspace_size bytes of workspace.
- *   smaq_paged_prefill: n_rows rows. */
+ *   smaq_paged_prefill: n_rows rows; few rows share long walks over the cache and join them, and need
+ *     smaq_paged_prefill_workspace_size bytes of workspace (0 with many rows). */
 typedef struct smaq_paged_args {
   const void* q;
   int64_t q_stride_t, q_stride_h;
@@ -486,6 +487,7 @@ typedef struct smaq_paged_args {
 } smaq_paged_args;
 size_t smaq_paged_decode_workspace_size(int batch, int n_q_heads, int n_kv_heads, int head_dim);
 int smaq_paged_decode(const smaq_paged_args* args, void* stream);
+size_t smaq_paged_prefill_workspace_size(int64_t n_rows, int batch, int n_q_heads, int n_kv_heads, int head_dim);
 int smaq_paged_prefill(const smaq_paged_args* args, void* stream);
 /* SMAQ_ERR_DEVICE if a bounded wait of the tensor-core prefill kernel ran out since the last check
  * (clears it).  Synchronises the stream. */

@@ -377,6 +377,11 @@ int launch_simt(const PagedParams& p, cudaStream_t st) {
 
 }  // namespace smaq
 
+extern "C" size_t smaq_paged_prefill_workspace_size(int64_t n_rows, int batch, int n_q_heads, int n_kv_heads, int head_dim) {
+  // only the tensor-core kernel shares walks; the size is the same for every dtype and alignment
+  return head_dim == 64 || head_dim == 128 ? smaq::prefill_tc_workspace(n_rows, batch, n_q_heads, n_kv_heads, head_dim) : 0;
+}
+
 extern "C" int smaq_paged_prefill(const smaq_paged_args* args, void* stream) {
   using namespace smaq;
   PagedParams p;

@@ -21,6 +21,8 @@
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
+#include <algorithm>
+
 #include "paged_prefill.cuh"
 #include "prefill_tc.cuh"
 #include "tcgen05.cuh"
@@ -58,11 +60,16 @@ struct PtParams {
   PagedParams p;
   int tma;         // keys and values come through the tensor maps where every token of a block is seen
   int box;         // slots a box: page_size, at most PT_N
+  int splits;      // CTAs that share a tile's walk, at most
+  float* parts;    // [tile][KV head][split]: accumulators [PT_ROWS][D], maxima, sums, whether a special value was met
   CUtensorMap k, v;
 };
+__host__ __device__ constexpr int64_t part_floats(int D) { return int64_t(PT_ROWS) * (D + 2) + 4; }
+// Splits of a walk of n blocks: two blocks each at least.
+__device__ __forceinline__ int splits_of(int n, int most) { return max(1, min(most, n / 2)); }
 
 struct PtBars {
-  uint64_t q_full, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready[2], o_full[2];
+  uint64_t q_full, v_part, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready[2], o_full[2];
   uint32_t tmem;
   int special;
   // the tile and its walk: read from here where needed, the softmax has no registers for them
@@ -114,15 +121,23 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
   const uint32_t base_raw = smem_u32(smem_raw), pad = (1024u - (base_raw & 1023u)) & 1023u;
   uint8_t* smem = smem_raw + pad;
   const uint32_t qs = base_raw + pad, ks = qs + 2 * TILE, vs = ks + STAGES * TILE;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kvh = int(blockIdx.x % unsigned(a.n_kv_heads)), tile = int(blockIdx.x / unsigned(a.n_kv_heads));
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, share = int(blockIdx.x % unsigned(pt.splits));
+  const int kvh = int(blockIdx.x / unsigned(pt.splits) % unsigned(a.n_kv_heads)), tile = int(blockIdx.x / unsigned(pt.splits * a.n_kv_heads));
+  pdl_launch_dependents();
 
-  write_padding(p, kvh, tile, int(gridDim.x / unsigned(a.n_kv_heads)));
-  int n, tiles, last;
+  int n, first_block, tiles, last;  // blocks of this CTA's share, the first of them
+  bool alone;                      // the share is the whole walk
   {
     const PrefillTile t = find_tile<PT_THREADS>(p, tile, PT_ROWS, true, sums, found);
-    if (t.rows == 0) return;
     const PrefillBlocks blocks(t, PT_N);
-    n = blocks.count;
+    const int shares = t.rows ? splits_of(blocks.count, pt.splits) : 0;
+    if (share >= shares) {  // also where the number of tiles that the host allows for exceeds theirs
+      if (share == 0) write_padding(p, kvh, tile, int(gridDim.x / unsigned(pt.splits * a.n_kv_heads)));
+      return;
+    }
+    first_block = int(int64_t(blocks.count) * share / shares);
+    n = int(int64_t(blocks.count) * (share + 1) / shares) - first_block;
+    alone = shares == 1;
     tiles = t.rows > 128 ? 2 : 1;
     last = t.f0 + t.rows;
     if (threadIdx.x == 0) {
@@ -136,7 +151,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
   const PrefillBlocks& blocks = bars.blocks;
 
   if (threadIdx.x == 0) {
-    mbar_init(&bars.q_full, PT_LOADERS);
+    mbar_init(&bars.q_full, 2 * PT_TW);
+    mbar_init(&bars.v_part, 1);
     for (int s = 0; s < 2; ++s) {
       mbar_init(&bars.k_full[s], PT_LOADERS);
       mbar_init(&bars.v_full[s], PT_LOADERS);
@@ -158,6 +174,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
   const uint32_t s_col = 0, o_col = 256;  // S of tile i at s_col + 128 i, O at o_col + D i
   bool failed = false;
 
+  // a row's chunk of eight channels in an operand
+  auto at = [](int r, int ch) { return uint32_t((r >> 3) * GROUP + (ch >> 3) * 1024 + (r & 7) * 128 + (((ch & 7) ^ (r & 7)) << 4)); };
+  auto base_of = [&](int j) { return blocks.base(first_block + j, PT_N); };
   auto seen_by_all = [&](int base) {
     return base + PT_N <= t.prefix || (base + PT_N <= bars.least + 1 && (a.window == 0 || base > bars.most - a.window));
   };
@@ -170,30 +189,24 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
       // ---- copies
       const int w = warp - PT_LOAD_WARP, tid = threadIdx.x - PT_LOAD_WARP * 32;
       const uint32_t lead = elect_one();
-      auto at = [&](int r, int ch) { return uint32_t((r >> 3) * GROUP + (ch >> 3) * 1024 + (r & 7) * 128 + (((ch & 7) ^ (r & 7)) << 4)); };
-      for (int i = tid; i < tiles * 128 * CH; i += PT_LOADERS) {
-        const int r = i / CH, ch = i % CH, fr = t.f0 + r, tok = fast_div(fr, p.group_div);
-        const bool live = r < t.rows;
-        const T* src = static_cast<const T*>(a.q) + (live ? (t.first + tok) * a.q_stride_t + (kvh * p.group + fr - tok * p.group) * a.q_stride_h + ch * 8 : 0);
-        cp_async16(qs + at(r, ch), src, live ? 16u : 0u);
-      }
-      cp_async_commit();
-      cp_async_wait<0>();
-      fence_proxy_async_smem();
-      mbar_arrive(&bars.q_full);
       const int32_t* table = a.block_table + t.b * a.table_stride;
-      // Blocks whose every token is seen by some row come by TMA, in boxes of one page (or 128 slots of it), the warps in
-      // turn.  (Issued by the lanes of one warp side by side, boxes cost about 150 cycles each, 5000 a block.)
+      // By TMA a block comes in boxes of one page (or 128 slots of it), the warps in turn; a box without a token that some
+      // row sees is left out.  (Issued by the lanes of one warp side by side, boxes cost about 150 cycles each.)
       const int per = PT_N / pt.box;
       auto whole = [&](int k) {
-        const int b = blocks.base(k, PT_N);
-        return pt.tma && (b + PT_N <= t.prefix || (b >= t.lo && b + PT_N <= t.hi));
+        const int b = base_of(k);
+        return b + PT_N <= t.prefix || (b >= t.lo && b + PT_N <= t.hi);
+      };
+      auto needed = [&](int k) {  // this lane's box of block k
+        const int b = base_of(k) + lane * pt.box;
+        return pt.tma && k < n && lane < per && (b < t.prefix || (b + pt.box > t.lo && b < t.hi));
       };
       auto page_of = [&](int k) {
-        if (k >= n || lane >= per || !whole(k)) return 0;
-        const int64_t blk = fast_div(blocks.base(k, PT_N) + lane * pt.box, p.page_div);
+        if (!needed(k)) return 0;
+        const int64_t blk = fast_div(base_of(k) + lane * pt.box, p.page_div);
         return int(min(max(int64_t(__ldg(table + blk)), int64_t(0)), a.n_pages - 1));
       };
+      int partial = 0;  // blocks whose values came through v_part
       // Blocks that come by cp.async: warp w brings rows r0 .. r0 + rows of every operand.
       const int r0 = w * 43, rows = min(43, PT_N - r0);
       // values of a block that some rows see in part: look for infinities and NaN in this warp's rows
@@ -205,23 +218,40 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
       auto fetch = [&](int j, int s, bool values, int page) {
         uint64_t* bar = values ? &bars.v_full[s] : &bars.k_full[s];
         const uint32_t dst = (values ? vs : ks) + s * TILE;
-        const bool part = values && !seen_by_all(blocks.base(j, PT_N));
-        if (whole(j)) {
-          if (tid == 0) mbar_arrive_expect_tx(bar, TILE);
-          const int first = blocks.base(j, PT_N), slot = per > 1 ? 0 : first - fast_div(first, p.page_div) * a.page_size;
-          for (int b = w; b < per; b += PT_MMA_WARP - PT_LOAD_WARP)
-            tma_5d(lead, dst + b * pt.box * (D * 2), values ? &pt.v : &pt.k, kvh * int(a.c_stride_h), 0, 0, slot >> 3, __shfl_sync(~0u, page, b), bar);
-          if (tid != 0) mbar_arrive(bar);
-          if (part) {
-            if (!warp_wait(bar, (j / STAGES) & 1)) failed = true;
-            look_for_special(s);
-            fence_proxy_async_smem();  // before the stage is filled again
+        const bool part = values && !seen_by_all(base_of(j));
+        if (pt.tma) {
+          // The scores of tokens that no row sees are replaced whatever their keys are, but their values are multiplied by
+          // zero: in a block with such tokens the values arrive at v_part and their rows are cleared.
+          const bool clear = values && !whole(j);
+          const uint32_t boxes = __ballot_sync(~0u, needed(j));
+          if (tid == 0) mbar_arrive_expect_tx(clear ? &bars.v_part : bar, __popc(boxes) * pt.box * D * 2);
+          const int first = base_of(j), slot = per > 1 ? 0 : first - fast_div(first, p.page_div) * a.page_size;
+          for (int b = w; b < per; b += PT_MMA_WARP - PT_LOAD_WARP) {
+            const int pg = __shfl_sync(~0u, page, b);
+            if (boxes >> b & 1)
+              tma_5d(lead, dst + b * pt.box * (D * 2), values ? &pt.v : &pt.k, kvh * int(a.c_stride_h), 0, 0, slot >> 3, pg, clear ? &bars.v_part : bar);
+          }
+          if (clear) {
+            if (!warp_wait(&bars.v_part, partial++ & 1)) failed = true;
+            for (int i = lane; i < rows * CH; i += 32)
+              if (!tile_sees(t, first + r0 + i / CH)) *reinterpret_cast<uint4*>(smem + (dst - qs) + at(r0 + i / CH, i % CH)) = make_uint4(0, 0, 0, 0);
+            __syncwarp();
+            if (part) look_for_special(s);
+            fence_proxy_async_smem();
+            mbar_arrive(bar);
+          } else {
+            if (tid != 0) mbar_arrive(bar);
+            if (part) {
+              if (!warp_wait(bar, (j / STAGES) & 1)) failed = true;
+              look_for_special(s);
+              fence_proxy_async_smem();  // before the stage is filled again
+            }
           }
           return;
         }
         const T* cache = static_cast<const T*>(values ? a.v_cache : a.k_cache);
         auto offset = [&](int r) {
-          const int tok = blocks.base(j, PT_N) + r0 + r;
+          const int tok = base_of(j) + r0 + r;
           return r < rows && tile_sees(t, tok) ? token_offset(p, table, tok) + kvh * a.c_stride_h : int64_t(-1);
         };
         const int64_t off0 = offset(lane), off1 = offset(lane + 32);
@@ -299,6 +329,18 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    // ---- queries
+    for (int i = threadIdx.x; i < tiles * 128 * CH; i += 64 * PT_TW) {
+      const int r = i / CH, ch = i % CH, fr = t.f0 + r, tok = fast_div(fr, p.group_div);
+      const bool live = r < t.rows;
+      const T* src = static_cast<const T*>(a.q) + (live ? (t.first + tok) * a.q_stride_t + (kvh * p.group + fr - tok * p.group) * a.q_stride_h + ch * 8 : 0);
+      cp_async16(qs + at(r, ch), src, live ? 16u : 0u);
+    }
+    cp_async_commit();
+    cp_async_wait<0>();
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bars.q_full);
     constexpr int C = PT_N / PT_SPLIT;                  // columns a thread
     const int i = warp / PT_TW, half = (warp >> 2) & 1;  // tile, half of the columns
     if (i < tiles) {
@@ -310,7 +352,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
       const uint32_t ts = tmem + lanes + s_col + 128 * i, to = tmem + lanes + o_col + D * i + half * (D / PT_SPLIT);
       float m = -INFINITY;  // reference maximum of the row, log2
       for (int j = 0; j < n; ++j) {
-        const int base = blocks.base(j, PT_N) + half * C;
+        const int base = base_of(j) + half * C;
         const bool part = !seen_by_all(base - half * C);
         if (!warp_wait(&bars.s_full[i], j & 1)) bars.fail[i][warp & 3] = 1;
         fence_after();
@@ -443,30 +485,50 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
       bars.row[n & 1][i][half][row] = l;
       named_bar(meet, 64);
       l += bars.row[n & 1][i][half ^ 1][row];
-      const float inv = l == 0.f ? 0.f : 1.0f / l;
-      T* out = static_cast<T*>(a.out) + int64_t(t.first + tok) * a.o_stride_t + h * a.o_stride_h + half * (D / PT_SPLIT);
+      if (alone) {
+        const float inv = l == 0.f ? 0.f : 1.0f / l;
+        T* out = static_cast<T*>(a.out) + int64_t(t.first + tok) * a.o_stride_t + h * a.o_stride_h + half * (D / PT_SPLIT);
 #pragma unroll
-      for (int c = 0; c < D / PT_SPLIT / 32; ++c) {
-        uint32_t o[32], w[16];
-        if (n > 0) {
+        for (int c = 0; c < D / PT_SPLIT / 32; ++c) {
+          uint32_t o[32], w[16];
+          if (n > 0) {
+            ld32(to + 32 * c, o);
+            ld_wait();
+          } else {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = 0u;
+          }
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float u = __uint_as_float(o[e]) * inv, v = __uint_as_float(o[e + 1]) * inv;
+            odd += (u + v) * 0.f;
+            w[e / 2] = pack2<DT>(u, v);
+          }
+          if (f < last && !failed) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) reinterpret_cast<uint4*>(out + 32 * c)[e] = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+          }
+        }
+        if (a.lse && half == 0 && f < last) a.lse[int64_t(t.first + tok) * a.n_q_heads + h] = (m + log2f(l)) * kLn2;
+      } else {
+        float* part = pt.parts + int64_t(blockIdx.x) * part_floats(D);
+        const int r = 128 * i + row;
+#pragma unroll
+        for (int c = 0; c < D / PT_SPLIT / 32; ++c) {
+          uint32_t o[32];
           ld32(to + 32 * c, o);
           ld_wait();
-        } else {
+          if (f < last) {
 #pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0u;
+            for (int e = 0; e < 8; ++e)
+              reinterpret_cast<uint4*>(part + r * D + half * (D / PT_SPLIT) + 32 * c)[e] = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          }
         }
-#pragma unroll
-        for (int e = 0; e < 32; e += 2) {
-          const float u = __uint_as_float(o[e]) * inv, v = __uint_as_float(o[e + 1]) * inv;
-          odd += (u + v) * 0.f;
-          w[e / 2] = pack2<DT>(u, v);
-        }
-        if (f < last && !failed) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) reinterpret_cast<uint4*>(out + 32 * c)[e] = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
+        if (half == 0 && f < last) {
+          part[PT_ROWS * D + r] = m;
+          part[PT_ROWS * (D + 1) + r] = l;
         }
       }
-      if (a.lse && half == 0 && f < last) a.lse[int64_t(t.first + tok) * a.n_q_heads + h] = (m + log2f(l)) * kLn2;
     }
   }
   if (failed) atomicOr(&g_prefill_fault, 1u);
@@ -476,9 +538,68 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
     fence_after();
     dealloc(bars.tmem, PT_COLS);
   }
+  if (share == 0) write_padding(p, kvh, tile, int(gridDim.x / unsigned(pt.splits * a.n_kv_heads)));
+  if (!alone) {
+    if (threadIdx.x == 0) pt.parts[(int64_t(blockIdx.x) + 1) * part_floats(D) - 4] = bars.special ? 1.f : 0.f;
+    return;
+  }
   if (warp < PT_LOAD_WARP && bars.special && warp / PT_TW < tiles) {
     uint32_t redo = __ballot_sync(~0u, odd != 0.f && l == l && f < last);
     for (; redo; redo &= redo - 1) exact_row(p, t, kvh, __shfl_sync(~0u, f, __ffs(redo) - 1));
+  }
+}
+
+// ---------------------------------------------------------------- join of split walks
+constexpr int PJ_THREADS = 256, PJ_ROWS = 32;
+
+// PJ_ROWS rows of one tile and KV head, a warp each in turn: the shares in order.
+template <class DT, int D>
+__global__ void __launch_bounds__(PJ_THREADS) prefill_join_kernel(const __grid_constant__ PtParams pt) {
+  using T = typename DT::T;
+  constexpr int E = D / 32;
+  const PagedParams& p = pt.p;
+  const smaq_paged_args& a = p.a;
+  __shared__ int sums[PJ_THREADS / 32], found[2];
+  const int chunk = int(blockIdx.x % (PT_ROWS / PJ_ROWS)), unit = int(blockIdx.x / (PT_ROWS / PJ_ROWS));
+  const int kvh = unit % a.n_kv_heads, tile = unit / a.n_kv_heads, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const PrefillTile t = find_tile<PJ_THREADS>(p, tile, PT_ROWS, true, sums, found);
+  pdl_wait();  // every CTA waits, so this grid ends after the other
+  const int shares = t.rows ? splits_of(PrefillBlocks(t, PT_N).count, pt.splits) : 0;
+  if (shares < 2) return;
+  const float* parts = pt.parts + int64_t(unit) * pt.splits * part_floats(D);
+  bool special = false;
+  for (int z = 0; z < shares; ++z) special |= parts[(z + 1) * part_floats(D) - 4] != 0.f;
+  for (int r = chunk * PJ_ROWS + warp; r < min((chunk + 1) * PJ_ROWS, t.rows); r += PJ_THREADS / 32) {
+    float m = -INFINITY, l = 0.f, o[E] = {};
+    for (int z = 0; z < shares; ++z) m = fmaxf(m, parts[z * part_floats(D) + PT_ROWS * D + r]);
+    const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll 4
+    for (int z = 0; z < shares; ++z) {
+      const float* part = parts + z * part_floats(D);
+      const float f = ex2(part[PT_ROWS * D + r] - base);
+      l += f * part[PT_ROWS * (D + 1) + r];
+      float x[E];
+      if constexpr (E == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(part + r * D + 4 * lane);
+      else *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(part + r * D + 2 * lane);
+#pragma unroll
+      for (int e = 0; e < E; ++e) o[e] += f * x[e];
+    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    const int f = t.f0 + r, tok = fast_div(f, p.group_div), h = kvh * p.group + f - tok * p.group;
+    T* out = static_cast<T*>(a.out) + int64_t(t.first + tok) * a.o_stride_t + h * a.o_stride_h + E * lane;
+    float odd = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      o[e] *= inv;
+      odd += o[e] * 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(out + e) = pack2<DT>(o[e], o[e + 1]);
+    if (a.lse && lane == 0) a.lse[int64_t(t.first + tok) * a.n_q_heads + h] = (m + log2f(l)) * kLn2;
+    if (special && __any_sync(~0u, odd != 0.f) && l == l) {
+      __syncwarp();
+      exact_row(p, t, kvh, f);
+    }
   }
 }
 
@@ -510,6 +631,12 @@ bool encode(CUtensorMap* map, const smaq_paged_args& a, const void* cache, int b
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// Tiles that any cu_query of this many rows and requests can have.
+int64_t most_tiles(int64_t n_rows, int batch, int group) { return (n_rows * group + PT_ROWS - 1) / PT_ROWS + batch; }
+// CTAs a tile: walks are shared where the tiles alone leave half of the GPU idle.  (The host does not know how long
+// the walks are: a CTA without a share ends at once.)  16 rows of 32/8 heads behind 16K tokens: 227 -> SPLIT_US us.
+int splits_for(int64_t units) { return int(std::max<int64_t>(1, std::min<int64_t>(32, num_sms() / std::max<int64_t>(units, 1)))); }
+
 template <class DT, int D>
 int launch(const PagedParams& p, cudaStream_t st) {
   PtParams pt;
@@ -523,13 +650,37 @@ int launch(const PagedParams& p, cudaStream_t st) {
               : a.softcap > 0.f            ? prefill_tc_kernel<DT, D, PT_CAP>
                                            : prefill_tc_kernel<DT, D, PT_PLAIN>;
   if (const int rc = allow_smem(reinterpret_cast<const void*>(kern), PtCfg<D>::SMEM, "paged_prefill")) return rc;
-  const int64_t tiles = (p.a.n_rows * p.group + PT_ROWS - 1) / PT_ROWS + p.a.batch;
-  if (tiles * a.n_kv_heads >= (int64_t(1) << 31)) return fail(SMAQ_ERR_UNSUPPORTED, "paged_prefill: too many rows");
-  kern<<<unsigned(tiles * a.n_kv_heads), PT_THREADS, PtCfg<D>::SMEM, st>>>(pt);
-  return cuda_status(cudaGetLastError(), "paged_prefill");
+  const int64_t units = most_tiles(a.n_rows, a.batch, p.group) * a.n_kv_heads;
+  pt.splits = splits_for(units);
+  pt.parts = static_cast<float*>(a.workspace);
+  if (units * pt.splits * (PT_ROWS / PJ_ROWS) >= (int64_t(1) << 31)) return fail(SMAQ_ERR_UNSUPPORTED, "paged_prefill: too many rows");
+  const size_t need = prefill_tc_workspace(a.n_rows, a.batch, a.n_q_heads, a.n_kv_heads, D);
+  if (need && (!a.workspace || a.workspace_bytes < need))
+    return fail(SMAQ_ERR_WORKSPACE, "paged_prefill: workspace %zu bytes, needs %zu", a.workspace ? a.workspace_bytes : size_t(0), need);
+  if (need && reinterpret_cast<uintptr_t>(a.workspace) % 16) return fail(SMAQ_ERR_INVALID, "paged_prefill: workspace must be 16-byte aligned");
+  kern<<<unsigned(units * pt.splits), PT_THREADS, PtCfg<D>::SMEM, st>>>(pt);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess || pt.splits == 1) return cuda_status(e, "paged_prefill");
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(unsigned(units * (PT_ROWS / PJ_ROWS)));
+  cfg.blockDim = dim3(PJ_THREADS);
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cuda_status(cudaLaunchKernelEx(&cfg, prefill_join_kernel<DT, D>, pt), "paged_prefill join");
 }
 
 }  // namespace
+
+size_t prefill_tc_workspace(int64_t n_rows, int batch, int n_q_heads, int n_kv_heads, int head_dim) {
+  if (n_rows <= 0 || batch < 0 || n_kv_heads <= 0 || n_q_heads < n_kv_heads) return 0;
+  const int64_t units = most_tiles(n_rows, batch, n_q_heads / n_kv_heads) * n_kv_heads;
+  const int splits = splits_for(units);
+  return splits > 1 ? size_t(units) * splits * part_floats(head_dim) * sizeof(float) : 0;
+}
 
 bool prefill_tc_eligible(const smaq_paged_args& a) {
 #ifdef NO_TC

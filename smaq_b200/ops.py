@@ -686,6 +686,10 @@ def paged_decode_workspace_bytes(batch: int, n_q_heads: int, n_kv_heads: int, he
     return int(_lib.load().smaq_paged_decode_workspace_size(batch, n_q_heads, n_kv_heads, head_dim))
 
 
+def paged_prefill_workspace_bytes(n_rows: int, batch: int, n_q_heads: int, n_kv_heads: int, head_dim: int) -> int:
+    return int(_lib.load().smaq_paged_prefill_workspace_size(n_rows, batch, n_q_heads, n_kv_heads, head_dim))
+
+
 def _paged(name, q, k_cache, v_cache, block_table, seq_lens, cu_query, prefix_lens, scale, window, softcap, slopes,
            out, return_lse, workspace):
     if q.dim() != 3:
@@ -730,13 +734,14 @@ def _paged(name, q, k_cache, v_cache, block_table, seq_lens, cu_query, prefix_le
     if cu_query is None:
         if T != B:
             raise ValueError(f"q has {T} rows for {B} requests; one row a request")
-        if workspace is None:
-            workspace = torch.empty(lib.smaq_paged_decode_workspace_size(B, Hq, Hk, D), dtype=torch.uint8,
-                                    device=q.device)
-        ws, ws_bytes, call = workspace.data_ptr(), workspace.numel() * workspace.element_size(), lib.smaq_paged_decode
+        call, need = lib.smaq_paged_decode, lib.smaq_paged_decode_workspace_size(B, Hq, Hk, D)
     else:
         cu_query = _int32("cu_query", cu_query, B + 1)
-        call = lib.smaq_paged_prefill
+        call, need = lib.smaq_paged_prefill, lib.smaq_paged_prefill_workspace_size(T, B, Hq, Hk, D)
+    if workspace is None and need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+    if workspace is not None:
+        ws, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
     st = call(
         _lib.pack_paged(q.data_ptr(), qt, qh, k_cache.data_ptr(), v_cache.data_ptr(), cp, cs, ch,
                         block_table.data_ptr(), max(row, M), seq_lens.data_ptr(), _addr(cu_query), _addr(prefix_lens),
@@ -768,17 +773,18 @@ def paged_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
                   seq_lens: torch.Tensor, cu_query: torch.Tensor, *, prefix_lens: Optional[torch.Tensor] = None,
                   scale: Optional[float] = None, window: Optional[int] = None, softcap: Optional[float] = None,
                   slopes: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
-                  return_lse: bool = False):
+                  return_lse: bool = False, workspace: Optional[torch.Tensor] = None):
     """Attention of prompt chunks over the exact paged cache (smaq_paged_prefill).
 
     Rows ``cu_query[b] .. cu_query[b + 1]`` of ``q [T, Hq, D]`` are request ``b``'s newest tokens (the
     last ones of its ``seq_lens[b]``, already written): row ``i`` sees tokens up to its own, the last
     ``window`` of them if given, and the first ``prefix_lens[b]`` in any case.  Requests never see one
-    another.  Other arguments as ``paged_decode``; rows past ``cu_query[B]`` give zeros."""
+    another.  Other arguments as ``paged_decode`` (``workspace``: ``paged_prefill_workspace_bytes``
+    bytes, which are 0 for many rows); rows past ``cu_query[B]`` give zeros."""
     if cu_query is None:
         raise ValueError("paged_prefill needs cu_query")
     return _paged("smaq_paged_prefill", q, k_cache, v_cache, block_table, seq_lens, cu_query, prefix_lens, scale,
-                  window, softcap, slopes, out, return_lse, None)
+                  window, softcap, slopes, out, return_lse, workspace)
 
 
 # --------------------------------------------------------------------- failure detection

@@ -149,6 +149,34 @@ def test_prefill_infinities_reach_only_rows_that_see_them(cuda, dtype):
     assert float((b.float() - a.float())[same].abs().max()) <= tol * float(a.float().abs().max())
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("news,ctx,Hq,Hkv,D,page,kw", [
+    ([16], [3000], 8, 2, 128, 16, {}), ([1, 0, 5], [2999, 10, 700], 8, 2, 64, 8, dict(slopes=True)),
+    ([70], [1500], 4, 4, 128, 24, dict(softcap=9.0)), ([3, 130], [513, 2000], 7, 1, 128, 128, dict(window=900, prefix=[40, 300])),
+    ([200], [900], 4, 1, 64, 256, dict(window=200)), ([33], [2500], 2, 1, 128, 1, {})])
+def test_prefill_shared_walks(cuda, dtype, news, ctx, Hq, Hkv, D, page, kw):
+    """Few rows behind long contexts: several CTAs share a tile's walk and their parts are joined."""
+    from smaq_b200 import ops
+    assert ops.paged_prefill_workspace_bytes(sum(news), len(news), Hq, Hkv, D) > 0
+    prefill(cuda, news, ctx, Hq, Hkv, D, page, dtype, pad=3, **kw)
+
+
+def test_prefill_shared_walks_infinities(cuda):
+    """An infinite value in a window's edge block leaves rows that do not see it as they are, whichever share met it."""
+    from smaq_b200 import ops
+    k, v, table = paged_case(cuda, [2000], 1, 128, 16, BF)
+    q = queries(cuda, 40, 2, 128, BF)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    args = (table, i32([2000]), i32([0, 40]))
+    a = ops.paged_prefill(q, k, v, *args, window=1000)
+    v[table[0, 60].long(), 12, 0, 3] = math.inf            # token 972: rows of positions 1960 .. 1971 see it
+    b = ops.paged_prefill(q, k, v, *args, window=1000)
+    assert bool((b[:12, :, 3] == math.inf).all()) and bool(torch.isfinite(b[12:]).all())
+    assert float((b[12:].float() - a[12:].float()).abs().max()) <= 4 * UNIT[BF] * float(a.float().abs().max())
+    with pytest.raises(RuntimeError, match="WORKSPACE"):
+        ops.paged_prefill(q, k, v, *args, workspace=torch.empty(64, dtype=torch.uint8, device=cuda))
+
+
 def test_not_admitted_and_broken_tables_stay_inside(cuda):
     """A request of length 0 with query rows gives zeros; page numbers and lengths past the cache read in bounds."""
     from smaq_b200 import ops
