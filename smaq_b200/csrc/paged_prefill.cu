@@ -34,11 +34,12 @@ __global__ void __launch_bounds__(PM_THREADS, 2) prefill_mma_kernel(const __grid
   constexpr int N = PmCfg<D>::N, STAGE = PmCfg<D>::STAGE, CH = D / 8, NT = D / 8;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ int64_t offs[2][N];
-  __shared__ int sums[PM_THREADS / 32], found[2];
+  __shared__ int sums[PM_THREADS / 32];
+  __shared__ PrefillTile found;
   const smaq_paged_args& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, kvh = blockIdx.y;
   write_padding(p, kvh, blockIdx.x, gridDim.x);
-  const PrefillTile t = find_tile<PM_THREADS>(p, blockIdx.x, PmCfg<D>::ROWS, true, sums, found);
+  const PrefillTile t = find_tile<PM_THREADS>(p, blockIdx.x, PmCfg<D>::ROWS, true, sums, &found);
   if (t.rows == 0) return;
   const PrefillBlocks blocks(t, N);
   const uint32_t qs = smem_u32(smem), ring = qs + PmCfg<D>::Q;
@@ -216,11 +217,12 @@ __global__ void __launch_bounds__(PM_THREADS) prefill_simt_kernel(const __grid_c
   constexpr int GROUPS = PM_THREADS / 8, WARPS = PM_THREADS / 32;
   __shared__ __align__(16) float qs[PX_ROWS][32 * NI];
   __shared__ float acc[WARPS][PX_ROWS][32 * NI + 2];
-  __shared__ int sums[WARPS], found[2];
+  __shared__ int sums[WARPS];
+  __shared__ PrefillTile found;
   const smaq_paged_args& a = p.a;
   const int D = a.head_dim, l = threadIdx.x & 7, grp = threadIdx.x >> 3, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, kvh = blockIdx.y;
   write_padding(p, kvh, blockIdx.x, gridDim.x);
-  const PrefillTile t = find_tile<PM_THREADS>(p, blockIdx.x, PX_ROWS, true, sums, found);
+  const PrefillTile t = find_tile<PM_THREADS>(p, blockIdx.x, PX_ROWS, true, sums, &found);
   if (t.rows == 0) return;
   for (int i = threadIdx.x; i < PX_ROWS * 32 * NI; i += PM_THREADS) {
     const int r = i / (32 * NI), e = i % (32 * NI), f = t.f0 + r, tok = f / p.group;
@@ -340,16 +342,17 @@ __global__ void __launch_bounds__(PM_THREADS) prefill_simt_kernel(const __grid_c
   }
 }
 
-// Tiles that any cu_query of this many rows and requests can have.
-int64_t most_tiles(const PagedParams& p, int size) {
-  return (p.a.n_rows * p.group + size - 1) / size + p.a.batch;
+// At least one CTA a KV head, for the rows past the last request's.
+int64_t grid_tiles(const PagedParams& p, int size) {
+  const int64_t n = most_tiles(p.a.n_rows, p.a.batch, p.group, size);
+  return n > 0 ? n : 1;
 }
 
 template <class DT, int D>
 int launch_mma(const PagedParams& p, cudaStream_t st) {
   auto kern = p.a.softcap > 0.f ? prefill_mma_kernel<DT, D, true> : prefill_mma_kernel<DT, D, false>;
   if (const int rc = allow_smem(reinterpret_cast<const void*>(kern), PmCfg<D>::SMEM, "paged_prefill")) return rc;
-  kern<<<dim3(unsigned(most_tiles(p, PmCfg<D>::ROWS)), p.a.n_kv_heads), PM_THREADS, PmCfg<D>::SMEM, st>>>(p);
+  kern<<<dim3(unsigned(grid_tiles(p, PmCfg<D>::ROWS)), p.a.n_kv_heads), PM_THREADS, PmCfg<D>::SMEM, st>>>(p);
   return cuda_status(cudaGetLastError(), "paged_prefill");
 }
 template <class DT>
@@ -365,7 +368,7 @@ int launch_simt(const PagedParams& p, cudaStream_t st) {
   const int D = p.a.head_dim;
   const bool vec = D % 4 == 0 && paged_aligned(p.a);
   auto go = [&](auto kern) {
-    kern<<<dim3(unsigned(most_tiles(p, PX_ROWS)), p.a.n_kv_heads), PM_THREADS, 0, st>>>(p);
+    kern<<<dim3(unsigned(grid_tiles(p, PX_ROWS)), p.a.n_kv_heads), PM_THREADS, 0, st>>>(p);
     return cuda_status(cudaGetLastError(), "paged_prefill");
   };
   if (D <= 64) return vec ? go(prefill_simt_kernel<DT, 2, true>) : go(prefill_simt_kernel<DT, 2, false>);
@@ -389,7 +392,7 @@ extern "C" int smaq_paged_prefill(const smaq_paged_args* args, void* stream) {
   const smaq_paged_args& a = p.a;
   if (a.n_rows == 0) return SMAQ_OK;
   if (a.n_kv_heads > 65535) return fail(SMAQ_ERR_UNSUPPORTED, "paged_prefill: %d KV heads above 65535", a.n_kv_heads);
-  if (most_tiles(p, PX_ROWS) >= (int64_t(1) << 31)) return fail(SMAQ_ERR_UNSUPPORTED, "paged_prefill: too many rows");
+  if (grid_tiles(p, PX_ROWS) >= (int64_t(1) << 31)) return fail(SMAQ_ERR_UNSUPPORTED, "paged_prefill: too many rows");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (prefill_tc_eligible(a)) return launch_prefill_tc(p, st);
   if (a.dtype != SMAQ_F32 && (a.head_dim == 64 || a.head_dim == 128 || a.head_dim == 256) && paged_aligned(a))

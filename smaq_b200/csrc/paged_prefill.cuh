@@ -21,17 +21,22 @@ __device__ __forceinline__ int cu_at(const PagedParams& p, int b) {
   return int(min(int64_t(max(__ldg(p.a.cu_query + b), 0)), p.a.n_rows));
 }
 
-// Tile `x` (counted over all requests) for blocks of THREADS threads.  `found` and `sums` are shared.
+// Tile `x` (counted over all requests) for blocks of THREADS threads, as long as the tiles of `size` rows reach
+// (rows 0: no such tile).  Every thread loads one request's facts at once, and the one whose request it is fills `out`.
+// `sums` and `out` are shared; all threads return the same.
 template <int THREADS>
-__device__ __forceinline__ PrefillTile find_tile(const PagedParams& p, int x, int size, bool reverse, int* sums, int* found) {
+__device__ __forceinline__ PrefillTile find_tile(const PagedParams& p, int x, int size, bool reverse, int* sums, PrefillTile* out) {
   const int B = p.a.batch, lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  int total = 0, mine = 0, before = 0;
+  int total = 0, mine = 0, before = 0, c0 = 0, c1 = 0, len = 0, prefix = 0;
   auto step = [&](int b0) {
     const int b = b0 + threadIdx.x;
     mine = 0;
     if (b < B) {
-      const int64_t f = int64_t(max(cu_at(p, b + 1) - cu_at(p, b), 0)) * p.group;
-      mine = int((f + size - 1) / size);
+      c0 = cu_at(p, b);
+      c1 = cu_at(p, b + 1);
+      len = paged_len(p, b);
+      prefix = p.a.prefix_lens ? min(max(__ldg(p.a.prefix_lens + b), 0), len) : 0;
+      mine = int((int64_t(max(c1 - c0, 0)) * p.group + size - 1) / size);
     }
     int v = mine;
 #pragma unroll
@@ -51,33 +56,38 @@ __device__ __forceinline__ PrefillTile find_tile(const PagedParams& p, int x, in
     before = base + v - mine;
     return all;
   };
+  if (threadIdx.x == 0) out->rows = 0;
   for (int b0 = 0; b0 < B; b0 += THREADS) total += step(b0);
-  PrefillTile t;
-  t.rows = 0;
-  if (x >= total) return t;
-  if (reverse) x = total - 1 - x;
-  int base = 0;
-  for (int b0 = 0; b0 < B && base <= x; b0 += THREADS) {
-    const int all = B <= THREADS ? total : step(b0);
-    if (x >= base + before && x < base + before + mine) {
-      found[0] = b0 + threadIdx.x;
-      found[1] = x - base - before;
+  if (x < total) {
+    if (reverse) x = total - 1 - x;
+    int base = 0;
+    for (int b0 = 0; b0 < B && base <= x; b0 += THREADS) {
+      const int all = B <= THREADS ? total : step(b0);
+      if (x >= base + before && x < base + before + mine) {
+        PrefillTile t;
+        const int n = c1 - c0;
+        t.b = b0 + threadIdx.x;
+        t.f0 = (x - base - before) * size;
+        t.first = c0;
+        t.len = len;
+        t.past = len - n;
+        t.prefix = prefix;
+        t.rows = int(min(int64_t(size), int64_t(n) * p.group - t.f0));
+        const int i0 = t.past + t.f0 / p.group, i1 = t.past + (t.f0 + t.rows - 1) / p.group;
+        t.hi = max(min(i1 + 1, t.len), 0);
+        t.lo = p.a.window > 0 ? min(max(i0 - p.a.window + 1, 0), t.hi) : 0;
+        *out = t;
+      }
+      base += all;
     }
-    base += all;
   }
   __syncthreads();
-  t.b = found[0];
-  t.f0 = found[1] * size;
-  t.first = cu_at(p, t.b);
-  const int n = cu_at(p, t.b + 1) - t.first;
-  t.rows = int(min(int64_t(size), int64_t(n) * p.group - t.f0));
-  t.len = paged_len(p, t.b);
-  t.past = t.len - n;
-  t.prefix = p.a.prefix_lens ? min(max(__ldg(p.a.prefix_lens + t.b), 0), t.len) : 0;
-  const int i0 = t.past + t.f0 / p.group, i1 = t.past + (t.f0 + t.rows - 1) / p.group;
-  t.hi = max(min(i1 + 1, t.len), 0);
-  t.lo = p.a.window > 0 ? min(max(i0 - p.a.window + 1, 0), t.hi) : 0;
-  return t;
+  return *out;
+}
+
+// Tiles of `size` rows that any cu_query of this many rows and requests can have: sum of ceil(x_b / size).
+inline int64_t most_tiles(int64_t n_rows, int batch, int group, int size) {
+  return (n_rows * group + int64_t(batch) * (size - 1)) / size;
 }
 
 // Whether some row of the tile sees token j: others are read as zeros.

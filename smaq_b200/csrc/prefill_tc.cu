@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
   constexpr uint32_t ID_S = idesc(DT::code == SMAQ_BF16, PT_N, false), ID_O = idesc(DT::code == SMAQ_BF16, D, true);
   extern __shared__ uint8_t smem_raw[];
   __shared__ PtBars bars;
-  __shared__ int sums[PT_THREADS / 32], found[2];
+  __shared__ int sums[PT_THREADS / 32];
   const smaq_paged_args& a = p.a;
   const uint32_t base_raw = smem_u32(smem_raw), pad = (1024u - (base_raw & 1023u)) & 1023u;
   uint8_t* smem = smem_raw + pad;
@@ -128,7 +128,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
   int n, first_block, tiles, last;  // blocks of this CTA's share, the first of them
   bool alone;                      // the share is the whole walk
   {
-    const PrefillTile t = find_tile<PT_THREADS>(p, tile, PT_ROWS, true, sums, found);
+    const PrefillTile t = find_tile<PT_THREADS>(p, tile, PT_ROWS, true, sums, &bars.t);
     const PrefillBlocks blocks(t, PT_N);
     const int shares = t.rows ? splits_of(blocks.count, pt.splits) : 0;
     if (share >= shares) {  // also where the number of tiles that the host allows for exceeds theirs
@@ -141,7 +141,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
     tiles = t.rows > 128 ? 2 : 1;
     last = t.f0 + t.rows;
     if (threadIdx.x == 0) {
-      bars.t = t;
       bars.blocks = blocks;
       bars.least = t.past + fast_div(t.f0, p.group_div);
       bars.most = t.past + fast_div(last - 1, p.group_div);
@@ -212,7 +211,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
       // values of a block that some rows see in part: look for infinities and NaN in this warp's rows
       auto look_for_special = [&](int s) {
         bool odd_value = false;
-        for (int i = lane; i < rows * CH; i += 32) odd_value |= any_special<DT>(*reinterpret_cast<const uint4*>(smem + (vs - qs) + s * TILE + at(r0 + i / CH, i % CH)));
+        const uint8_t* stage = smem + (vs - qs) + s * TILE;
+#pragma unroll 8
+        for (int i = lane; i < rows * CH; i += 32) odd_value |= any_special<DT>(*reinterpret_cast<const uint4*>(stage + at(r0 + i / CH, i % CH)));
         if (odd_value) bars.special = 1;
       };
       auto fetch = [&](int j, int s, bool values, int page) {
@@ -233,8 +234,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
           }
           if (clear) {
             if (!warp_wait(&bars.v_part, partial++ & 1)) failed = true;
+            const int pre = t.prefix - first, lo = t.lo - first, hi = t.hi - first;
+#pragma unroll 4
             for (int i = lane; i < rows * CH; i += 32)
-              if (!tile_sees(t, first + r0 + i / CH)) *reinterpret_cast<uint4*>(smem + (dst - qs) + at(r0 + i / CH, i % CH)) = make_uint4(0, 0, 0, 0);
+              if (const int r = r0 + i / CH; r >= pre && (r < lo || r >= hi)) *reinterpret_cast<uint4*>(smem + (dst - qs) + at(r0 + i / CH, i % CH)) = make_uint4(0, 0, 0, 0);
             __syncwarp();
             if (part) look_for_special(s);
             fence_proxy_async_smem();
@@ -559,10 +562,11 @@ __global__ void __launch_bounds__(PJ_THREADS) prefill_join_kernel(const __grid_c
   constexpr int E = D / 32;
   const PagedParams& p = pt.p;
   const smaq_paged_args& a = p.a;
-  __shared__ int sums[PJ_THREADS / 32], found[2];
+  __shared__ int sums[PJ_THREADS / 32];
+  __shared__ PrefillTile found;
   const int chunk = int(blockIdx.x % (PT_ROWS / PJ_ROWS)), unit = int(blockIdx.x / (PT_ROWS / PJ_ROWS));
   const int kvh = unit % a.n_kv_heads, tile = unit / a.n_kv_heads, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const PrefillTile t = find_tile<PJ_THREADS>(p, tile, PT_ROWS, true, sums, found);
+  const PrefillTile t = find_tile<PJ_THREADS>(p, tile, PT_ROWS, true, sums, &found);
   pdl_wait();  // every CTA waits, so this grid ends after the other
   const int shares = t.rows ? splits_of(PrefillBlocks(t, PT_N).count, pt.splits) : 0;
   if (shares < 2) return;
@@ -631,8 +635,7 @@ bool encode(CUtensorMap* map, const smaq_paged_args& a, const void* cache, int b
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Tiles that any cu_query of this many rows and requests can have.
-int64_t most_tiles(int64_t n_rows, int batch, int group) { return (n_rows * group + PT_ROWS - 1) / PT_ROWS + batch; }
+int64_t grid_tiles(int64_t n_rows, int batch, int group) { return std::max<int64_t>(1, most_tiles(n_rows, batch, group, PT_ROWS)); }
 // CTAs a tile: walks are shared where the tiles alone leave half of the GPU idle.  (The host does not know how long
 // the walks are: a CTA without a share ends at once.)  16 rows of 32/8 heads behind 16K tokens: 227 -> SPLIT_US us.
 int splits_for(int64_t units) { return int(std::max<int64_t>(1, std::min<int64_t>(32, num_sms() / std::max<int64_t>(units, 1)))); }
@@ -650,7 +653,7 @@ int launch(const PagedParams& p, cudaStream_t st) {
               : a.softcap > 0.f            ? prefill_tc_kernel<DT, D, PT_CAP>
                                            : prefill_tc_kernel<DT, D, PT_PLAIN>;
   if (const int rc = allow_smem(reinterpret_cast<const void*>(kern), PtCfg<D>::SMEM, "paged_prefill")) return rc;
-  const int64_t units = most_tiles(a.n_rows, a.batch, p.group) * a.n_kv_heads;
+  const int64_t units = grid_tiles(a.n_rows, a.batch, p.group) * a.n_kv_heads;
   pt.splits = splits_for(units);
   pt.parts = static_cast<float*>(a.workspace);
   if (units * pt.splits * (PT_ROWS / PJ_ROWS) >= (int64_t(1) << 31)) return fail(SMAQ_ERR_UNSUPPORTED, "paged_prefill: too many rows");
@@ -677,7 +680,7 @@ int launch(const PagedParams& p, cudaStream_t st) {
 
 size_t prefill_tc_workspace(int64_t n_rows, int batch, int n_q_heads, int n_kv_heads, int head_dim) {
   if (n_rows <= 0 || batch < 0 || n_kv_heads <= 0 || n_q_heads < n_kv_heads) return 0;
-  const int64_t units = most_tiles(n_rows, batch, n_q_heads / n_kv_heads) * n_kv_heads;
+  const int64_t units = grid_tiles(n_rows, batch, n_q_heads / n_kv_heads) * n_kv_heads;
   const int splits = splits_for(units);
   return splits > 1 ? size_t(units) * splits * part_floats(head_dim) * sizeof(float) : 0;
 }
