@@ -487,7 +487,8 @@ typedef struct smaq_paged_args {
 } smaq_paged_args;
 size_t smaq_paged_decode_workspace_size(int batch, int n_q_heads, int n_kv_heads, int head_dim);
 int smaq_paged_decode(const smaq_paged_args* args, void* stream);
-size_t smaq_paged_prefill_workspace_size(int64_t n_rows, int batch, int n_q_heads, int n_kv_heads, int head_dim);
+size_t smaq_paged_prefill_workspace_size(int64_t n_rows, int batch, int n_q_heads, int n_kv_heads, int head_dim,
+                                         int64_t max_tokens /* max_blocks * page_size */);
 int smaq_paged_prefill(const smaq_paged_args* args, void* stream);
 /* SMAQ_ERR_DEVICE if a bounded wait of the tensor-core prefill kernel ran out since the last check
  * (clears it).  Synchronises the stream. */

@@ -186,7 +186,7 @@ def load() -> C.CDLL:
     lib.smaq_paged_decode_workspace_size.restype = C.c_size_t
     lib.smaq_paged_decode.argtypes = [C.c_char_p, vp]
     lib.smaq_paged_decode.restype = i32
-    lib.smaq_paged_prefill_workspace_size.argtypes = [i64, i32, i32, i32, i32]
+    lib.smaq_paged_prefill_workspace_size.argtypes = [i64, i32, i32, i32, i32, i64]
     lib.smaq_paged_prefill_workspace_size.restype = C.c_size_t
     lib.smaq_paged_prefill.argtypes = [C.c_char_p, vp]
     lib.smaq_paged_prefill.restype = i32

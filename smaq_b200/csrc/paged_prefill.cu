@@ -6,7 +6,8 @@
 // sees, with a running maximum and sum per row.  The tiles of all requests are numbered from cu_query on the
 // GPU; the host knows only the number of rows.  Tiles with the longest walks start first.
 //
-// prefill_mma_kernel (bf16 / fp16, head_dim 64 / 128 / 256): four warps of 16 rows, m16n8k16 products, blocks of
+// prefill_tc.cu (bf16 / fp16, head_dim 64 / 128 / 256): the tensor-core kernel, everything but tables of one block.
+// prefill_mma_kernel (the same types and head dims, tables of up to 128 tokens): four warps of 16 rows, m16n8k16 products, blocks of
 //   64 (head_dim 256: 32) tokens brought by cp.async into two stages, page lookups two blocks ahead.
 // prefill_simt_kernel (fp32, other head dims and alignments): tiles of four rows, 16 lane groups with a token
 //   each; all arithmetic in 32 bits.
@@ -380,9 +381,9 @@ int launch_simt(const PagedParams& p, cudaStream_t st) {
 
 }  // namespace smaq
 
-extern "C" size_t smaq_paged_prefill_workspace_size(int64_t n_rows, int batch, int n_q_heads, int n_kv_heads, int head_dim) {
+extern "C" size_t smaq_paged_prefill_workspace_size(int64_t n_rows, int batch, int n_q_heads, int n_kv_heads, int head_dim, int64_t max_tokens) {
   // only the tensor-core kernel shares walks; the size is the same for every dtype and alignment
-  return head_dim == 64 || head_dim == 128 ? smaq::prefill_tc_workspace(n_rows, batch, n_q_heads, n_kv_heads, head_dim) : 0;
+  return head_dim == 64 || head_dim == 128 || head_dim == 256 ? smaq::prefill_tc_workspace(n_rows, batch, n_q_heads, n_kv_heads, head_dim, max_tokens) : 0;
 }
 
 extern "C" int smaq_paged_prefill(const smaq_paged_args* args, void* stream) {

@@ -37,11 +37,13 @@ __device__ unsigned int g_prefill_fault;
 
 constexpr int PT_SPLIT = 2;               // softmax threads a row
 constexpr int PT_TW = 4 * PT_SPLIT;       // softmax warps a tile
-constexpr int PT_THREADS = 32 * (2 * PT_TW + 4);
 constexpr int PT_N = 128;                 // tokens a block
-constexpr int PT_ROWS = 256;
-constexpr int PT_LOAD_WARP = 2 * PT_TW, PT_MMA_WARP = PT_LOAD_WARP + 3;
-constexpr int PT_LOADERS = 32 * (PT_MMA_WARP - PT_LOAD_WARP);
+constexpr int PT_LOADERS = 96;            // three warps of copies
+constexpr int PJ_ROWS = 32;               // rows a CTA of the join
+// Tiles a CTA: tensor memory has room for the scores and accumulators of two at head_dim 128, of one at 256.
+__host__ __device__ constexpr int pt_tiles(int D) { return D == 256 ? 1 : 2; }
+__host__ __device__ constexpr int pt_rows(int D) { return 128 * pt_tiles(D); }
+__host__ __device__ constexpr int pt_threads(int D) { return 32 * (PT_TW * pt_tiles(D) + 4); }
 constexpr uint32_t PT_COLS = 512;
 constexpr float PT_LAG = 8.0f;            // log2
 constexpr uint32_t PT_SPIN = 1u << 24;    // polls before a wait gives up
@@ -51,9 +53,10 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) { retu
 
 template <int D>
 struct PtCfg {
+  static constexpr int TILES = pt_tiles(D);
   static constexpr int TILE = 128 * D * 2;              // bytes: 128 rows of queries, keys or values
-  static constexpr int STAGES = 2;
-  static constexpr int SMEM = 2 * TILE + 2 * STAGES * TILE + 1024;
+  static constexpr int STAGES = D == 256 ? 1 : 2;
+  static constexpr int SMEM = TILES * TILE + 2 * STAGES * TILE + 1024;
 };
 
 struct PtParams {
@@ -61,15 +64,15 @@ struct PtParams {
   int tma;         // keys and values come through the tensor maps where every token of a block is seen
   int box;         // slots a box: page_size, at most PT_N
   int splits;      // CTAs that share a tile's walk, at most
-  float* parts;    // [tile][KV head][split]: accumulators [PT_ROWS][D], maxima, sums, whether a special value was met
+  float* parts;    // [tile][KV head][split]: accumulators [rows][D], maxima, sums, whether a special value was met
   CUtensorMap k, v;
 };
-__host__ __device__ constexpr int64_t part_floats(int D) { return int64_t(PT_ROWS) * (D + 2) + 4; }
+__host__ __device__ constexpr int64_t part_floats(int D) { return int64_t(pt_rows(D)) * (D + 2) + 4; }
 // Splits of a walk of n blocks: two blocks each at least.
 __device__ __forceinline__ int splits_of(int n, int most) { return max(1, min(most, n / 2)); }
 
 struct PtBars {
-  uint64_t q_full, v_part, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready[2], o_full[2];
+  uint64_t q_full, v_part, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready[2], o_step, o_full[2];
   uint32_t tmem;
   int special;
   // the tile and its walk: read from here where needed, the softmax has no registers for them
@@ -109,18 +112,19 @@ __device__ __forceinline__ void exp2_group(uint64_t (&x)[PT_OF]) {
 }
 
 template <class DT, int D, int MODE>
-__global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_constant__ PtParams pt) {
+__global__ void __launch_bounds__(pt_threads(D), 1) prefill_tc_kernel(const __grid_constant__ PtParams pt) {
   using T = typename DT::T;
   const PagedParams& p = pt.p;
+  constexpr int TILES = PtCfg<D>::TILES, ROWS = pt_rows(D), LOAD_WARP = PT_TW * TILES, MMA_WARP = LOAD_WARP + 3;
   constexpr int TILE = PtCfg<D>::TILE, STAGES = PtCfg<D>::STAGES, CH = D / 8, GROUP = 8 * D * 2;  // GROUP: 8 rows, 64-channel atoms side by side
   constexpr uint32_t ID_S = idesc(DT::code == SMAQ_BF16, PT_N, false), ID_O = idesc(DT::code == SMAQ_BF16, D, true);
   extern __shared__ uint8_t smem_raw[];
   __shared__ PtBars bars;
-  __shared__ int sums[PT_THREADS / 32];
+  __shared__ int sums[pt_threads(D) / 32];
   const smaq_paged_args& a = p.a;
   const uint32_t base_raw = smem_u32(smem_raw), pad = (1024u - (base_raw & 1023u)) & 1023u;
   uint8_t* smem = smem_raw + pad;
-  const uint32_t qs = base_raw + pad, ks = qs + 2 * TILE, vs = ks + STAGES * TILE;
+  const uint32_t qs = base_raw + pad, ks = qs + TILES * TILE, vs = ks + STAGES * TILE;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, share = int(blockIdx.x % unsigned(pt.splits));
   const int kvh = int(blockIdx.x / unsigned(pt.splits) % unsigned(a.n_kv_heads)), tile = int(blockIdx.x / unsigned(pt.splits * a.n_kv_heads));
   pdl_launch_dependents();
@@ -128,7 +132,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
   int n, first_block, tiles, last;  // blocks of this CTA's share, the first of them
   bool alone;                      // the share is the whole walk
   {
-    const PrefillTile t = find_tile<PT_THREADS>(p, tile, PT_ROWS, true, sums, &bars.t);
+    const PrefillTile t = find_tile<pt_threads(D)>(p, tile, ROWS, true, sums, &bars.t);
     const PrefillBlocks blocks(t, PT_N);
     const int shares = t.rows ? splits_of(blocks.count, pt.splits) : 0;
     if (share >= shares) {  // also where the number of tiles that the host allows for exceeds theirs
@@ -150,7 +154,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
   const PrefillBlocks& blocks = bars.blocks;
 
   if (threadIdx.x == 0) {
-    mbar_init(&bars.q_full, 2 * PT_TW);
+    mbar_init(&bars.q_full, TILES * PT_TW);
+    mbar_init(&bars.o_step, 1);
     mbar_init(&bars.v_part, 1);
     for (int s = 0; s < 2; ++s) {
       mbar_init(&bars.k_full[s], PT_LOADERS);
@@ -165,12 +170,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
     for (int i = 0; i < 8; ++i) bars.fail[i >> 2][i & 3] = 0;
     fence_mbar_init();
   }
-  if (warp == PT_MMA_WARP) alloc(&bars.tmem, PT_COLS);
+  if (warp == MMA_WARP) alloc(&bars.tmem, PT_COLS);
   fence_before();
   __syncthreads();
   fence_after();
   constexpr uint32_t tmem = 0;  // all 512 columns are this CTA's: the allocation starts at 0
-  const uint32_t s_col = 0, o_col = 256;  // S of tile i at s_col + 128 i, O at o_col + D i
+  constexpr uint32_t s_col = 0, o_col = 256;  // S of tile i (one tile: of blocks of parity i) at s_col + 128 i, O at o_col + D i
   bool failed = false;
 
   // a row's chunk of eight channels in an operand
@@ -182,11 +187,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
   float odd = 0.f, l = 0.f;  // softmax threads: NaN where an output is not finite; sum of weights
   int f = 0;
 
-  if (warp >= PT_LOAD_WARP) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");  // 128 x 64 + 512 x 104 = 640 x 96, the launch's
-    if (warp < PT_MMA_WARP) {
+  if (warp >= LOAD_WARP) {
+    if constexpr (TILES == 2) asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");  // 128 x 64 + 512 x 104 = 640 x 96, the launch's
+    if (warp < MMA_WARP) {
       // ---- copies
-      const int w = warp - PT_LOAD_WARP, tid = threadIdx.x - PT_LOAD_WARP * 32;
+      const int w = warp - LOAD_WARP, tid = threadIdx.x - LOAD_WARP * 32;
       const uint32_t lead = elect_one();
       const int32_t* table = a.block_table + t.b * a.table_stride;
       // By TMA a block comes in boxes of one page (or 128 slots of it), the warps in turn; a box without a token that some
@@ -227,7 +232,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
           const uint32_t boxes = __ballot_sync(~0u, needed(j));
           if (tid == 0) mbar_arrive_expect_tx(clear ? &bars.v_part : bar, __popc(boxes) * pt.box * D * 2);
           const int first = base_of(j), slot = per > 1 ? 0 : first - fast_div(first, p.page_div) * a.page_size;
-          for (int b = w; b < per; b += PT_MMA_WARP - PT_LOAD_WARP) {
+          for (int b = w; b < per; b += MMA_WARP - LOAD_WARP) {
             const int pg = __shfl_sync(~0u, page, b);
             if (boxes >> b & 1)
               tma_5d(lead, dst + b * pt.box * (D * 2), values ? &pt.v : &pt.k, kvh * int(a.c_stride_h), 0, 0, slot >> 3, pg, clear ? &bars.v_part : bar);
@@ -286,17 +291,24 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
         if (failed) break;
         page = next;
       }
-    } else if (warp == PT_MMA_WARP && n > 0) {
+    } else if (warp == MMA_WARP && n > 0) {
       // ---- products
       const uint32_t lead = elect_one();
       auto scores = [&](int i, int j) {
-        const uint32_t q = qs + i * TILE, k = ks + (j % STAGES) * TILE;
+        const uint32_t q = qs + (TILES == 2 ? i * TILE : 0), k = ks + (j % STAGES) * TILE;
 #pragma unroll
         for (int c = 0; c < D / 16; ++c) {
           const uint32_t at = uint32_t((c >> 2) * 1024 + (c & 3) * 32);
           mma_ss(lead, tmem + s_col + 128 * i, desc(q + at, GROUP, 16), desc(k + at, GROUP, 16), ID_S, c > 0);
         }
         commit(lead, &bars.s_full[i]);
+      };
+      auto values = [&](int i, int j) {
+        const uint32_t v = vs + (j % STAGES) * TILE;
+#pragma unroll
+        for (int c = 0; c < PT_N / 16; ++c)
+          mma_ts(lead, tmem + o_col + (TILES == 2 ? D * i : 0), tmem + s_col + 128 * i + 64 * (c >> 2) + 8 * (c & 3), desc(v + c * 2 * GROUP, GROUP, 1024),
+                 ID_O, (j > 0) | (c > 0));
       };
       bool ok = warp_wait(&bars.q_full, 0) && warp_wait(&bars.k_full[0], 0);
       if (ok) {
@@ -306,14 +318,30 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
       }
       for (int j = 0; ok && j < n; ++j) {
         const int s = j % STAGES, s1 = (j + 1) % STAGES;
+        if constexpr (TILES == 1) {
+          // the next block's scores, in the other buffer, keep the tensor cores busy during this block's softmax
+          if (j + 1 < n) {
+            ok = warp_wait(&bars.k_full[s1], ((j + 1) / STAGES) & 1);
+            if (!ok) break;
+            fence_after();
+            scores((j + 1) & 1, j + 1);
+            commit(lead, &bars.k_empty[s1]);
+          }
+          ok = warp_wait(&bars.v_full[s], (j / STAGES) & 1) && warp_wait(&bars.p_ready[j & 1], (j >> 1) & 1);
+          if (!ok) break;
+          fence_after();
+          values(j & 1, j);
+          commit(lead, &bars.o_step);
+          commit(lead, &bars.v_empty[s]);
+          if (j + 1 == n) commit(lead, &bars.o_full[0]);
+          continue;
+        }
         ok = warp_wait(&bars.v_full[s], (j / STAGES) & 1);
         for (int i = 0; ok && i < tiles; ++i) {
           ok = warp_wait(&bars.p_ready[i], j & 1);
           if (!ok) break;
           fence_after();
-#pragma unroll
-          for (int c = 0; c < PT_N / 16; ++c)
-            mma_ts(lead, tmem + o_col + D * i, tmem + s_col + 128 * i + 64 * (c >> 2) + 8 * (c & 3), desc(vs + s * TILE + c * 2 * GROUP, GROUP, 1024), ID_O, (j > 0) | (c > 0));
+          values(i, j);
           if (j + 1 < n) {
             if (i == 0) ok = warp_wait(&bars.k_full[s1], ((j + 1) / STAGES) & 1);
             if (!ok) break;
@@ -331,9 +359,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
       failed = !ok;
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");
+    if constexpr (TILES == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");  // one tile: 384 threads have 168 anyway
     // ---- queries
-    for (int i = threadIdx.x; i < tiles * 128 * CH; i += 64 * PT_TW) {
+    for (int i = threadIdx.x; i < tiles * 128 * CH; i += LOAD_WARP * 32) {
       const int r = i / CH, ch = i % CH, fr = t.f0 + r, tok = fast_div(fr, p.group_div);
       const bool live = r < t.rows;
       const T* src = static_cast<const T*>(a.q) + (live ? (t.first + tok) * a.q_stride_t + (kvh * p.group + fr - tok * p.group) * a.q_stride_h + ch * 8 : 0);
@@ -352,12 +380,14 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
       const int tok = fast_div(f, p.group_div), h = kvh * p.group + f - tok * p.group, pos = t.past + tok;
       const float slope = a.slopes && f < last ? a.slopes[h] * kLog2e : 0.f;
       const uint32_t lanes = uint32_t(32 * (warp & 3)) << 16;
-      const uint32_t ts = tmem + lanes + s_col + 128 * i, to = tmem + lanes + o_col + D * i + half * (D / PT_SPLIT);
+      const uint32_t to = tmem + lanes + o_col + D * i + half * (D / PT_SPLIT);
       float m = -INFINITY;  // reference maximum of the row, log2
       for (int j = 0; j < n; ++j) {
         const int base = base_of(j) + half * C;
         const bool part = !seen_by_all(base - half * C);
-        if (!warp_wait(&bars.s_full[i], j & 1)) bars.fail[i][warp & 3] = 1;
+        const int buf = TILES == 2 ? i : j & 1;  // of the scores
+        const uint32_t ts = tmem + lanes + s_col + 128 * buf;
+        if (!warp_wait(&bars.s_full[buf], (TILES == 2 ? j : j >> 1) & 1)) bars.fail[i][warp & 3] = 1;
         fence_after();
         // Two passes over the scores, 32 columns at a time, so that they need not stay in registers: the first
         // finds the maximum and puts capped, biased or masked scores back, the second makes the weights.
@@ -439,6 +469,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
         if (__any_sync(~0u, factor != 1.f)) {
           l *= factor;
           if (j > 0) {
+            if constexpr (TILES == 1) {  // these scores were multiplied before the last block's values
+              if (!warp_wait(&bars.o_step, (j - 1) & 1)) bars.fail[i][warp & 3] = 1;
+              fence_after();
+            }
 #pragma unroll
             for (int c = 0; c < D / PT_SPLIT / 32; ++c) {
               uint32_t o[32];
@@ -481,7 +515,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
         st_wait();
         fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&bars.p_ready[i]);
+        if (lane == 0) mbar_arrive(&bars.p_ready[buf]);
       }
       if (n > 0 && !failed && !warp_wait(&bars.o_full[i], 0)) failed = true;
       fence_after();
@@ -528,8 +562,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
           }
         }
         if (half == 0 && f < last) {
-          part[PT_ROWS * D + r] = m;
-          part[PT_ROWS * (D + 1) + r] = l;
+          part[ROWS * D + r] = m;
+          part[ROWS * (D + 1) + r] = l;
         }
       }
     }
@@ -537,7 +571,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
   if (failed) atomicOr(&g_prefill_fault, 1u);
   fence_before();
   __syncthreads();
-  if (warp == PT_MMA_WARP) {
+  if (warp == MMA_WARP) {
     fence_after();
     dealloc(bars.tmem, PT_COLS);
   }
@@ -546,27 +580,27 @@ __global__ void __launch_bounds__(PT_THREADS, 1) prefill_tc_kernel(const __grid_
     if (threadIdx.x == 0) pt.parts[(int64_t(blockIdx.x) + 1) * part_floats(D) - 4] = bars.special ? 1.f : 0.f;
     return;
   }
-  if (warp < PT_LOAD_WARP && bars.special && warp / PT_TW < tiles) {
+  if (warp < LOAD_WARP && bars.special && warp / PT_TW < tiles) {
     uint32_t redo = __ballot_sync(~0u, odd != 0.f && l == l && f < last);
     for (; redo; redo &= redo - 1) exact_row(p, t, kvh, __shfl_sync(~0u, f, __ffs(redo) - 1));
   }
 }
 
 // ---------------------------------------------------------------- join of split walks
-constexpr int PJ_THREADS = 256, PJ_ROWS = 32;
+constexpr int PJ_THREADS = 256;
 
 // PJ_ROWS rows of one tile and KV head, a warp each in turn: the shares in order.
 template <class DT, int D>
 __global__ void __launch_bounds__(PJ_THREADS) prefill_join_kernel(const __grid_constant__ PtParams pt) {
   using T = typename DT::T;
-  constexpr int E = D / 32;
+  constexpr int E = D / 32, ROWS = pt_rows(D);
   const PagedParams& p = pt.p;
   const smaq_paged_args& a = p.a;
   __shared__ int sums[PJ_THREADS / 32];
   __shared__ PrefillTile found;
-  const int chunk = int(blockIdx.x % (PT_ROWS / PJ_ROWS)), unit = int(blockIdx.x / (PT_ROWS / PJ_ROWS));
+  const int chunk = int(blockIdx.x % (ROWS / PJ_ROWS)), unit = int(blockIdx.x / (ROWS / PJ_ROWS));
   const int kvh = unit % a.n_kv_heads, tile = unit / a.n_kv_heads, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const PrefillTile t = find_tile<PJ_THREADS>(p, tile, PT_ROWS, true, sums, &found);
+  const PrefillTile t = find_tile<PJ_THREADS>(p, tile, ROWS, true, sums, &found);
   pdl_wait();  // every CTA waits, so this grid ends after the other
   const int shares = t.rows ? splits_of(PrefillBlocks(t, PT_N).count, pt.splits) : 0;
   if (shares < 2) return;
@@ -575,16 +609,16 @@ __global__ void __launch_bounds__(PJ_THREADS) prefill_join_kernel(const __grid_c
   for (int z = 0; z < shares; ++z) special |= parts[(z + 1) * part_floats(D) - 4] != 0.f;
   for (int r = chunk * PJ_ROWS + warp; r < min((chunk + 1) * PJ_ROWS, t.rows); r += PJ_THREADS / 32) {
     float m = -INFINITY, l = 0.f, o[E] = {};
-    for (int z = 0; z < shares; ++z) m = fmaxf(m, parts[z * part_floats(D) + PT_ROWS * D + r]);
+    for (int z = 0; z < shares; ++z) m = fmaxf(m, parts[z * part_floats(D) + ROWS * D + r]);
     const float base = m == -INFINITY ? 0.f : m;
 #pragma unroll 4
     for (int z = 0; z < shares; ++z) {
       const float* part = parts + z * part_floats(D);
-      const float f = ex2(part[PT_ROWS * D + r] - base);
-      l += f * part[PT_ROWS * (D + 1) + r];
+      const float f = ex2(part[ROWS * D + r] - base);
+      l += f * part[ROWS * (D + 1) + r];
       float x[E];
-      if constexpr (E == 4) *reinterpret_cast<float4*>(x) = *reinterpret_cast<const float4*>(part + r * D + 4 * lane);
-      else *reinterpret_cast<float2*>(x) = *reinterpret_cast<const float2*>(part + r * D + 2 * lane);
+#pragma unroll
+      for (int e = 0; e < E; e += 2) *reinterpret_cast<float2*>(x + e) = *reinterpret_cast<const float2*>(part + r * D + E * lane + e);
 #pragma unroll
       for (int e = 0; e < E; ++e) o[e] += f * x[e];
     }
@@ -635,10 +669,13 @@ bool encode(CUtensorMap* map, const smaq_paged_args& a, const void* cache, int b
             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-int64_t grid_tiles(int64_t n_rows, int batch, int group) { return std::max<int64_t>(1, most_tiles(n_rows, batch, group, PT_ROWS)); }
+int64_t grid_tiles(int64_t n_rows, int batch, int group, int D) { return std::max<int64_t>(1, most_tiles(n_rows, batch, group, pt_rows(D))); }
 // CTAs a tile: walks are shared where the tiles alone leave half of the GPU idle.  (The host does not know how long
-// the walks are: a CTA without a share ends at once.)  16 rows of 32/8 heads behind 16K tokens: 227 -> SPLIT_US us.
-int splits_for(int64_t units) { return int(std::max<int64_t>(1, std::min<int64_t>(32, num_sms() / std::max<int64_t>(units, 1)))); }
+// the walks are: a CTA without a share ends at once.)  16 rows of 32/8 heads behind 16K tokens: 227 -> 46 us.
+int splits_for(int64_t units, int64_t max_tokens) {
+  const int64_t idle = num_sms() / std::max<int64_t>(units, 1), worth = max_tokens / (2 * PT_N);  // two blocks a share
+  return int(std::max<int64_t>(1, std::min<int64_t>(32, std::min(idle, worth))));
+}
 
 template <class DT, int D>
 int launch(const PagedParams& p, cudaStream_t st) {
@@ -653,19 +690,19 @@ int launch(const PagedParams& p, cudaStream_t st) {
               : a.softcap > 0.f            ? prefill_tc_kernel<DT, D, PT_CAP>
                                            : prefill_tc_kernel<DT, D, PT_PLAIN>;
   if (const int rc = allow_smem(reinterpret_cast<const void*>(kern), PtCfg<D>::SMEM, "paged_prefill")) return rc;
-  const int64_t units = grid_tiles(a.n_rows, a.batch, p.group) * a.n_kv_heads;
-  pt.splits = splits_for(units);
+  const int64_t units = grid_tiles(a.n_rows, a.batch, p.group, D) * a.n_kv_heads;
+  pt.splits = splits_for(units, int64_t(a.max_blocks) * a.page_size);
   pt.parts = static_cast<float*>(a.workspace);
-  if (units * pt.splits * (PT_ROWS / PJ_ROWS) >= (int64_t(1) << 31)) return fail(SMAQ_ERR_UNSUPPORTED, "paged_prefill: too many rows");
-  const size_t need = prefill_tc_workspace(a.n_rows, a.batch, a.n_q_heads, a.n_kv_heads, D);
+  if (units * pt.splits * (pt_rows(D) / PJ_ROWS) >= (int64_t(1) << 31)) return fail(SMAQ_ERR_UNSUPPORTED, "paged_prefill: too many rows");
+  const size_t need = prefill_tc_workspace(a.n_rows, a.batch, a.n_q_heads, a.n_kv_heads, D, int64_t(a.max_blocks) * a.page_size);
   if (need && (!a.workspace || a.workspace_bytes < need))
     return fail(SMAQ_ERR_WORKSPACE, "paged_prefill: workspace %zu bytes, needs %zu", a.workspace ? a.workspace_bytes : size_t(0), need);
   if (need && reinterpret_cast<uintptr_t>(a.workspace) % 16) return fail(SMAQ_ERR_INVALID, "paged_prefill: workspace must be 16-byte aligned");
-  kern<<<unsigned(units * pt.splits), PT_THREADS, PtCfg<D>::SMEM, st>>>(pt);
+  kern<<<unsigned(units * pt.splits), pt_threads(D), PtCfg<D>::SMEM, st>>>(pt);
   const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess || pt.splits == 1) return cuda_status(e, "paged_prefill");
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(unsigned(units * (PT_ROWS / PJ_ROWS)));
+  cfg.gridDim = dim3(unsigned(units * (pt_rows(D) / PJ_ROWS)));
   cfg.blockDim = dim3(PJ_THREADS);
   cfg.stream = st;
   cudaLaunchAttribute attr;
@@ -678,23 +715,27 @@ int launch(const PagedParams& p, cudaStream_t st) {
 
 }  // namespace
 
-size_t prefill_tc_workspace(int64_t n_rows, int batch, int n_q_heads, int n_kv_heads, int head_dim) {
+size_t prefill_tc_workspace(int64_t n_rows, int batch, int n_q_heads, int n_kv_heads, int head_dim, int64_t max_tokens) {
   if (n_rows <= 0 || batch < 0 || n_kv_heads <= 0 || n_q_heads < n_kv_heads) return 0;
-  const int64_t units = grid_tiles(n_rows, batch, n_q_heads / n_kv_heads) * n_kv_heads;
-  const int splits = splits_for(units);
+  const int64_t units = grid_tiles(n_rows, batch, n_q_heads / n_kv_heads, head_dim) * n_kv_heads;
+  const int splits = splits_for(units, max_tokens);
   return splits > 1 ? size_t(units) * splits * part_floats(head_dim) * sizeof(float) : 0;
 }
 
 bool prefill_tc_eligible(const smaq_paged_args& a) {
-#ifdef NO_TC
-  return false;
-#endif
-  return a.dtype != SMAQ_F32 && (a.head_dim == 64 || a.head_dim == 128) && paged_aligned(a);
+  // Walks of one block leave the tensor cores nothing to overlap: up to 128 tokens of table the warp-level kernel
+  // takes 16.5 us a call (host included) where this one takes 20; at 256 tokens both take 20, from 512 on this one wins.
+  if (int64_t(a.max_blocks) * a.page_size <= PT_N) return false;
+  return a.dtype != SMAQ_F32 && (a.head_dim == 64 || a.head_dim == 128 || a.head_dim == 256) && paged_aligned(a);
 }
 
 int launch_prefill_tc(const PagedParams& p, cudaStream_t st) {
-  if (p.a.dtype == SMAQ_BF16) return p.a.head_dim == 64 ? launch<BF16, 64>(p, st) : launch<BF16, 128>(p, st);
-  return p.a.head_dim == 64 ? launch<F16, 64>(p, st) : launch<F16, 128>(p, st);
+  const bool bf16 = p.a.dtype == SMAQ_BF16;
+  switch (p.a.head_dim) {
+    case 64: return bf16 ? launch<BF16, 64>(p, st) : launch<F16, 64>(p, st);
+    case 128: return bf16 ? launch<BF16, 128>(p, st) : launch<F16, 128>(p, st);
+    default: return bf16 ? launch<BF16, 256>(p, st) : launch<F16, 256>(p, st);
+  }
 }
 
 }  // namespace smaq

@@ -686,8 +686,10 @@ def paged_decode_workspace_bytes(batch: int, n_q_heads: int, n_kv_heads: int, he
     return int(_lib.load().smaq_paged_decode_workspace_size(batch, n_q_heads, n_kv_heads, head_dim))
 
 
-def paged_prefill_workspace_bytes(n_rows: int, batch: int, n_q_heads: int, n_kv_heads: int, head_dim: int) -> int:
-    return int(_lib.load().smaq_paged_prefill_workspace_size(n_rows, batch, n_q_heads, n_kv_heads, head_dim))
+def paged_prefill_workspace_bytes(n_rows: int, batch: int, n_q_heads: int, n_kv_heads: int, head_dim: int,
+                                  max_tokens: int = 2 ** 31) -> int:
+    """``max_tokens``: what the block table has room for (``M * page_size``)."""
+    return int(_lib.load().smaq_paged_prefill_workspace_size(n_rows, batch, n_q_heads, n_kv_heads, head_dim, max_tokens))
 
 
 def _paged(name, q, k_cache, v_cache, block_table, seq_lens, cu_query, prefix_lens, scale, window, softcap, slopes,
@@ -737,7 +739,8 @@ def _paged(name, q, k_cache, v_cache, block_table, seq_lens, cu_query, prefix_le
         call, need = lib.smaq_paged_decode, lib.smaq_paged_decode_workspace_size(B, Hq, Hk, D)
     else:
         cu_query = _int32("cu_query", cu_query, B + 1)
-        call, need = lib.smaq_paged_prefill, lib.smaq_paged_prefill_workspace_size(T, B, Hq, Hk, D)
+        call, need = lib.smaq_paged_prefill, lib.smaq_paged_prefill_workspace_size(T, B, Hq, Hk, D,
+                                                                                     M * page_size)
     if workspace is None and need:
         workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
     if workspace is not None:
