@@ -242,7 +242,8 @@ struct Feed {
   static constexpr int CH = ROW / 16;  // 16-byte chunks a token; chunk c of row r lies at c ^ (r % 8)
   Walk in;
   int count, looked = 0, issued = 0;
-  int64_t row_off = -1;  // offset of token (lane & 15) of the unit looked up last, < 0: not visible
+  const uint8_t* row = nullptr;  // this lane's chunk of the keys of token (lane & 15) of the unit looked up last
+  uint32_t visible_rows = 0;     // bit r: token r of it is visible, from this lane's first row on
   uint8_t* ring;
 
   __device__ __forceinline__ void start(const DecodeParamsX& d, int b, int64_t into, int units, uint8_t* at) {
@@ -260,24 +261,30 @@ struct Feed {
     if (looked >= count) return;
     if (looked) in.next(d);
     ++looked;
-    const int lane = threadIdx.x & 31, j = in.v.lo + in.t * PD_UNIT + (threadIdx.x >> 5) * 16 + (lane & 15);
-    row_off = -1;
+    const int lane = threadIdx.x & 31, j0 = in.v.lo + in.t * PD_UNIT + (threadIdx.x >> 5) * 16, j = j0 + (lane & 15);
+    const int n = min(max(in.v.hi - j0, 0), 16);
+    int64_t off = 0;
     if (j < in.v.hi)
-      row_off = token_offset(d.p, d.p.a.block_table + in.b * d.p.a.table_stride, j) + int64_t(in.s / d.tiles) * d.p.a.c_stride_h;
+      off = token_offset(d.p, d.p.a.block_table + in.b * d.p.a.table_stride, j) + int64_t(in.s / d.tiles) * d.p.a.c_stride_h;
+    row = static_cast<const uint8_t*>(d.p.a.k_cache) + off * int64_t(sizeof(T));
+    visible_rows = ((1u << n) - 1u) >> (lane / CH);
   }
   __device__ __forceinline__ void issue(const DecodeParamsX& d) {
     if (issued < count) {
       const int lane = threadIdx.x & 31;
+      // a step is 32 / CH rows; the swizzle of its first row is a constant, that of the lane's row within it is not
+      constexpr int PER = 32 / CH;
+      const int mine = lane / CH, ch = lane % CH;
       const uint32_t st = smem_u32(ring + (issued % S::N) * S::BYTES);
+      const uint32_t lane_dst = uint32_t(mine * ROW + ((ch ^ mine) << 4));
+      const int64_t to_values = static_cast<const uint8_t*>(d.p.a.v_cache) - static_cast<const uint8_t*>(d.p.a.k_cache) + ch * 16;
 #pragma unroll
-      for (int i = 0; i < 16 * CH / 32; ++i) {
-        const int r = (i * 32 + lane) / CH, ch = (i * 32 + lane) % CH;
-        const int64_t off = __shfl_sync(~0u, row_off, r);
-        const uint32_t at = st + uint32_t(r * ROW + ((ch ^ (r & 7)) << 4));
-        const int64_t from = (off < 0 ? 0 : off) + ch * int(16 / sizeof(T));
-        const uint32_t n = off < 0 ? 0u : 16u;
-        cp_async16(at, static_cast<const T*>(d.p.a.k_cache) + from, n);
-        cp_async16(at + 16 * ROW, static_cast<const T*>(d.p.a.v_cache) + from, n);
+      for (int i = 0; i < 16 / PER; ++i) {
+        const uint8_t* from = reinterpret_cast<const uint8_t*>(__shfl_sync(~0u, reinterpret_cast<uint64_t>(row), i * PER + mine));
+        const uint32_t at = st + uint32_t(i * PER * ROW) + (lane_dst ^ uint32_t((i * PER & 7) << 4));
+        const uint32_t n = (visible_rows >> (i * PER) & 1u) << 4;
+        cp_async16(at, from + ch * 16, n);
+        cp_async16(at + 16 * ROW, from + to_values, n);
       }
       ++issued;
     }

@@ -473,7 +473,7 @@ __global__ void __launch_bounds__(pt_threads(D), 1) prefill_tc_kernel(const __gr
               if (!warp_wait(&bars.o_step, (j - 1) & 1)) bars.fail[i][warp & 3] = 1;
               fence_after();
             }
-#pragma unroll
+#pragma unroll 1  // cold: unrolled, its code costs the first pass 10 us of 519
             for (int c = 0; c < D / PT_SPLIT / 32; ++c) {
               uint32_t o[32];
               ld32(to + 32 * c, o);
@@ -525,7 +525,7 @@ __global__ void __launch_bounds__(pt_threads(D), 1) prefill_tc_kernel(const __gr
       if (alone) {
         const float inv = l == 0.f ? 0.f : 1.0f / l;
         T* out = static_cast<T*>(a.out) + int64_t(t.first + tok) * a.o_stride_t + h * a.o_stride_h + half * (D / PT_SPLIT);
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < D / PT_SPLIT / 32; ++c) {
           uint32_t o[32], w[16];
           if (n > 0) {
@@ -550,7 +550,7 @@ __global__ void __launch_bounds__(pt_threads(D), 1) prefill_tc_kernel(const __gr
       } else {
         float* part = pt.parts + int64_t(blockIdx.x) * part_floats(D);
         const int r = 128 * i + row;
-#pragma unroll
+#pragma unroll 1
         for (int c = 0; c < D / PT_SPLIT / 32; ++c) {
           uint32_t o[32];
           ld32(to + 32 * c, o);
