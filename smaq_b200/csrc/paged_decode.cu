@@ -6,7 +6,7 @@
 // so the design is about bytes in flight and an even split.
 //
 // Split.  A segment is (request, KV head, tile of up to 16 query heads); its visible tokens are cut into
-// units of 64, and the units of all segments, in order, are cut into equal runs, one a CTA (two CTAs an
+// units of 64, and the units of all segments, in order, are cut into runs of equal cost, one a CTA (two CTAs an
 // SM), whatever the lengths.  Each CTA finds its run from seq_lens by itself.  A segment that lies in one
 // run is finished there; of the others every CTA leaves (m, sum, accumulator) in slot cta + segment, which is
 // distinct because a run's walk raises one of the two at each step, and the join kernel, launched with
@@ -114,59 +114,10 @@ __device__ __forceinline__ int64_t block_prefix(int64_t v, int64_t* warp_sums, i
   return total;
 }
 
-struct RunStart {
-  int64_t total;       // units of all segments
-  int b;               // request the run begins in
-  int64_t into;        // units into that request
-};
-
-// Total units, and where unit `u(total)` lies.
-template <class F>
-__device__ __forceinline__ RunStart find_run(const DecodeParamsX& d, int64_t* warp_sums, int* found_b, int64_t* found_into, F unit_of_total) {
-  RunStart r;
-  const int B = d.p.a.batch;
-  r.total = 0;
-  int64_t mine = 0, before = 0;
-  for (int b0 = 0; b0 < B; b0 += PD_THREADS) {
-    const int b = b0 + threadIdx.x;
-    mine = b < B ? int64_t(visible(d.p, b).units) * d.segs : 0;
-    r.total += block_prefix(mine, warp_sums, before);
-  }
-  const int64_t u = unit_of_total(r.total);
-  if (B <= PD_THREADS) {
-    if (u >= before && u < before + mine) {
-      *found_b = threadIdx.x;
-      *found_into = u - before;
-    }
-  } else {
-    int64_t base = 0;
-    for (int b0 = 0; b0 < B && base <= u; b0 += PD_THREADS) {
-      const int b = b0 + threadIdx.x;
-      mine = b < B ? int64_t(visible(d.p, b).units) * d.segs : 0;
-      const int64_t sum = block_prefix(mine, warp_sums, before);
-      if (u >= base + before && u < base + before + mine) {
-        *found_b = b;
-        *found_into = u - base - before;
-      }
-      base += sum;
-    }
-  }
-  __syncthreads();
-  r.b = *found_b;
-  r.into = *found_into;
-  return r;
-}
-
 // Walks the units of a run in order: request, segment of it, unit of the segment.
 struct Walk {
   int b, s, t;
   Visible v;
-  __device__ __forceinline__ void start(const DecodeParamsX& d, int b_, int64_t into) {
-    b = b_;
-    v = visible(d.p, b);
-    s = int(into / v.units);
-    t = int(into - int64_t(s) * v.units);
-  }
   // to the next unit; the caller knows that one exists
   __device__ __forceinline__ void next(const DecodeParamsX& d) {
     if (++t < v.units) return;
@@ -180,14 +131,72 @@ struct Walk {
   }
 };
 
-// Run of CTA c: units [first(c), first(c + 1)).  With fewer units than CTAs the first `total` CTAs get one
-// each, so that no CTA within a segment's range is without a slot.
+// Runs are equal in cost: a unit costs 1, and beginning a segment (its queries, and joining the warps at its end) as
+// much as PD_START units of a CTA among others.  Without that, CTAs that met many short segments ended 10 us after the
+// others in a ragged windowed batch.  The cost of a request's segments and how many requests have any, packed:
+constexpr int PD_START = 1, PD_PACK = 24;  // batch < 2^24
+__device__ __forceinline__ int64_t packed_cost(const DecodeParamsX& d, int b) {
+  const int units = b < d.p.a.batch ? visible(d.p, b).units : 0;
+  return units ? (int64_t(units + PD_START) * d.segs << PD_PACK) + 1 : 0;
+}
+// Run of CTA c: costs [first(c), first(c + 1)).  With a total below the number of CTAs, the first ones get 1
+// each, so that no CTA between those of a segment's first and last unit is without a unit of it.
 __device__ __forceinline__ int64_t run_first(int64_t c, int64_t total, int grid) {
   return total < grid ? min(c, total) : c * total / grid;
 }
-// The CTA that has unit u.
+// The CTA that has cost position u.
 __device__ __forceinline__ int run_of(int64_t u, int64_t total, int grid) {
   return total < grid ? int(u) : int(((u + 1) * grid - 1) / total);
+}
+
+struct Spot {
+  int b, s, t;    // a unit
+  int64_t index;  // its number among all units
+};
+struct RunShared {
+  int64_t warp_sums[PD_THREADS / 32];
+  Spot spot[2];
+};
+
+// The CTA's run: its first unit and the number of its units.
+__device__ __forceinline__ int find_run(const DecodeParamsX& d, RunShared& sh, Walk& at) {
+  const int B = d.p.a.batch;
+  int64_t sum = 0, mine = 0, before = 0;
+  for (int b0 = 0; b0 < B; b0 += PD_THREADS) {
+    mine = packed_cost(d, b0 + threadIdx.x);
+    sum += block_prefix(mine, sh.warp_sums, before);
+  }
+  constexpr int64_t COUNT = (int64_t(1) << PD_PACK) - 1;
+  const int64_t total = sum >> PD_PACK;
+  const int64_t ends[2] = {run_first(blockIdx.x, total, d.grid), run_first(int64_t(blockIdx.x) + 1, total, d.grid)};
+  if (ends[0] == ends[1]) return 0;
+  if (threadIdx.x == 0) sh.spot[1].index = total - (sum & COUNT) * PD_START * d.segs;  // the end of all
+  __syncthreads();
+  int64_t base = 0;
+  for (int b0 = 0; b0 < B && (base >> PD_PACK) <= ends[1]; b0 += PD_THREADS) {
+    int64_t chunk = sum;
+    if (B > PD_THREADS) {
+      mine = packed_cost(d, b0 + threadIdx.x);
+      chunk = block_prefix(mine, sh.warp_sums, before);
+    }
+    const int64_t from = base + before, cost = from >> PD_PACK;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int64_t into = ends[e] - cost;
+      if (mine && into >= 0 && into < mine >> PD_PACK) {
+        const int per = int((mine >> PD_PACK) / d.segs), s = int(into / per), t = max(int(into - int64_t(s) * per) - PD_START, 0);
+        const int units = per - PD_START;
+        sh.spot[e] = {b0 + int(threadIdx.x), s, t, cost - (from & COUNT) * PD_START * d.segs + int64_t(s) * units + t};
+      }
+    }
+    base += chunk;
+  }
+  __syncthreads();
+  at.b = sh.spot[0].b;
+  at.s = sh.spot[0].s;
+  at.t = sh.spot[0].t;
+  at.v = visible(d.p, at.b);
+  return int(sh.spot[1].index - sh.spot[0].index);
 }
 
 // Rows of requests that see nothing.
@@ -246,15 +255,24 @@ struct Feed {
   uint32_t visible_rows = 0;     // bit r: token r of it is visible, from this lane's first row on
   uint8_t* ring;
 
-  __device__ __forceinline__ void start(const DecodeParamsX& d, int b, int64_t into, int units, uint8_t* at) {
-    in.start(d, b, into);
+  __device__ __forceinline__ void start(const DecodeParamsX& d, const Walk& first, int units, uint8_t* at) {
+    in = first;
     count = units;
     ring = at;
-    look_up(d);
-#pragma unroll 1
-    for (int i = 0; i < S::N - 1; ++i) {
-      issue(d);
+    // the first stages' lookups side by side: one after the other they took 3 us before the first copy
+    const uint8_t* rows[S::N];
+    uint32_t seen[S::N];
+#pragma unroll
+    for (int i = 0; i < S::N; ++i) {
       look_up(d);
+      rows[i] = row;
+      seen[i] = visible_rows;
+    }
+#pragma unroll
+    for (int i = 0; i < S::N; ++i) {
+      row = rows[i];
+      visible_rows = seen[i];
+      if (i + 1 < S::N) issue(d);
     }
   }
   __device__ __forceinline__ void look_up(const DecodeParamsX& d) {
@@ -314,27 +332,22 @@ __global__ void __launch_bounds__(PD_THREADS, Stages<2 * D>::CTAS) paged_decode_
   constexpr int KS = D / 16;        // contraction steps of the scores
   constexpr int NT = D / 8;         // output column tiles
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int64_t warp_sums[PD_THREADS / 32], found_into;
-  __shared__ int found_b;
+  __shared__ RunShared run;
   const PagedParams& p = d.p;
   const smaq_paged_args& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_launch_dependents();
-  write_empty(d);
-  const RunStart run = find_run(d, warp_sums, &found_b, &found_into,
-                                [&](int64_t total) { return run_first(blockIdx.x, total, d.grid); });
-  const int64_t u0 = run_first(blockIdx.x, run.total, d.grid), u1 = run_first(int64_t(blockIdx.x) + 1, run.total, d.grid);
-  const int count = int(u1 - u0);
-  if (count <= 0) return;
+  Walk at;
+  const int count = find_run(d, run, at);
 
   using S = Stages<2 * D>;
   float* merge = reinterpret_cast<float*>(smem + 4 * S::N * S::BYTES);
   Feed<T, 2 * D> feed;
-  feed.start(d, run.b, run.into, count, smem + warp * S::N * S::BYTES);
+  if (count > 0) feed.start(d, at, count, smem + warp * S::N * S::BYTES);
+  write_empty(d);  // behind the first copies
+  if (count <= 0) return;
 
   // ---- compute
-  Walk at;
-  at.start(d, run.b, run.into);
   uint32_t qf[KS][4];
   float o[NT][4];
   float m0, m1, l0, l1;  // rows lane / 4 and lane / 4 + 8
@@ -566,24 +579,20 @@ __global__ void __launch_bounds__(PD_THREADS, Stages<4 * D>::CTAS) paged_decode_
   using S = Stages<4 * D>;
   constexpr int E = D / 32, LD = D + 2;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int64_t warp_sums[PD_THREADS / 32], found_into;
-  __shared__ int found_b;
+  __shared__ RunShared run;
   const PagedParams& p = d.p;
   const smaq_paged_args& a = p.a;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_launch_dependents();
-  write_empty(d);
-  const RunStart run = find_run(d, warp_sums, &found_b, &found_into, [&](int64_t total) { return run_first(blockIdx.x, total, d.grid); });
-  const int64_t u0 = run_first(blockIdx.x, run.total, d.grid), u1 = run_first(int64_t(blockIdx.x) + 1, run.total, d.grid);
-  const int count = int(u1 - u0);
-  if (count <= 0) return;
+  Walk at;
+  const int count = find_run(d, run, at);
   Feed<float, 4 * D> feed;
-  feed.start(d, run.b, run.into, count, smem + warp * S::N * S::BYTES);
+  if (count > 0) feed.start(d, at, count, smem + warp * S::N * S::BYTES);
+  write_empty(d);  // behind the first copies
+  if (count <= 0) return;
   float* areas = reinterpret_cast<float*>(smem + 4 * S::N * S::BYTES);
   float *mine = areas + warp * Q::AREA, *ps = areas + 4 * Q::AREA + warp * 16 * R;
 
-  Walk at;
-  at.start(d, run.b, run.into);
   const int tok = lane & 15, half = lane >> 4;
   float o[R][E], m[R], l[R], slope[R];
   bool fresh = true;
@@ -753,8 +762,7 @@ template <class DT, int NI, bool VEC>
 __global__ void __launch_bounds__(PD_THREADS) paged_simt_kernel(const __grid_constant__ DecodeParamsX d) {
   using T = typename DT::T;
   constexpr int GROUPS = PD_THREADS / 8;
-  __shared__ int64_t warp_sums[PD_THREADS / 32], found_into;
-  __shared__ int found_b;
+  __shared__ RunShared run;
   __shared__ __align__(16) float qs[PS_ROWS][32 * NI];
   __shared__ float acc[PD_THREADS / 32][PS_ROWS][32 * NI + 2];
   const PagedParams& p = d.p;
@@ -762,13 +770,9 @@ __global__ void __launch_bounds__(PD_THREADS) paged_simt_kernel(const __grid_con
   const int D = a.head_dim, LD = D + 2, l = threadIdx.x & 7, grp = threadIdx.x >> 3, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   pdl_launch_dependents();
   write_empty(d);
-  const RunStart run = find_run(d, warp_sums, &found_b, &found_into,
-                                [&](int64_t total) { return run_first(blockIdx.x, total, d.grid); });
-  const int64_t u0 = run_first(blockIdx.x, run.total, d.grid), u1 = run_first(int64_t(blockIdx.x) + 1, run.total, d.grid);
-  int left = int(u1 - u0);
-  if (left <= 0) return;
   Walk at;
-  at.start(d, run.b, run.into);
+  int left = find_run(d, run, at);
+  if (left <= 0) return;
   while (left > 0) {
     const int n = min(left, at.v.units - at.t);  // units of this segment in the run
     const int kvh = at.s / d.tiles, tile = at.s - kvh * d.tiles;
@@ -928,20 +932,19 @@ __global__ void __launch_bounds__(PD_THREADS) paged_join_kernel(const __grid_con
   const int b = blockIdx.x / a.n_q_heads, h = blockIdx.x - b * a.n_q_heads, D = a.head_dim, LD = D + 2;
   const int kvh = h / p.group, tile = (h - kvh * p.group) / tile_rows, r = h - kvh * p.group - tile * tile_rows;
   const int s = kvh * d.tiles + tile;
-  int64_t total = 0;
+  int64_t costs = 0;
   for (int b0 = 0; b0 < a.batch; b0 += PD_THREADS) {
-    const int i = b0 + threadIdx.x;
     int64_t before;
-    const int64_t mine = i < a.batch ? int64_t(visible(p, i).units) * d.segs : 0;
-    const int64_t sum = block_prefix(mine, warp_sums, before);
-    if (i == b) my_first = total + before;
-    total += sum;
+    const int64_t chunk = block_prefix(packed_cost(d, b0 + threadIdx.x), warp_sums, before);
+    if (b0 + int(threadIdx.x) == b) my_first = (costs + before) >> PD_PACK;
+    costs += chunk;
   }
   __syncthreads();
+  const int64_t total = costs >> PD_PACK;
   const int units = visible(p, b).units;
   pdl_wait();  // the slots are complete from here on; every CTA waits, so this grid ends after the other
   if (units == 0) return;
-  const int64_t f = my_first + int64_t(s) * units, e = f + units - 1;
+  const int64_t f = my_first + int64_t(s) * (units + PD_START) + PD_START, e = f + units - 1;
   const int c0 = run_of(f, total, d.grid), c1 = run_of(e, total, d.grid);
   if (c0 == c1) return;
   const int64_t step = int64_t(d.rows) * LD;
@@ -1054,6 +1057,7 @@ extern "C" int smaq_paged_decode(const smaq_paged_args* args, void* stream) {
   const smaq_paged_args& a = d.p.a;
   if (a.n_rows != a.batch) return fail(SMAQ_ERR_INVALID, "paged_decode: %lld rows for batch %d (one row a request)", (long long)a.n_rows, a.batch);
   if (a.batch == 0) return SMAQ_OK;
+  if (a.batch >= 1 << PD_PACK) return fail(SMAQ_ERR_UNSUPPORTED, "paged_decode: batch %d", a.batch);
   const size_t need = smaq_paged_decode_workspace_size(a.batch, a.n_q_heads, a.n_kv_heads, a.head_dim);
   if (!a.workspace || a.workspace_bytes < need)
     return fail(SMAQ_ERR_WORKSPACE, "paged_decode: workspace %zu bytes, needs %zu", a.workspace ? a.workspace_bytes : size_t(0), need);
