@@ -490,9 +490,9 @@ int smaq_paged_decode(const smaq_paged_args* args, void* stream);
 size_t smaq_paged_prefill_workspace_size(int64_t n_rows, int batch, int n_q_heads, int n_kv_heads, int head_dim,
                                          int64_t max_tokens /* max_blocks * page_size */);
 int smaq_paged_prefill(const smaq_paged_args* args, void* stream);
-/* SMAQ_ERR_DEVICE if a bounded wait of the tensor-core prefill kernel ran out since the last check
- * (clears it).  Synchronises the stream. */
-int smaq_prefill_status(void* stream);
+/* SMAQ_ERR_DEVICE if a bounded wait of smaq_paged_prefill or smaq_norm_rope ran out since the last
+ * check (clears it).  Synchronises the stream. */
+int smaq_exact_status(void* stream);
 /* sizeof(smaq_tables_args), smaq_norm_rope_args, smaq_paged_args for which = 0, 1, 2, else 0. */
 size_t smaq_paged_args_size(int which);
 

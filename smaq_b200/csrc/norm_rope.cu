@@ -10,6 +10,7 @@
 // are read once into registers and serve all heads that the lane group walks; it walks more heads a token
 // when there are enough tokens to fill the GPU, and loads a head ahead.  Values are copied by the same
 // walk.  Bound by HBM bytes for prompts, by latency for decode steps.
+// norm_rope_staged_kernel: the same arithmetic for many tokens, rows staged in shared memory by bulk copies.
 // norm_rope_any_kernel: any head_dim and alignment, one warp a head, element by element.
 #include "common.cuh"
 #include "ptx.cuh"
@@ -64,6 +65,13 @@ __device__ __forceinline__ Vec8<DT> load8(const typename DT::T* p) {
   return v;
 }
 template <class DT>
+__device__ __forceinline__ Vec8<DT> load8s(const typename DT::T* p) {  // from shared memory
+  Vec8<DT> v;
+  v.u = *reinterpret_cast<const decltype(v.u)*>(p);
+  if constexpr (DT::code == SMAQ_F32) v.w = reinterpret_cast<const float4*>(p)[1];
+  return v;
+}
+template <class DT>
 __device__ __forceinline__ void store8(typename DT::T* p, const Vec8<DT>& v) {
   *reinterpret_cast<decltype(v.u)*>(p) = v.u;
   if constexpr (DT::code == SMAQ_F32) reinterpret_cast<float4*>(p)[1] = v.w;
@@ -110,6 +118,27 @@ __device__ __forceinline__ void load8f(const float* p, uint64_t* x) {
   x[1] = pair(u.z, u.w);
   x[2] = pair(w.x, w.y);
   x[3] = pair(w.z, w.w);
+}
+
+// Turns this lane's eight pairs.  Interleaved: the cosines and sines of vector a's four pairs, then b's.
+template <bool INTERLEAVED>
+__device__ __forceinline__ void rotate(uint64_t (&x)[8], const uint64_t (&c)[4], const uint64_t (&s)[4]) {
+  if constexpr (INTERLEAVED) {  // a packed pair is a rotated pair
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float2 u = split(x[i]), c2 = split(c[i >> 1]), s2 = split(s[i >> 1]);
+      const float cc = i & 1 ? c2.y : c2.x, sn = i & 1 ? s2.y : s2.x;
+      x[i] = pair(u.x * cc - u.y * sn, u.y * cc + u.x * sn);
+    }
+  } else {  // pair i is (i, i + 8) of this lane's sixteen
+    const uint64_t minus = pair(-1.0f, -1.0f);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint64_t u = x[i], v = x[i + 4];
+      x[i] = fma2(mul2(v, s[i]), minus, mul2(u, c[i]));
+      x[i + 4] = fma2(v, c[i], mul2(u, s[i]));
+    }
+  }
 }
 
 // LANES lanes a head (a power of two >= head_dim / 16).  A lane group walks `per` heads of one kind (queries, keys
@@ -221,24 +250,7 @@ __global__ void __launch_bounds__(NR_THREADS, NR_CTAS) norm_rope_kernel(const __
 #pragma unroll
       for (int i = 0; i < 8; ++i) x[i] = mul2(x[i], mul2(r2, w[i]));
     }
-    if (turned) {
-      if constexpr (INTERLEAVED) {  // a packed pair is a rotated pair
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float2 u = split(x[i]), c2 = split(c[i >> 1]), s2 = split(s[i >> 1]);
-          const float cc = i & 1 ? c2.y : c2.x, sn = i & 1 ? s2.y : s2.x;
-          x[i] = pair(u.x * cc - u.y * sn, u.y * cc + u.x * sn);
-        }
-      } else {  // pair i is (i, i + 8) of this lane's sixteen
-        const uint64_t minus = pair(-1.0f, -1.0f);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint64_t u = x[i], v = x[i + 4];
-          x[i] = fma2(mul2(v, s[i]), minus, mul2(u, c[i]));
-          x[i + 4] = fma2(v, c[i], mul2(u, s[i]));
-        }
-      }
-    }
+    if (turned) rotate<INTERLEAVED>(x, c, s);
     if (!live) continue;
     const Vec8<DT> va = pack8<DT>(x), vb = pack8<DT>(x + 4);
     if (dst) {
@@ -252,6 +264,172 @@ __global__ void __launch_bounds__(NR_THREADS, NR_CTAS) norm_rope_kernel(const __
       also += D;
     }
   }
+}
+
+// ---------------------------------------------------------------- many tokens
+// The rows of `per` tokens at a time come to shared memory by bulk copies, two batches in turn, so that bytes in
+// flight do not cost registers; a lane group then takes head after head of one token from there (8192 tokens at 32/8 heads:
+// 49 us, 4.2 TB/s; an elementwise pass over as many bytes takes 33).  Values go from shared memory
+// to the cache by bulk copies too.  For heads that lie side by side in a token.
+constexpr int NS_THREADS = 256, NS_CTAS = 2, NS_SMEM = 112 * 1024, NS_MOST = 8;
+constexpr int NS_ROUNDS = 5;
+constexpr uint32_t NS_SPIN = 1u << 24;
+
+__device__ unsigned int g_norm_rope_fault;
+
+__device__ __forceinline__ void bulk_s2g(void* dst, uint32_t src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes) : "memory");
+}
+
+struct NsBars {
+  uint64_t full[2];
+  int dead;             // a wait ran out
+  int pos[2][NS_MOST];  // table rows of a batch's tokens, < 0: outside the table
+};
+
+template <class DT, int LANES, bool INTERLEAVED>
+__global__ void __launch_bounds__(NS_THREADS, NS_CTAS) norm_rope_staged_kernel(const __grid_constant__ NrParams p) {
+  using T = typename DT::T;
+  constexpr int GROUPS = NS_THREADS / LANES;
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ NsBars bars;
+  const smaq_norm_rope_args& a = p.a;
+  const int D = a.head_dim, R = a.rotary_dim, lane = threadIdx.x % LANES, group = threadIdx.x / LANES;
+  const unsigned mask = (LANES == 32 ? ~0u : ((1u << LANES) - 1u) << ((threadIdx.x & 31) / LANES * LANES));
+  const uint32_t row = uint32_t(D * sizeof(T)), q_bytes = a.n_q_heads * row, k_bytes = a.n_kv_heads * row, r_bytes = R * 4;
+  const uint32_t v_bytes = a.k_cache ? k_bytes : 0, token = q_bytes + k_bytes + v_bytes + r_bytes, batch = token * p.per;
+  const bool live = lane < D / 16, turned = lane < R / 16;
+  const int ea = turned ? 8 * lane : R + 16 * (lane - R / 16), ahead = turned ? R / 2 : 8;
+  const int64_t batches = (a.n_tokens + p.per - 1) / p.per;
+  // A lane group serves one token of a batch: heads first, first + share, ..; its cosines and weights stay in registers.
+  const int share = GROUPS / p.per, mine = group / share, first = group - mine * share;
+  uint64_t wq[8] = {}, wk[8] = {};
+  if (live && a.q_weight) {
+    load8f(a.q_weight + ea, wq);
+    load8f(a.q_weight + ea + ahead, wq + 4);
+  }
+  if (live && a.k_weight) {
+    load8f(a.k_weight + ea, wk);
+    load8f(a.k_weight + ea + ahead, wk + 4);
+  }
+
+  // the first warp brings a batch: lane i its token i
+  auto bring = [&](int64_t n, int s) {
+    const int64_t t = n * p.per + threadIdx.x;
+    const bool has = int(threadIdx.x) < p.per && t < a.n_tokens;
+    const int pos = has ? a.positions[t] : -1;
+    const bool known = pos >= 0 && pos < a.n_positions;
+    if (has) bars.pos[s][threadIdx.x] = known ? pos : -1;
+    const uint32_t bytes = has ? token - (known ? 0 : r_bytes) : 0;
+    const uint32_t total = __reduce_add_sync(~0u, bytes);
+    __syncwarp();  // the positions are written before the arrival that publishes them
+    if (threadIdx.x == 0) mbar_arrive_expect_tx(&bars.full[s], total);
+    __syncwarp();
+    if (!has) return;
+    uint8_t* dst = smem + s * batch + threadIdx.x * token;
+    bulk_g2s(dst, static_cast<const T*>(a.q) + t * a.q_stride_t, q_bytes, &bars.full[s]);
+    bulk_g2s(dst + q_bytes, static_cast<const T*>(a.k) + t * a.k_stride_t, k_bytes, &bars.full[s]);
+    if (v_bytes) bulk_g2s(dst + q_bytes + k_bytes, static_cast<const T*>(a.v) + t * a.v_stride_t, v_bytes, &bars.full[s]);
+    if (known && r_bytes) bulk_g2s(dst + q_bytes + k_bytes + v_bytes, a.table + int64_t(pos) * R, r_bytes, &bars.full[s]);
+  };
+  if (threadIdx.x == 0) {
+    mbar_init(&bars.full[0], 1);
+    mbar_init(&bars.full[1], 1);
+    bars.dead = 0;
+    fence_mbar_init();
+  }
+  __syncthreads();
+  if (threadIdx.x < 32) {
+    bring(blockIdx.x, 0);
+    if (int64_t(blockIdx.x) + gridDim.x < batches) bring(int64_t(blockIdx.x) + gridDim.x, 1);
+  }
+  int turn = 0;
+  for (int64_t n = blockIdx.x; n < batches; n += gridDim.x, ++turn) {
+    const int s = turn & 1, tokens = int(min(int64_t(p.per), a.n_tokens - n * p.per));
+    if (!mbar_wait(&bars.full[s], (turn >> 1) & 1, NS_SPIN)) bars.dead = 1;
+    const uint8_t* base = smem + s * batch;
+    if (v_bytes && int(threadIdx.x) < tokens) {  // values: straight on
+      const int64_t t = n * p.per + threadIdx.x, at = slot_offset(p, a.slots[t]);
+      if (at >= 0) {
+        const uint32_t src = smem_u32(base) + threadIdx.x * token + q_bytes + k_bytes;
+        if (a.c_stride_h == D) bulk_s2g(static_cast<T*>(a.v_cache) + at, src, v_bytes);
+        else
+          for (int h = 0; h < a.n_kv_heads; ++h) bulk_s2g(static_cast<T*>(a.v_cache) + at + h * a.c_stride_h, src + h * row, row);
+      }
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    }
+    if (mine < tokens) {
+      const int64_t t = n * p.per + mine;
+      const uint8_t* rows = base + mine * token;
+      uint64_t c[4], sn[4];
+      if (turned) {
+        const float* cs = reinterpret_cast<const float*>(rows + q_bytes + k_bytes + v_bytes);
+        if (bars.pos[s][mine] >= 0) {
+          const float4* c4 = reinterpret_cast<const float4*>(cs + (INTERLEAVED ? ea / 2 : ea));
+          const float4* d4 = reinterpret_cast<const float4*>(cs + (INTERLEAVED ? (ea + ahead) / 2 : ea + 4));
+          const float4 c0 = c4[0], c1 = d4[0], s0 = c4[R / 8], s1 = d4[R / 8];
+          c[0] = pair(c0.x, c0.y); c[1] = pair(c0.z, c0.w); c[2] = pair(c1.x, c1.y); c[3] = pair(c1.z, c1.w);
+          sn[0] = pair(s0.x, s0.y); sn[1] = pair(s0.z, s0.w); sn[2] = pair(s1.x, s1.y); sn[3] = pair(s1.z, s1.w);
+        } else {
+          const float nan = __int_as_float(0x7FC00000);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) c[e] = sn[e] = pair(nan, nan);
+        }
+      }
+      auto turn_row = [&](const T* src, bool weighted, const uint64_t (&w)[8], T* dst, T* also) {
+        uint64_t x[8] = {};
+        if (live) {
+          const Vec8<DT> va = load8s<DT>(src), vb = load8s<DT>(src + ahead);
+          unpack8<DT>(va, x);
+          unpack8<DT>(vb, x + 4);
+        }
+        if (weighted) {
+          uint64_t sq[2] = {0, 0};
+#pragma unroll
+          for (int e = 0; e < 8; ++e) sq[e & 1] = fma2(x[e], x[e], sq[e & 1]);
+          const float2 f = split(add2(sq[0], sq[1]));
+          float ss = f.x + f.y;
+#pragma unroll
+          for (int o = LANES / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
+          const float r = rsqrtf(fmaf(ss, p.inv_dim, a.eps));
+          const uint64_t r2 = pair(r, r);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = mul2(x[e], mul2(r2, w[e]));
+        }
+        if (turned) rotate<INTERLEAVED>(x, c, sn);
+        if (!live) return;
+        const Vec8<DT> va = pack8<DT>(x), vb = pack8<DT>(x + 4);
+        if (dst) {
+          store8<DT>(dst, va);
+          store8<DT>(dst + ahead, vb);
+        }
+        if (also) {
+          store8<DT>(also, va);
+          store8<DT>(also + ahead, vb);
+        }
+      };
+      const T* q = reinterpret_cast<const T*>(rows) + ea;
+      T* qo = static_cast<T*>(a.q_out) + t * a.n_q_heads * D + ea;
+      int h = first;
+      for (; h < a.n_q_heads; h += share) turn_row(q + h * D, a.q_weight != nullptr, wq, qo + h * D, nullptr);
+      const int64_t at = a.k_cache ? slot_offset(p, a.slots[t]) : -1;
+      T* kc = at < 0 ? nullptr : static_cast<T*>(a.k_cache) + at + ea;
+      T* ko = a.k_out ? static_cast<T*>(a.k_out) + t * a.n_kv_heads * D + ea : nullptr;
+      for (; h < a.n_q_heads + a.n_kv_heads; h += share) {  // keys follow the queries
+        const int hk = h - a.n_q_heads;
+        turn_row(q + h * D, a.k_weight != nullptr, wk, kc ? kc + hk * a.c_stride_h : nullptr, ko ? ko + hk * D : nullptr);
+      }
+    }
+    // the stage is read (by the value copies too) before it is filled again
+    if (v_bytes && int(threadIdx.x) < p.per) asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+    fence_proxy_async_smem();
+    __syncthreads();
+    if (bars.dead) break;
+    const int64_t next = n + 2 * int64_t(gridDim.x);
+    if (threadIdx.x < 32 && next < batches) bring(next, s);
+  }
+  if (v_bytes && int(threadIdx.x) < p.per) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  if (threadIdx.x == 0 && bars.dead) atomicOr(&g_norm_rope_fault, 1u);
 }
 
 __global__ void __launch_bounds__(NR_THREADS) norm_rope_any_kernel(const __grid_constant__ NrParams p) {
@@ -303,8 +481,30 @@ __global__ void __launch_bounds__(NR_THREADS) norm_rope_any_kernel(const __grid_
   for (int e = R + lane; e < D; e += 32) put(e, normed(e));
 }
 
+// Tokens a batch of the staged kernel, 0 where it does not serve: heads side by side, and tokens enough for five rounds
+// of batches on every CTA.  At 32/8 heads of 128 with the cache write: 16384 tokens 88 us against the other kernel's
+// 101, 8192 (7 rounds) 49 / 54, 4096 (3.5 rounds) 31 / 31, 2000 21 / 16; at 12/4 heads of 64 8000 tokens (3.4 rounds) 22 / 17.
+int staged_tokens(const smaq_norm_rope_args& a, int size) {
+  const bool cache = a.k_cache != nullptr;
+  if (a.q_stride_h != a.head_dim || a.k_stride_h != a.head_dim || (cache && a.v_stride_h != a.head_dim)) return 0;
+  const int64_t token = int64_t(a.n_q_heads + a.n_kv_heads * (cache ? 2 : 1)) * a.head_dim * size + a.rotary_dim * 4;
+  const int64_t per = NS_SMEM / 2 / token;
+  int two = 0;
+  for (int i = 1; i <= per && i <= NS_MOST; i *= 2) two = i;  // the lane groups divide over the tokens
+  return two && a.n_tokens >= int64_t(num_sms()) * NS_CTAS * NS_ROUNDS * two ? two : 0;
+}
+
 template <class DT, int LANES>
-int launch_lanes(const NrParams& p, cudaStream_t st) {
+int launch_lanes(NrParams& p, cudaStream_t st) {
+  if (const int per = staged_tokens(p.a, int(sizeof(typename DT::T)))) {
+    p.per = per;
+    const int64_t token = int64_t(p.heads) * p.a.head_dim * sizeof(typename DT::T) + p.a.rotary_dim * 4, batches = (p.a.n_tokens + per - 1) / per;
+    auto kern = p.a.interleaved ? norm_rope_staged_kernel<DT, LANES, true> : norm_rope_staged_kernel<DT, LANES, false>;
+    if (const int rc = allow_smem(reinterpret_cast<const void*>(kern), NS_SMEM, "norm_rope")) return rc;
+    const int64_t most = int64_t(num_sms()) * NS_CTAS, grid = batches < most ? batches : most;
+    kern<<<unsigned(grid), NS_THREADS, size_t(2 * token * per), st>>>(p);
+    return cuda_status(cudaGetLastError(), "norm_rope");
+  }
   const int64_t jobs = p.a.n_tokens * p.groups, per_cta = NR_THREADS / LANES, grid = (jobs + per_cta - 1) / per_cta;
   if (grid >= (int64_t(1) << 31)) return fail(SMAQ_ERR_UNSUPPORTED, "norm_rope: too many rows");
   if (p.a.interleaved) norm_rope_kernel<DT, LANES, true><<<unsigned(grid), NR_THREADS, 0, st>>>(p);
@@ -381,3 +581,13 @@ extern "C" int smaq_norm_rope(const smaq_norm_rope_args* args, void* stream) {
     default: return launch_dtype<F16>(p, st);
   }
 }
+
+namespace smaq {
+int norm_rope_fault(bool& set) {
+  unsigned int word = 0, zero = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(&word, g_norm_rope_fault, sizeof(word));
+  if (e == cudaSuccess && word) e = cudaMemcpyToSymbol(g_norm_rope_fault, &zero, sizeof(zero));
+  set = word != 0;
+  return cuda_status(e, "exact status: read");
+}
+}  // namespace smaq

@@ -740,13 +740,19 @@ int launch_prefill_tc(const PagedParams& p, cudaStream_t st) {
 
 }  // namespace smaq
 
-extern "C" int smaq_prefill_status(void* stream) {
+namespace smaq {
+int norm_rope_fault(bool& set);  // norm_rope.cu
+}
+
+extern "C" int smaq_exact_status(void* stream) {
   cudaError_t e = cudaStreamSynchronize(static_cast<cudaStream_t>(stream));
-  if (e != cudaSuccess) return smaq::cuda_status(e, "prefill status: stream");
+  if (e != cudaSuccess) return smaq::cuda_status(e, "exact status: stream");
   unsigned int word = 0, zero = 0;
   e = cudaMemcpyFromSymbol(&word, smaq::g_prefill_fault, sizeof(word));
   if (e == cudaSuccess && word) e = cudaMemcpyToSymbol(smaq::g_prefill_fault, &zero, sizeof(zero));
-  if (e != cudaSuccess) return smaq::cuda_status(e, "prefill status: read");
-  if (word) return smaq::fail(SMAQ_ERR_DEVICE, "prefill: a bounded device wait of the tensor-core kernel ran out");
+  if (e != cudaSuccess) return smaq::cuda_status(e, "exact status: read");
+  bool rope = false;
+  if (const int st = smaq::norm_rope_fault(rope)) return st;
+  if (word || rope) return smaq::fail(SMAQ_ERR_DEVICE, "%s: a bounded device wait ran out", word ? "paged_prefill" : "norm_rope");
   return SMAQ_OK;
 }

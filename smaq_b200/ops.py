@@ -804,9 +804,10 @@ def append_status() -> None:
     _lib.check(_lib.load().smaq_append_status(_stream()), "smaq_append_status")
 
 
-def prefill_status() -> None:
-    """Raise if a bounded device wait of ``paged_prefill`` ran out since the last check (clears it)."""
-    _lib.check(_lib.load().smaq_prefill_status(_stream()), "smaq_prefill_status")
+def exact_status() -> None:
+    """Raise if a bounded device wait of ``paged_prefill`` or ``norm_rope`` ran out since the last check
+    (clears it).  Synchronises the current stream."""
+    _lib.check(_lib.load().smaq_exact_status(_stream()), "smaq_exact_status")
 
 
 def selftest_wait_timeout(spin_limit: int = 1 << 12) -> int:

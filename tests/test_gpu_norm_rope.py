@@ -44,6 +44,42 @@ def test_formula(cuda, dtype, interleaved, T, Hq, Hk, D, R, norm):
         near(got, *norm_rope_ref(x, w, 1e-5, pos, table, interleaved), D)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("T,Hq,Hk,D,R,norm,interleaved,cache", [
+    (11999, 6, 2, 128, 128, True, False, True), (12003, 4, 1, 64, 32, True, True, True), (11901, 2, 2, 256, 64, True, False, False),
+    (12500, 3, 1, 80, 48, False, True, False), (6201, 28, 4, 128, 128, False, False, True), (11877, 2, 1, 512, 512, True, True, True),
+    (1201, 4, 2, 128, 128, True, False, True)])
+def test_many_tokens(cuda, dtype, T, Hq, Hk, D, R, norm, interleaved, cache):
+    """Enough tokens for the staged kernel: several batches a block, a ragged last one, positions and slots outside."""
+    from smaq_b200 import ops
+    q, k, v, pos, table, (wq, wk) = case(cuda, T, Hq, Hk, D, R, dtype, norm, seed=7)
+    pos[5], pos[T - 1], pos[1000] = 500, -3, 2 ** 31 - 1
+    kw = dict(q_weight=wq, k_weight=wk, eps=1e-5, interleaved=interleaved)
+    if cache:
+        P = T // 16 + 2
+        kc, vc = torch.full((2, P, 16, Hk, D), 7.0, device=cuda, dtype=dtype).unbind(0)
+        slots = torch.randperm(P * 16, generator=torch.Generator().manual_seed(1))[:T].to(cuda)
+        slots[7], slots[T - 2] = -1, P * 16
+        qo, _ = ops.norm_rope(q, k, pos, table, v=v, k_cache=kc, v_cache=vc, slots=slots, **kw)
+        keep = (slots >= 0) & (slots < P * 16)
+        ko = kc.view(-1, Hk, D)[slots.clamp(0, P * 16 - 1)]
+        assert torch.equal(vc.view(-1, Hk, D)[slots[keep]], v[keep])
+        left = torch.ones(P * 16, dtype=torch.bool, device=cuda)
+        left[slots[keep]] = False
+        assert bool((kc.view(-1, Hk, D)[left] == 7).all()) and bool((vc.view(-1, Hk, D)[left] == 7).all())
+    else:
+        qo, ko = ops.norm_rope(q, k, pos, table, **kw)
+        keep = torch.ones(T, dtype=torch.bool, device=cuda)
+    ops.exact_status()
+    bad = (pos < 0) | (pos >= 500)
+    ok = ~bad
+    for got, x, w in ((qo, q, wq), (ko, k, wk)):
+        rows = ok & keep if got is ko else ok
+        near(got[rows], *norm_rope_ref(x[rows], w, 1e-5, pos[rows], table, interleaved), D)
+        rows = bad & keep if got is ko else bad
+        assert bool(torch.isnan(got[rows][..., :R]).all()) and not bool(torch.isnan(got[rows][..., R:]).any())
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("D,page", [(128, 16), (64, 24), (36, 5)])
 def test_cache_write(cuda, dtype, D, page):
