@@ -690,6 +690,19 @@ int launch(const PagedParams& p, cudaStream_t st) {
               : a.softcap > 0.f            ? prefill_tc_kernel<DT, D, PT_CAP>
                                            : prefill_tc_kernel<DT, D, PT_PLAIN>;
   if (const int rc = allow_smem(reinterpret_cast<const void*>(kern), PtCfg<D>::SMEM, "paged_prefill")) return rc;
+  if constexpr (PtCfg<D>::TILES == 2) {
+    // the warpgroups' shares after setmaxnreg are what the block is launched with: with fewer registers a thread than
+    // that it would wait for them for good
+    static const int regs = [] {
+      int least = 255;
+      for (auto k : {prefill_tc_kernel<DT, D, PT_PLAIN>, prefill_tc_kernel<DT, D, PT_CAP>, prefill_tc_kernel<DT, D, PT_ANY>}) {
+        cudaFuncAttributes f;
+        least = std::min(least, cudaFuncGetAttributes(&f, k) == cudaSuccess ? f.numRegs : 0);
+      }
+      return least;
+    }();
+    if (regs * pt_threads(D) < 128 * 64 + 512 * 104) return fail(SMAQ_ERR_UNSUPPORTED, "paged_prefill: built with %d registers a thread", regs);
+  }
   const int64_t units = grid_tiles(a.n_rows, a.batch, p.group, D) * a.n_kv_heads;
   pt.splits = splits_for(units, int64_t(a.max_blocks) * a.page_size);
   pt.parts = static_cast<float*>(a.workspace);
