@@ -1,4 +1,4 @@
-// Prefill attention on the 5th-generation tensor cores (bf16 / fp16, head_dim 64 and 128).
+// Prefill attention on the 5th-generation tensor cores (bf16 / fp16, head_dim 64, 128 and 256).
 //
 // A CTA holds 256 rows (tokens times grouped heads, paged_prefill.cuh) as two tiles of 128 and walks blocks of 128
 // tokens.  For each tile and block S = Q K^T goes to tensor memory, a warpgroup turns it into weights P there, and
@@ -6,17 +6,22 @@
 // the other.
 //   warps 0-7, 8-15  softmax of tile 0, 1: a thread has one half of a row's scores and goes over them twice, 32 columns at a time
 //                    (maximum, weights); the halves' maxima meet in shared memory.  (One thread a row with its 128 scores in
-//                    registers has half the warps to hide latencies with: 541 us against 539 at 8192 tokens, 728 against 712
-//                    capped.)
-//   warps 16-18      copies: queries once, then keys and values, whole blocks by TMA in boxes of a page, the blocks with tokens
-//                    that no row sees, and page sizes that do not fit the block, by cp.async of 16 bytes (such tokens are written
-//                    as zeros), both in the 128-byte swizzled operand layout;
+//                    registers has half the warps to hide latencies with: measured together, 541 us against 539 at 8192
+//                    tokens, 728 against 712 capped.)
+//   warps 16-18      copies of keys and values, by TMA in boxes of a page (where a block has tokens that no row sees, the values'
+//                    rows are cleared), or by cp.async of 16 bytes for page sizes that do not tile a block (such tokens are
+//                    written as zeros), both in the 128-byte swizzled operand layout; the softmax threads load the queries;
 //   warp 19          issues all products.
 // Tensor memory: S0 S1 (128 columns each), O0 O1 (head_dim each); P overwrites its S.  The product for the next S of a tile is
 // issued right behind the product that reads its P, and its completion also says that O is at rest: a softmax warp may
 // then rescale O, which it does only when a row's maximum grew by more than 2^8 (the reference maximum of a row
 // lags by at most that, so weights stay below 2^8 in either type).
+// At head_dim 256 there is room for one tile (128 rows, half the softmax warps): S0 and S1 are then blocks of even and odd
+// number, the next block's scores are computed during this block's softmax, and O is waited for by itself.
 // Weights are rounded once, to the cache's type; the sums are of the unrounded ones.
+// Few rows with long walks: several CTAs share a tile's walk and prefill_join_kernel adds their parts in order.
+// Bound by both the products and the exponentials (2048 cycles a block each, of about 3300 in all): 8192 tokens at 32/8
+// heads of 128 in 514 us, 1070 TFLOP/s, 64% of what a library product reaches in short runs.
 // Every wait is bounded; one that runs out sets g_prefill_fault and the CTA drains.
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -87,10 +92,10 @@ __device__ __forceinline__ void named_bar(int id, int threads) { asm volatile("b
 
 enum { PT_PLAIN = 0, PT_CAP = 1, PT_ANY = 2 };  // scores: scaled by a positive factor; capped; everything else
 // Of every PT_OF pairs of exponentials so many come from the polynomial, the others from the special-function unit,
-// which alone would need as long as the products.  At 8192 tokens and 32/8 heads 0, 1, 2, 3 of 8 took 578, 539, 557,
-// 558 us; a capped score takes two exponentials and a reciprocal: (4, 2), (2, 2), (6, 2), (4, 4) of 8 for (tanh, weight)
-// took 712, 725, 726, 735 us on chunks of 64/8 heads behind 8K tokens.
-constexpr int PT_POLY = 1, PT_POLY_CAP = 4, PT_POLY_EXP = 2;
+// which alone would need as long as the products.  At 8192 tokens and 32/8 heads 0, 1, 2, 3 of 8 took 515, 514, 533,
+// 548 us; a capped score takes two exponentials and a reciprocal: (4, 2), (5, 2), (5, 3), (4, 1), (6, 3) of 8 for (tanh,
+// weight) took 673, 666, 676, 684, 689 us on chunks of 64/8 heads behind 8K tokens.
+constexpr int PT_POLY = 1, PT_POLY_CAP = 5, PT_POLY_EXP = 2;
 constexpr int PT_OF = 8;
 
 // 2^x of PT_OF pairs, POLY of them by the polynomial.

@@ -127,6 +127,11 @@ def test_prefill_padding_rows_and_many_requests(cuda, dtype):
     prefill(cuda, [(i * 5) % 9 for i in range(200)], [(i * 11) % 30 for i in range(200)], 4, 2, 64, 16, dtype, pad=37)
 
 
+@pytest.mark.parametrize("dtype", [BF, SF])
+def test_prefill_more_requests_than_threads(cuda, dtype):
+    prefill(cuda, [(i * 5) % 4 for i in range(1500)], [(i * 11) % 20 for i in range(1500)], 2, 1, 64, 16, dtype, pad=5)
+
+
 @pytest.mark.parametrize("dtype", [BF, HF, SF])
 def test_prefill_infinities_reach_only_rows_that_see_them(cuda, dtype):
     """A later token's infinite or NaN value or key in the same block leaves the rows before it as they are."""
