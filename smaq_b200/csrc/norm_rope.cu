@@ -271,8 +271,8 @@ __global__ void __launch_bounds__(NR_THREADS, NR_CTAS) norm_rope_kernel(const __
 // flight do not cost registers; a lane group then takes head after head of one token from there (8192 tokens at 32/8 heads:
 // 49 us, 4.2 TB/s; an elementwise pass over as many bytes takes 33).  Values go from shared memory
 // to the cache by bulk copies too.  For heads that lie side by side in a token.
-constexpr int NS_THREADS = 256, NS_CTAS = 2, NS_SMEM = 112 * 1024, NS_MOST = 8;
-constexpr int NS_ROUNDS = 5;
+constexpr int NS_THREADS = 256, NS_CTAS = 2, NS_SMEM = 112 * 1024, NS_MOST = 16;
+constexpr int NS_ROUNDS = 3;
 constexpr uint32_t NS_SPIN = 1u << 24;
 
 __device__ unsigned int g_norm_rope_fault;
@@ -481,22 +481,23 @@ __global__ void __launch_bounds__(NR_THREADS) norm_rope_any_kernel(const __grid_
   for (int e = R + lane; e < D; e += 32) put(e, normed(e));
 }
 
-// Tokens a batch of the staged kernel, 0 where it does not serve: heads side by side, and tokens enough for five rounds
-// of batches on every CTA.  At 32/8 heads of 128 with the cache write: 16384 tokens 88 us against the other kernel's
-// 101, 8192 (7 rounds) 49 / 54, 4096 (3.5 rounds) 31 / 31, 2000 21 / 16; at 12/4 heads of 64 8000 tokens (3.4 rounds) 22 / 17.
-int staged_tokens(const smaq_norm_rope_args& a, int size) {
+// Tokens a batch of the staged kernel, 0 where it does not serve: heads side by side, batches of 40 KB or more, and tokens
+// enough for three rounds of batches on every CTA.  Against the other kernel, with the cache write: 32/8 heads of 128,
+// 16384 tokens 88 us / 101, 8192 (7 rounds) 49 / 54, 4096 (3.5) 31 / 30, 2000 (1.7) 16.5 / 15.8; 32/8 of 256, 4000
+// tokens 47 / 53; 12/4 of 64, 16000 tokens 30 / 33; 8/1 of 64, 16000 tokens in batches of 25 KB 26 / 21.
+int staged_tokens(const smaq_norm_rope_args& a, int size, int groups) {
   const bool cache = a.k_cache != nullptr;
   if (a.q_stride_h != a.head_dim || a.k_stride_h != a.head_dim || (cache && a.v_stride_h != a.head_dim)) return 0;
   const int64_t token = int64_t(a.n_q_heads + a.n_kv_heads * (cache ? 2 : 1)) * a.head_dim * size + a.rotary_dim * 4;
   const int64_t per = NS_SMEM / 2 / token;
   int two = 0;
-  for (int i = 1; i <= per && i <= NS_MOST; i *= 2) two = i;  // the lane groups divide over the tokens
-  return two && a.n_tokens >= int64_t(num_sms()) * NS_CTAS * NS_ROUNDS * two ? two : 0;
+  for (int i = 1; i <= per && i <= NS_MOST && i <= groups; i *= 2) two = i;  // the lane groups divide over the tokens
+  return two * token >= 40 * 1024 && a.n_tokens >= int64_t(num_sms()) * NS_CTAS * NS_ROUNDS * two ? two : 0;
 }
 
 template <class DT, int LANES>
 int launch_lanes(NrParams& p, cudaStream_t st) {
-  if (const int per = staged_tokens(p.a, int(sizeof(typename DT::T)))) {
+  if (const int per = staged_tokens(p.a, int(sizeof(typename DT::T)), NS_THREADS / LANES)) {
     p.per = per;
     const int64_t token = int64_t(p.heads) * p.a.head_dim * sizeof(typename DT::T) + p.a.rotary_dim * 4, batches = (p.a.n_tokens + per - 1) / per;
     auto kern = p.a.interleaved ? norm_rope_staged_kernel<DT, LANES, true> : norm_rope_staged_kernel<DT, LANES, false>;

@@ -1076,6 +1076,8 @@ extern "C" int smaq_paged_decode(const smaq_paged_args* args, void* stream) {
                           : (sh.tile == 4 ? launch_f32<128, 4>(d, st) : launch_f32<128, 8>(d, st));
   else rc = a.dtype == SMAQ_F32 ? launch_simt<F32>(d, st) : a.dtype == SMAQ_BF16 ? launch_simt<BF16>(d, st) : launch_simt<F16>(d, st);
   if (rc) return rc;
+  // tables or windows of one unit: no segment can have been split
+  if (int64_t(a.max_blocks) * a.page_size <= PD_UNIT || (a.window > 0 && a.window <= PD_UNIT)) return SMAQ_OK;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(unsigned(a.batch) * unsigned(a.n_q_heads));
   cfg.blockDim = dim3(PD_THREADS);

@@ -539,22 +539,22 @@ def step_tables(free_blocks: torch.Tensor, free_count: torch.Tensor, context_len
             raise ValueError(f"finished must be a bool vector of length {B}")
         if not finished.is_contiguous():
             finished = finished.contiguous()
-    # one buffer: slots (8 bytes) first, positions on a 16-byte boundary, the rest
+    # two buffers and the flags; the small vectors lie behind the positions
     M, T = width[1], num_tokens
-    pad = (T + 3) // 4 * 4
-    buf = free_blocks.new_empty(3 * pad + 2 * B + 2)
-    slots, _, positions, _, cu, lens, left = buf.split_with_sizes([2 * T, 2 * (pad - T), T, pad - T, B + 1, B, 1])
-    admitted = torch.empty(B, dtype=torch.bool, device=free_blocks.device)
+    slots = free_blocks.new_empty(T, dtype=torch.int64)
+    buf = free_blocks.new_empty(T + 2 * B + 2)
+    positions, cu, lens, left = buf.split_with_sizes([T, B + 1, B, 1])
+    admitted = free_blocks.new_empty(B, dtype=torch.bool)
     at = buf.data_ptr()
-    rest = at + 12 * pad
+    rest = at + 4 * T
     st = _lib.load().smaq_step_tables(
         _lib.pack_tables(free_blocks.data_ptr(), free_count.data_ptr(), context_lens.data_ptr(), query_lens.data_ptr(),
                          _addr(finished), block_table.data_ptr(), max(block_table.stride(0), M), free_blocks.shape[0], T,
-                         B, M, block_size, rest, rest + 4 * (B + 1), at + 8 * pad, at, admitted.data_ptr(),
+                         B, M, block_size, rest, rest + 4 * (B + 1), at, slots.data_ptr(), admitted.data_ptr(),
                          rest + 4 * (2 * B + 1)), stream)
     if st:
         _lib.check(st, "smaq_step_tables")
-    return StepTables(cu, lens, positions, slots.view(torch.int64), left, admitted)
+    return StepTables(cu, lens, positions, slots, left, admitted)
 
 
 def rope_table(max_positions: int, rotary_dim: int, base: float = 10000.0, *, linear: float = 1.0,
@@ -742,7 +742,7 @@ def _paged(name, q, k_cache, v_cache, block_table, seq_lens, cu_query, prefix_le
         call, need = lib.smaq_paged_prefill, lib.smaq_paged_prefill_workspace_size(T, B, Hq, Hk, D,
                                                                                      M * page_size)
     if workspace is None and need:
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device)
+        workspace = q.new_empty(need, dtype=torch.uint8)
     if workspace is not None:
         ws, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
     st = call(
