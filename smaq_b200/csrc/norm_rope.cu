@@ -481,7 +481,7 @@ __global__ void __launch_bounds__(NR_THREADS) norm_rope_any_kernel(const __grid_
   for (int e = R + lane; e < D; e += 32) put(e, normed(e));
 }
 
-// Tokens a batch of the staged kernel, 0 where it does not serve: heads side by side, batches of 40 KB or more, and tokens
+// Tokens a batch of the staged kernel, 0 where it does not serve: heads side by side, batches of 32 KB or more, and tokens
 // enough for three rounds of batches on every CTA.  Against the other kernel, with the cache write: 32/8 heads of 128,
 // 16384 tokens 88 us / 101, 8192 (7 rounds) 49 / 54, 4096 (3.5) 31 / 30, 2000 (1.7) 16.5 / 15.8; 32/8 of 256, 4000
 // tokens 47 / 53; 12/4 of 64, 16000 tokens 30 / 33; 8/1 of 64, 16000 tokens in batches of 25 KB 26 / 21.
@@ -492,7 +492,7 @@ int staged_tokens(const smaq_norm_rope_args& a, int size, int groups) {
   const int64_t per = NS_SMEM / 2 / token;
   int two = 0;
   for (int i = 1; i <= per && i <= NS_MOST && i <= groups; i *= 2) two = i;  // the lane groups divide over the tokens
-  return two * token >= 40 * 1024 && a.n_tokens >= int64_t(num_sms()) * NS_CTAS * NS_ROUNDS * two ? two : 0;
+  return two * token >= 32 * 1024 && a.n_tokens >= int64_t(num_sms()) * NS_CTAS * NS_ROUNDS * two ? two : 0;
 }
 
 template <class DT, int LANES>

@@ -48,7 +48,8 @@ def test_formula(cuda, dtype, interleaved, T, Hq, Hk, D, R, norm):
 @pytest.mark.parametrize("T,Hq,Hk,D,R,norm,interleaved,cache", [
     (11999, 6, 2, 128, 128, True, False, True), (12003, 4, 1, 64, 32, True, True, True), (11901, 2, 2, 256, 64, True, False, False),
     (12500, 3, 1, 80, 48, False, True, False), (6201, 28, 4, 128, 128, False, False, True), (11877, 2, 1, 512, 512, True, True, True),
-    (1201, 4, 2, 128, 128, True, False, True)])
+    (1201, 4, 2, 128, 128, True, False, True), (14300, 6, 2, 128, 128, True, False, True), (14301, 2, 2, 256, 64, True, False, False),
+    (3700, 28, 4, 128, 128, False, True, True), (7203, 24, 6, 64, 32, True, True, True), (7105, 12, 4, 80, 48, True, True, False)])
 def test_many_tokens(cuda, dtype, T, Hq, Hk, D, R, norm, interleaved, cache):
     """Enough tokens for the staged kernel: several batches a block, a ragged last one, positions and slots outside."""
     from smaq_b200 import ops
