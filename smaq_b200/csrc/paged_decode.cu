@@ -18,10 +18,12 @@
 // before its copies.  Scores by m16n8k16 (rows = query heads of the group, zero rows above it); weights enter
 // the second product as hi + lo parts in the cache's type, which costs tensor time that is idle here and
 // keeps 16-bit rounding out of the weights.  Slots past the visible range are filled with zeros by the copy and
-// their scores replaced, so what they hold never matters.
+// their scores replaced, so what they hold never matters.  64 requests of 1K to 64K tokens at 28/4 heads of 128:
+// 323 us, 6.3 TB/s; 4 of 128K at 64/8: 357 us, 6.0 TB/s (both of 6.45 for a plain copy).
 //
 // paged_decode_f32_kernel (fp32, head_dim 64 / 128): the same rings; FMA throughout, since tf32 products in three parts
-// left 2e-6 in the scores (rounding inside the tensor cores' sums).
+// left 2e-6 in the scores (rounding inside the tensor cores' sums).  33 requests of 100 to 32K tokens, window 4096,
+// 12/4 heads of 64: 47 us, of which start and join are 12.
 // paged_simt_kernel (other head dims and alignments): 16 groups of eight lanes, one token a group, four query
 // rows a tile.
 #include "paged.cuh"

@@ -9,8 +9,8 @@
 // prefill_tc.cu (bf16 / fp16, head_dim 64 / 128 / 256): the tensor-core kernel, everything but tables of one block.
 // prefill_mma_kernel (the same types and head dims, tables of up to 128 tokens): four warps of 16 rows, m16n8k16 products, blocks of
 //   64 (head_dim 256: 32) tokens brought by cp.async into two stages, page lookups two blocks ahead.
-// prefill_simt_kernel (fp32, other head dims and alignments): tiles of four rows, 16 lane groups with a token
-//   each; all arithmetic in 32 bits.
+// prefill_fma_kernel, prefill_simt_kernel (fp32, other head dims and alignments): tiles of 64 rows by 64 tokens, or,
+//   with few rows, of four rows and 16 lane groups with a token each; all arithmetic in 32 bits.
 #include "paged_prefill.cuh"
 #include "prefill_tc.cuh"
 
@@ -343,6 +343,173 @@ __global__ void __launch_bounds__(PM_THREADS) prefill_simt_kernel(const __grid_c
   }
 }
 
+// ---------------------------------------------------------------- many rows in 32 bits
+// Tiles of 64 rows by blocks of 64 tokens in shared memory as 32-bit values, both products by FMA: a thread has 4 x 4
+// scores, then 4 rows by DP / 16 channels (DP: head_dim rounded up to 64).  2048 fp32 tokens at 32/8 heads of 128:
+// 1537 us, 22 TFLOP/s (four-row tiles: 3950 us), bound by the reads of shared memory: two float4 for 16 FMAs a thread.
+// Every product, weight and sum is fp32: tensor-core products would round the operands.
+constexpr int PF_THREADS = 256, PF_ROWS = 64, PF_N = 64, PF_LD = 68;  // PF_LD: 64 and a pad that keeps float4 aligned
+
+template <int DP>
+constexpr int pf_smem() { return (2 * DP * PF_LD + PF_N * DP + PF_N * PF_LD) * 4; }
+
+template <class DT, int DP, bool VEC>
+__global__ void __launch_bounds__(PF_THREADS, DP <= 128 ? 2 : 1) prefill_fma_kernel(const __grid_constant__ PagedParams p) {
+  using T = typename DT::T;
+  constexpr int NI = DP / 64;
+  extern __shared__ __align__(16) float sm[];
+  float *qs = sm, *ks = qs + DP * PF_LD, *vs = ks + DP * PF_LD, *ps = vs + PF_N * DP;
+  __shared__ int sums[PF_THREADS / 32];
+  __shared__ PrefillTile found;
+  const smaq_paged_args& a = p.a;
+  const int D = a.head_dim, tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, kvh = blockIdx.y;
+  write_padding(p, kvh, blockIdx.x, gridDim.x);
+  const PrefillTile t = find_tile<PF_THREADS>(p, blockIdx.x, PF_ROWS, true, sums, &found);
+  if (t.rows == 0) return;
+  const PrefillBlocks blocks(t, PF_N);
+  const int32_t* table = a.block_table + t.b * a.table_stride;
+  auto load4 = [&](const T* row, int e, float (&x)[4]) {  // elements e .. e + 3 of a row, zeros past its end
+    if constexpr (VEC) {
+      if (e < D) load_vec<DT, 4>(row + e, x);
+      else x[0] = x[1] = x[2] = x[3] = 0.f;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = e + i < D ? to_f(row[e + i]) : 0.f;
+    }
+  };
+  const int last = t.f0 + t.rows, least = t.past + fast_div(t.f0, p.group_div), most = t.past + fast_div(last - 1, p.group_div);
+  {
+    const int r = tid & 63, f = t.f0 + r, tok = fast_div(f, p.group_div);
+    const T* src = static_cast<const T*>(a.q) + (f < last ? int64_t(t.first + tok) * a.q_stride_t + (kvh * p.group + f - tok * p.group) * a.q_stride_h : 0);
+    for (int e = (tid >> 6) * 4; e < DP; e += 16) {
+      float x[4] = {};
+      if (f < last) load4(src, e, x);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) qs[(e + i) * PF_LD + r] = x[i];
+    }
+  }
+  int pos[4], head[4];
+  float slope[4], m[4], l[4], o[4][NI * 4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int f = t.f0 + ty * 4 + r, tok = fast_div(f, p.group_div);
+    pos[r] = t.past + tok;
+    head[r] = kvh * p.group + f - tok * p.group;
+    slope[r] = a.slopes && f < last ? a.slopes[head[r]] : 0.f;
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+#pragma unroll
+    for (int c = 0; c < NI * 4; ++c) o[r][c] = 0.f;
+  }
+  bool special = false;
+  for (int b = 0; b < blocks.count; ++b) {
+    const int base = blocks.base(b, PF_N);
+    const bool all = base + PF_N <= t.prefix || (base + PF_N <= least + 1 && (a.window == 0 || base > most - a.window));
+    __syncthreads();  // the block before is read
+    {  // keys: a token a lane, transposed
+      const int r = tid & 63, j = base + r;
+      const bool seen = tile_sees(t, j);
+      const T* row = static_cast<const T*>(a.k_cache) + (seen ? token_offset(p, table, j) + kvh * a.c_stride_h : 0);
+      for (int e = (tid >> 6) * 4; e < DP; e += 16) {
+        float x[4] = {};
+        if (seen) load4(row, e, x);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ks[(e + i) * PF_LD + r] = x[i];
+      }
+    }
+    for (int i = tid; i < PF_N * (DP / 4); i += PF_THREADS) {
+      const int r = i / (DP / 4), e = i % (DP / 4) * 4, j = base + r;
+      float x[4] = {};
+      if (tile_sees(t, j)) load4(static_cast<const T*>(a.v_cache) + token_offset(p, table, j) + kvh * a.c_stride_h, e, x);
+      if (!all) special |= !(fabsf(x[0]) + fabsf(x[1]) + fabsf(x[2]) + fabsf(x[3]) < INFINITY);
+      *reinterpret_cast<float4*>(vs + r * DP + e) = make_float4(x[0], x[1], x[2], x[3]);
+    }
+    __syncthreads();
+    float s[4][4] = {};
+#pragma unroll 8
+    for (int e = 0; e < DP; ++e) {
+      const float4 q = *reinterpret_cast<const float4*>(qs + e * PF_LD + ty * 4), k = *reinterpret_cast<const float4*>(ks + e * PF_LD + tx * 4);
+      const float qv[4] = {q.x, q.y, q.z, q.w}, kv[4] = {k.x, k.y, k.z, k.w};
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) s[r][c] = fmaf(qv[r], kv[c], s[r][c]);
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int j = base + tx * 4 + c;
+        float x = s[r][c] * a.scale;
+        if (a.softcap > 0.f) x = a.softcap * tanhf(x / a.softcap);
+        if (a.slopes) x -= slope[r] * fabsf(float(pos[r] - j));
+        x *= kLog2e;
+        s[r][c] = all || (j < t.len && row_sees(p, t, pos[r], j)) ? x : -INFINITY;
+        mx = fmaxf(mx, s[r][c]);
+      }
+#pragma unroll
+      for (int w = 1; w < 16; w <<= 1) mx = fmaxf(mx, __shfl_xor_sync(~0u, mx, w));
+      if (mx > m[r]) {  // alike for the sixteen threads of a row
+        const float f = ex2(m[r] - mx);
+        m[r] = mx;
+        l[r] *= f;
+#pragma unroll
+        for (int c = 0; c < NI * 4; ++c) o[r][c] *= f;
+      }
+      const float z = m[r] == -INFINITY ? 0.f : m[r];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        s[r][c] = ex2(s[r][c] - z);
+        l[r] += s[r][c];
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) *reinterpret_cast<float4*>(ps + (tx * 4 + c) * PF_LD + ty * 4) = make_float4(s[0][c], s[1][c], s[2][c], s[3][c]);
+    __syncthreads();
+#pragma unroll 4
+    for (int j = 0; j < PF_N; ++j) {
+      const float4 w = *reinterpret_cast<const float4*>(ps + j * PF_LD + ty * 4);
+      const float wv[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int i = 0; i < NI; ++i) {
+        const float4 v = *reinterpret_cast<const float4*>(vs + j * DP + tx * 4 + 64 * i);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          o[r][4 * i] = fmaf(wv[r], v.x, o[r][4 * i]);
+          o[r][4 * i + 1] = fmaf(wv[r], v.y, o[r][4 * i + 1]);
+          o[r][4 * i + 2] = fmaf(wv[r], v.z, o[r][4 * i + 2]);
+          o[r][4 * i + 3] = fmaf(wv[r], v.w, o[r][4 * i + 3]);
+        }
+      }
+    }
+  }
+  uint32_t redo = 0;  // of this warp's eight rows: 4 (ty & 1) + r
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+#pragma unroll
+    for (int w = 1; w < 16; w <<= 1) l[r] += __shfl_xor_sync(~0u, l[r], w);
+    const int f = t.f0 + ty * 4 + r, tok = fast_div(f, p.group_div);
+    const int64_t at = int64_t(t.first + tok) * a.o_stride_t + head[r] * a.o_stride_h;
+    float odd = 0.f;
+#pragma unroll
+    for (int c = 0; c < NI * 4; ++c) {
+      const float x = l[r] == 0.f ? 0.f : o[r][c] / l[r];
+      const int e = tx * 4 + 64 * (c / 4) + c % 4;
+      odd += x * 0.f;
+      if (f < last && e < D) store_elem(a.out, a.dtype, at + e, x);
+    }
+    if (a.lse && tx == 0 && f < last) a.lse[int64_t(t.first + tok) * a.n_q_heads + head[r]] = (m[r] + log2f(l[r])) * kLn2;
+    const uint32_t bad = __ballot_sync(~0u, odd != 0.f && l[r] == l[r] && f < last);
+    redo |= (bad & 0xFFFFu ? 1u : 0u) << r | (bad >> 16 ? 1u : 0u) << (4 + r);
+  }
+  if (__syncthreads_or(special)) {
+    const int first = t.f0 + (tid >> 5) * 8;  // the warp's rows
+    for (int r = 0; r < 8; ++r)
+      if (redo >> r & 1) exact_row(p, t, kvh, first + r);
+  }
+}
+
 // At least one CTA a KV head, for the rows past the last request's.
 int64_t grid_tiles(const PagedParams& p, int size) {
   const int64_t n = most_tiles(p.a.n_rows, p.a.batch, p.group, size);
@@ -364,10 +531,25 @@ int launch_mma_dim(const PagedParams& p, cudaStream_t st) {
     default: return launch_mma<DT, 256>(p, st);
   }
 }
+template <class DT, int DP, bool VEC>
+int launch_fma(const PagedParams& p, cudaStream_t st) {
+  if (const int rc = allow_smem(reinterpret_cast<const void*>(prefill_fma_kernel<DT, DP, VEC>), pf_smem<DP>(), "paged_prefill")) return rc;
+  prefill_fma_kernel<DT, DP, VEC><<<dim3(unsigned(grid_tiles(p, PF_ROWS)), p.a.n_kv_heads), PF_THREADS, pf_smem<DP>(), st>>>(p);
+  return cuda_status(cudaGetLastError(), "paged_prefill");
+}
+// Tiles of 64 rows from 24 rows a request on (tokens times grouped heads) and 16 rows an SM over all KV heads, tiles of
+// four below: they are 16 times as many CTAs, and a CTA is twice as quick.  fp32, 32/8 heads of 128, tiles of 64 / of
+// four: 16 requests of 1000 tokens and 2, 4, 8, 16 new ones 264, 264, 265, 268 / 135, 251, 366, 602 us; one of 2000
+// tokens and 32, 64, 96, 128 new ones 404, 417, 418, 429 / 199, 418, 430, 633 us.
 template <class DT>
 int launch_simt(const PagedParams& p, cudaStream_t st) {
   const int D = p.a.head_dim;
   const bool vec = D % 4 == 0 && paged_aligned(p.a);
+  if (p.a.n_rows * p.group >= 24 * int64_t(p.a.batch) && p.a.n_rows * p.a.n_q_heads >= 16 * int64_t(num_sms())) {
+    if (D <= 64) return vec ? launch_fma<DT, 64, true>(p, st) : launch_fma<DT, 64, false>(p, st);
+    if (D <= 128) return vec ? launch_fma<DT, 128, true>(p, st) : launch_fma<DT, 128, false>(p, st);
+    return vec ? launch_fma<DT, 256, true>(p, st) : launch_fma<DT, 256, false>(p, st);
+  }
   auto go = [&](auto kern) {
     kern<<<dim3(unsigned(grid_tiles(p, PX_ROWS)), p.a.n_kv_heads), PM_THREADS, 0, st>>>(p);
     return cuda_status(cudaGetLastError(), "paged_prefill");

@@ -66,7 +66,7 @@ struct PtCfg {
 
 struct PtParams {
   PagedParams p;
-  int tma;         // keys and values come through the tensor maps where every token of a block is seen
+  int tma;         // keys and values come through the tensor maps where a block's pages allow it
   int box;         // slots a box: page_size, at most PT_N
   int splits;      // CTAs that share a tile's walk, at most
   float* parts;    // [tile][KV head][split]: accumulators [rows][D], maxima, sums, whether a special value was met

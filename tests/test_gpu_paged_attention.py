@@ -198,6 +198,37 @@ def test_not_admitted_and_broken_tables_stay_inside(cuda):
     assert bool(torch.isfinite(ops.paged_prefill(q, k, v, table, i32([64, 64]), i32([-3, 10, 10 ** 6]))).all())
 
 
+@pytest.mark.parametrize("dtype,D", [(SF, 64), (SF, 128), (SF, 256), (SF, 96), (SF, 33), (BF, 96), (HF, 36), (BF, 201)])
+@pytest.mark.parametrize("news,ctx,Hq,Hkv,page,kw", [
+    ([260, 0, 90], [140, 300, 0], 8, 2, 16, {}), ([1, 700], [90, 0], 7, 1, 24, dict(window=70, slopes=True)),
+    ([333], [500], 12, 12, 7, dict(window=33, prefix=[257], softcap=20.0)), ([100], [63], 28, 4, 64, dict(window=1, pad=70))])
+def test_prefill_many_rows_in_32_bits(cuda, dtype, D, news, ctx, Hq, Hkv, page, kw):
+    """fp32 and the head dims that the tensor cores do not take, with rows enough for tiles of 64."""
+    prefill(cuda, news, ctx, Hq, Hkv, D, page, dtype, **kw)
+
+
+@pytest.mark.parametrize("dtype,D", [(SF, 128), (SF, 256), (BF, 96), (SF, 33)])
+def test_prefill_many_rows_infinities(cuda, dtype, D):
+    from smaq_b200 import ops
+    k, v, table = paged_case(cuda, [400, 90], 2, D, 16, dtype)
+    q = queries(cuda, 470, 8, D, dtype)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    args = (table, i32([400, 90]), i32([0, 380, 470]))
+    a = ops.paged_prefill(q, k, v, *args)
+    v[table[0, 6].long(), 3, 0, 7] = math.inf       # token 99 of request 0: rows from 79 on, head 0 of the cache
+    v[table[0, 20].long(), 0, 1, 1] = math.nan      # token 320: rows from 300 on, head 1
+    k[table[1, 1].long(), 0, 1] = math.nan          # token 16 of request 1: rows from 396 on are NaN, head 1
+    b = ops.paged_prefill(q, k, v, *args)
+    good = torch.ones_like(b, dtype=torch.bool)
+    good[79:380, :4, 7] = False
+    good[300:380, 4:, 1] = False
+    good[396:, 4:] = False
+    assert bool((b[79:380, :4, 7] == math.inf).all()) and bool(torch.isnan(b[300:380, 4:, 1]).all()) and bool(torch.isnan(b[396:, 4:]).all())
+    assert bool(torch.isfinite(b[good]).all())
+    tol = 4 * UNIT[dtype] if dtype != SF else 1e-5
+    assert float((b.float() - a.float())[good].abs().max()) <= tol * float(a.float().abs().max())
+
+
 @pytest.mark.parametrize("dtype", [BF, SF])
 def test_strides_streams_workspace(cuda, dtype):
     """Queries and outputs as views of wider buffers, caches as the halves of one buffer, another stream, a kept workspace."""
