@@ -346,19 +346,22 @@ __global__ void __launch_bounds__(PM_THREADS) prefill_simt_kernel(const __grid_c
 // ---------------------------------------------------------------- many rows in 32 bits
 // Tiles of 64 rows by blocks of 64 tokens in shared memory as 32-bit values, both products by FMA: a thread has 4 x 4
 // scores, then 4 rows by DP / 16 channels (DP: head_dim rounded up to 64).  2048 fp32 tokens at 32/8 heads of 128:
-// 1537 us, 22 TFLOP/s (four-row tiles: 3950 us), bound by the reads of shared memory: two float4 for 16 FMAs a thread.
+// 1279 us, 27 TFLOP/s (four-row tiles: 3950 us), bound by the reads of shared memory (two float4 for 16 FMAs a thread)
+// and the loads between the products; eight rows a thread, with half the warps, take 1290 us.
 // Every product, weight and sum is fp32: tensor-core products would round the operands.
-constexpr int PF_THREADS = 256, PF_ROWS = 64, PF_N = 64, PF_LD = 68;  // PF_LD: 64 and a pad that keeps float4 aligned
+constexpr int64_t NO_SLOT = INT64_MIN;  // a token that no row sees
+constexpr int PF_THREADS = 256, PF_STEP = PF_THREADS / 16, PF_ROWS = 64, PF_N = 64, PF_LD = 68;  // PF_LD: 64 and a pad that keeps float4 aligned
 
 template <int DP>
-constexpr int pf_smem() { return (2 * DP * PF_LD + PF_N * DP + PF_N * PF_LD) * 4; }
+constexpr int pf_smem() { return (2 * DP * PF_LD + PF_N * DP + (DP > 128 ? PF_N * PF_LD : 0)) * 4; }
 
 template <class DT, int DP, bool VEC>
 __global__ void __launch_bounds__(PF_THREADS, DP <= 128 ? 2 : 1) prefill_fma_kernel(const __grid_constant__ PagedParams p) {
   using T = typename DT::T;
-  constexpr int NI = DP / 64;
+  constexpr int NI = DP / 64, U = 8;  // U: loads in flight a thread
   extern __shared__ __align__(16) float sm[];
-  float *qs = sm, *ks = qs + DP * PF_LD, *vs = ks + DP * PF_LD, *ps = vs + PF_N * DP;
+  __shared__ int64_t offs[2][PF_N];
+  float *qs = sm, *ks = qs + DP * PF_LD, *vs = ks + DP * PF_LD, *ps = DP > 128 ? vs + PF_N * DP : ks;  // up to 128 the weights take the keys' place: two CTAs an SM
   __shared__ int sums[PF_THREADS / 32];
   __shared__ PrefillTile found;
   const smaq_paged_args& a = p.a;
@@ -377,11 +380,18 @@ __global__ void __launch_bounds__(PF_THREADS, DP <= 128 ? 2 : 1) prefill_fma_ker
       for (int i = 0; i < 4; ++i) x[i] = e + i < D ? to_f(row[e + i]) : 0.f;
     }
   };
+  auto find_slots = [&](int b) {  // where a block's tokens lie
+    if (tid < PF_N) {
+      const int j = blocks.base(b, PF_N) + tid;
+      offs[b & 1][tid] = tile_sees(t, j) ? token_offset(p, table, j) + kvh * a.c_stride_h : NO_SLOT;
+    }
+  };
+  find_slots(0);
   const int last = t.f0 + t.rows, least = t.past + fast_div(t.f0, p.group_div), most = t.past + fast_div(last - 1, p.group_div);
   {
     const int r = tid & 63, f = t.f0 + r, tok = fast_div(f, p.group_div);
     const T* src = static_cast<const T*>(a.q) + (f < last ? int64_t(t.first + tok) * a.q_stride_t + (kvh * p.group + f - tok * p.group) * a.q_stride_h : 0);
-    for (int e = (tid >> 6) * 4; e < DP; e += 16) {
+    for (int e = (tid >> 6) * 4; e < DP; e += PF_STEP) {
       float x[4] = {};
       if (f < last) load4(src, e, x);
 #pragma unroll
@@ -407,24 +417,39 @@ __global__ void __launch_bounds__(PF_THREADS, DP <= 128 ? 2 : 1) prefill_fma_ker
     const bool all = base + PF_N <= t.prefix || (base + PF_N <= least + 1 && (a.window == 0 || base > most - a.window));
     __syncthreads();  // the block before is read
     {  // keys: a token a lane, transposed
-      const int r = tid & 63, j = base + r;
-      const bool seen = tile_sees(t, j);
-      const T* row = static_cast<const T*>(a.k_cache) + (seen ? token_offset(p, table, j) + kvh * a.c_stride_h : 0);
-      for (int e = (tid >> 6) * 4; e < DP; e += 16) {
-        float x[4] = {};
-        if (seen) load4(row, e, x);
+      const int r = tid & 63;
+      const int64_t off = offs[b & 1][r];
+#pragma unroll 1
+      for (int e0 = (tid >> 6) * 4; e0 < DP; e0 += U * PF_STEP) {
+        float x[U][4] = {};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) ks[(e + i) * PF_LD + r] = x[i];
+        for (int u = 0; u < U; ++u)
+          if (off != NO_SLOT && e0 + u * PF_STEP < DP) load4(static_cast<const T*>(a.k_cache) + off, e0 + u * PF_STEP, x[u]);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (e0 + u * PF_STEP < DP) ks[(e0 + u * PF_STEP + i) * PF_LD + r] = x[u][i];
       }
     }
-    for (int i = tid; i < PF_N * (DP / 4); i += PF_THREADS) {
-      const int r = i / (DP / 4), e = i % (DP / 4) * 4, j = base + r;
-      float x[4] = {};
-      if (tile_sees(t, j)) load4(static_cast<const T*>(a.v_cache) + token_offset(p, table, j) + kvh * a.c_stride_h, e, x);
-      if (!all) special |= !(fabsf(x[0]) + fabsf(x[1]) + fabsf(x[2]) + fabsf(x[3]) < INFINITY);
-      *reinterpret_cast<float4*>(vs + r * DP + e) = make_float4(x[0], x[1], x[2], x[3]);
+#pragma unroll 1
+    for (int i0 = tid; i0 < PF_N * (DP / 4); i0 += U * PF_THREADS) {
+      float x[U][4] = {};
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * PF_THREADS;
+        const int64_t off = offs[b & 1][i / (DP / 4) % PF_N];
+        if (off != NO_SLOT && i < PF_N * (DP / 4)) load4(static_cast<const T*>(a.v_cache) + off, i % (DP / 4) * 4, x[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int i = i0 + u * PF_THREADS;
+        if (!all) special |= !(fabsf(x[u][0]) + fabsf(x[u][1]) + fabsf(x[u][2]) + fabsf(x[u][3]) < INFINITY);
+        if (i < PF_N * (DP / 4)) *reinterpret_cast<float4*>(vs + i / (DP / 4) * DP + i % (DP / 4) * 4) = make_float4(x[u][0], x[u][1], x[u][2], x[u][3]);
+      }
     }
     __syncthreads();
+    if (b + 1 < blocks.count) find_slots(b + 1);
     float s[4][4] = {};
 #pragma unroll 8
     for (int e = 0; e < DP; ++e) {
@@ -464,6 +489,7 @@ __global__ void __launch_bounds__(PF_THREADS, DP <= 128 ? 2 : 1) prefill_fma_ker
         l[r] += s[r][c];
       }
     }
+    if (DP <= 128) __syncthreads();  // the keys are read
 #pragma unroll
     for (int c = 0; c < 4; ++c) *reinterpret_cast<float4*>(ps + (tx * 4 + c) * PF_LD + ty * 4) = make_float4(s[0][c], s[1][c], s[2][c], s[3][c]);
     __syncthreads();
@@ -484,7 +510,7 @@ __global__ void __launch_bounds__(PF_THREADS, DP <= 128 ? 2 : 1) prefill_fma_ker
       }
     }
   }
-  uint32_t redo = 0;  // of this warp's eight rows: 4 (ty & 1) + r
+  uint32_t redo = 0;  // of this warp's rows: 4 (ty & 1) + r
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
 #pragma unroll
@@ -537,15 +563,15 @@ int launch_fma(const PagedParams& p, cudaStream_t st) {
   prefill_fma_kernel<DT, DP, VEC><<<dim3(unsigned(grid_tiles(p, PF_ROWS)), p.a.n_kv_heads), PF_THREADS, pf_smem<DP>(), st>>>(p);
   return cuda_status(cudaGetLastError(), "paged_prefill");
 }
-// Tiles of 64 rows from 24 rows a request on (tokens times grouped heads) and 16 rows an SM over all KV heads, tiles of
+// Tiles of 64 rows from 24 rows a request on (tokens times grouped heads) and 12 rows an SM over all KV heads, tiles of
 // four below: they are 16 times as many CTAs, and a CTA is twice as quick.  fp32, 32/8 heads of 128, tiles of 64 / of
-// four: 16 requests of 1000 tokens and 2, 4, 8, 16 new ones 264, 264, 265, 268 / 135, 251, 366, 602 us; one of 2000
-// tokens and 32, 64, 96, 128 new ones 404, 417, 418, 429 / 199, 418, 430, 633 us.
+// four: 16 requests of 1000 tokens and 2, 4, 8, 16 new ones 207, 329, 335, 340 / 134, 250, 362, 598 us; one of 2000
+// tokens and 32, 48, 64, 96, 128 new ones 350, 350, 360, 361, 371 / 199, 219, 419, 429, 633 us.
 template <class DT>
 int launch_simt(const PagedParams& p, cudaStream_t st) {
   const int D = p.a.head_dim;
   const bool vec = D % 4 == 0 && paged_aligned(p.a);
-  if (p.a.n_rows * p.group >= 24 * int64_t(p.a.batch) && p.a.n_rows * p.a.n_q_heads >= 16 * int64_t(num_sms())) {
+  if (p.a.n_rows * p.group >= 24 * int64_t(p.a.batch) && p.a.n_rows * p.a.n_q_heads >= 12 * int64_t(num_sms())) {
     if (D <= 64) return vec ? launch_fma<DT, 64, true>(p, st) : launch_fma<DT, 64, false>(p, st);
     if (D <= 128) return vec ? launch_fma<DT, 128, true>(p, st) : launch_fma<DT, 128, false>(p, st);
     return vec ? launch_fma<DT, 256, true>(p, st) : launch_fma<DT, 256, false>(p, st);
