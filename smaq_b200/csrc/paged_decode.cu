@@ -955,10 +955,10 @@ __global__ void __launch_bounds__(PD_THREADS) paged_join_kernel(const __grid_con
   // every slot's maximum and sum at once, then its factor
   float m = -INFINITY;
   for (int i = threadIdx.x; i < n; i += PD_THREADS) {
-    const float2 ml = *reinterpret_cast<const float2*>(slot + i * step + D);
-    factor[i] = ml.x;
-    part[i] = ml.y;
-    m = fmaxf(m, ml.x);
+    const float* ml = slot + i * step + D;  // two scalars: at odd head dims a slot's rows start at odd floats
+    factor[i] = ml[0];
+    part[i] = ml[1];
+    m = fmaxf(m, factor[i]);
   }
   m = warp_max(m);
   if ((threadIdx.x & 31) == 0) reduce[threadIdx.x >> 5] = m;
