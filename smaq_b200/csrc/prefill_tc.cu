@@ -161,7 +161,7 @@ __global__ void __launch_bounds__(pt_threads(D), 1) prefill_tc_kernel(const __gr
   if (threadIdx.x == 0) {
     mbar_init(&bars.q_full, TILES * PT_TW);
     mbar_init(&bars.o_step, 1);
-    mbar_init(&bars.v_part, 1);
+    mbar_init(&bars.v_part, PT_LOADERS / 32);  // one arrival a copying warp: a phase ends only when all have passed the last
     for (int s = 0; s < 2; ++s) {
       mbar_init(&bars.k_full[s], PT_LOADERS);
       mbar_init(&bars.v_full[s], PT_LOADERS);
@@ -243,6 +243,7 @@ __global__ void __launch_bounds__(pt_threads(D), 1) prefill_tc_kernel(const __gr
               tma_5d(lead, dst + b * pt.box * (D * 2), values ? &pt.v : &pt.k, kvh * int(a.c_stride_h), 0, 0, slot >> 3, pg, clear ? &bars.v_part : bar);
           }
           if (clear) {
+            if (w > 0 && lane == 0) mbar_arrive(&bars.v_part);
             if (!warp_wait(&bars.v_part, partial++ & 1)) failed = true;
             const int pre = t.prefix - first, lo = t.lo - first, hi = t.hi - first;
 #pragma unroll 4
