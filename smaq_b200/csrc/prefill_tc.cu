@@ -202,10 +202,6 @@ __global__ void __launch_bounds__(pt_threads(D), 1) prefill_tc_kernel(const __gr
       // By TMA a block comes in boxes of one page (or 128 slots of it), the warps in turn; a box without a token that some
       // row sees is left out.  (Issued by the lanes of one warp side by side, boxes cost about 150 cycles each.)
       const int per = PT_N / pt.box;
-      auto whole = [&](int k) {
-        const int b = base_of(k);
-        return b + PT_N <= t.prefix || (b >= t.lo && b + PT_N <= t.hi);
-      };
       auto needed = [&](int k) {  // this lane's box of block k
         const int b = base_of(k) + lane * pt.box;
         return pt.tma && k < n && lane < per && (b < t.prefix || (b + pt.box > t.lo && b < t.hi));
@@ -231,35 +227,33 @@ __global__ void __launch_bounds__(pt_threads(D), 1) prefill_tc_kernel(const __gr
         const uint32_t dst = (values ? vs : ks) + s * TILE;
         const bool part = values && !seen_by_all(base_of(j));
         if (pt.tma) {
-          // The scores of tokens that no row sees are replaced whatever their keys are, but their values are multiplied by
-          // zero: in a block with such tokens the values arrive at v_part and their rows are cleared.
-          const bool clear = values && !whole(j);
+          // The scores of tokens that a row does not see are replaced whatever their keys are, but their values are multiplied
+          // by zero.  A block that is not seen by all rows therefore has its values arrive at v_part: rows that nobody sees are
+          // cleared and the others looked through before the products may have them, since from then on another warp may
+          // fill the stage again.
           const uint32_t boxes = __ballot_sync(~0u, needed(j));
-          if (tid == 0) mbar_arrive_expect_tx(clear ? &bars.v_part : bar, __popc(boxes) * pt.box * D * 2);
+          uint64_t* here = part ? &bars.v_part : bar;
+          if (tid == 0) mbar_arrive_expect_tx(here, __popc(boxes) * pt.box * D * 2);
           const int first = base_of(j), slot = per > 1 ? 0 : first - fast_div(first, p.page_div) * a.page_size;
           for (int b = w; b < per; b += MMA_WARP - LOAD_WARP) {
             const int pg = __shfl_sync(~0u, page, b);
-            if (boxes >> b & 1)
-              tma_5d(lead, dst + b * pt.box * (D * 2), values ? &pt.v : &pt.k, kvh * int(a.c_stride_h), 0, 0, slot >> 3, pg, clear ? &bars.v_part : bar);
+            if (boxes >> b & 1) tma_5d(lead, dst + b * pt.box * (D * 2), values ? &pt.v : &pt.k, kvh * int(a.c_stride_h), 0, 0, slot >> 3, pg, here);
           }
-          if (clear) {
-            if (w > 0 && lane == 0) mbar_arrive(&bars.v_part);
-            if (!warp_wait(&bars.v_part, partial++ & 1)) failed = true;
+          if (part) {
+            if (w > 0 && lane == 0) mbar_arrive(here);
+            if (!warp_wait(here, partial++ & 1)) failed = true;
             const int pre = t.prefix - first, lo = t.lo - first, hi = t.hi - first;
+            if (pre < PT_N && (lo > 0 || hi < PT_N)) {
 #pragma unroll 4
-            for (int i = lane; i < rows * CH; i += 32)
-              if (const int r = r0 + i / CH; r >= pre && (r < lo || r >= hi)) *reinterpret_cast<uint4*>(smem + (dst - qs) + at(r0 + i / CH, i % CH)) = make_uint4(0, 0, 0, 0);
-            __syncwarp();
-            if (part) look_for_special(s);
+              for (int i = lane; i < rows * CH; i += 32)
+                if (const int r = r0 + i / CH; r >= pre && (r < lo || r >= hi)) *reinterpret_cast<uint4*>(smem + (dst - qs) + at(r0 + i / CH, i % CH)) = make_uint4(0, 0, 0, 0);
+              __syncwarp();
+            }
+            look_for_special(s);
             fence_proxy_async_smem();
             mbar_arrive(bar);
-          } else {
-            if (tid != 0) mbar_arrive(bar);
-            if (part) {
-              if (!warp_wait(bar, (j / STAGES) & 1)) failed = true;
-              look_for_special(s);
-              fence_proxy_async_smem();  // before the stage is filled again
-            }
+          } else if (tid != 0) {
+            mbar_arrive(bar);
           }
           return;
         }

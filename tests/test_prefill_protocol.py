@@ -81,3 +81,48 @@ def test_no_order_of_steps_leaves_a_warp_waiting(blocks):
 def test_one_arrival_a_phase_is_not_enough():
     """The walk finds what it looks for: with the first warp's arrival alone a late warp's phase comes round again."""
     assert stuck_states(1, [(1, 0, 0)] * 4)
+
+
+def scans_first():
+    """Whether a block's rows are looked through before their warp lets the products have them."""
+    text = source()
+    copies = text[text.index("if (pt.tma) {"):]
+    copies = copies[:copies.index("return;")]
+    return copies.rindex("look_for_special(s)") < copies.index("mbar_arrive(bar)")
+
+
+def overwritten_scans(scan_first, blocks):
+    """Orders in which a warp copies into a stage whose rows another warp still looks through.  A warp's steps for a block:
+    copy when the products are through with the stage's last block, then scan and arrive, or arrive and scan."""
+    start, found = ((0, 0),) * WARPS + (0,), []        # (block, step) of each warp; blocks that the products are through with
+    seen, todo = {start}, [start]
+    while todo:
+        state = todo.pop()
+        warps, through = state[:WARPS], state[WARPS]
+        arrived = [b + (step == 2 and not scan_first) for b, step in warps]     # blocks that each warp has arrived for
+        ways = [warps + (through + 1,)] if through < min(arrived) else []
+        for i, (b, step) in enumerate(warps):
+            if b == blocks or (step == 0 and b >= STAGES and through <= b - STAGES):
+                continue
+            if step == 0:
+                if any(x[0] <= b - STAGES for x in warps):
+                    found.append(state)
+                new = (b, 1)
+            elif step == 1 and not scan_first:
+                new = (b, 2)
+            else:
+                new = (b + 1, 0)
+            ways.append(warps[:i] + (new,) + warps[i + 1:] + (through,))
+        for s in ways:
+            if s not in seen:
+                seen.add(s)
+                todo.append(s)
+    return found
+
+
+def test_no_stage_is_filled_while_it_is_looked_through():
+    assert not overwritten_scans(scans_first(), 4)
+
+
+def test_arriving_before_the_scan_is_not_enough():
+    assert overwritten_scans(False, 4)
