@@ -493,6 +493,10 @@ int smaq_paged_prefill(const smaq_paged_args* args, void* stream);
 /* SMAQ_ERR_DEVICE if a bounded wait of smaq_paged_prefill or smaq_norm_rope ran out since the last
  * check (clears it).  Synchronises the stream. */
 int smaq_exact_status(void* stream);
+/* Polls (4 us each) after which such a wait gives up, for later calls of this process; negative: the default, a
+ * second, which is also the most.  Small limits are for testing the error path: the rows concerned come out as NaN
+ * (smaq_paged_prefill) or are not written (smaq_norm_rope). */
+void smaq_exact_set_wait_limit(int64_t polls);
 /* sizeof(smaq_tables_args), smaq_norm_rope_args, smaq_paged_args for which = 0, 1, 2, else 0. */
 size_t smaq_paged_args_size(int which);
 

@@ -32,7 +32,7 @@ EXPORTS = (
     "smaq_kmeans", "smaq_comm_set_backend", "smaq_comm_unique_id", "smaq_comm_init", "smaq_comm_allgather",
     "smaq_comm_wait", "smaq_comm_status", "smaq_comm_abort", "smaq_comm_destroy",
     "smaq_paged_args_size", "smaq_step_tables", "smaq_norm_rope", "smaq_paged_decode_workspace_size",
-    "smaq_paged_decode", "smaq_paged_prefill_workspace_size", "smaq_paged_prefill", "smaq_exact_status",
+    "smaq_paged_decode", "smaq_paged_prefill_workspace_size", "smaq_paged_prefill", "smaq_exact_status", "smaq_exact_set_wait_limit",
 )
 
 vp = C.c_void_p
@@ -192,6 +192,8 @@ def load() -> C.CDLL:
     lib.smaq_paged_prefill.restype = i32
     lib.smaq_exact_status.argtypes = [vp]
     lib.smaq_exact_status.restype = i32
+    lib.smaq_exact_set_wait_limit.argtypes = [i64]
+    lib.smaq_exact_set_wait_limit.restype = None
     lib.smaq_last_error.restype = C.c_char_p
     lib.smaq_append.argtypes = [C.POINTER(AppendArgs), vp]
     lib.smaq_append.restype = i32

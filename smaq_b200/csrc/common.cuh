@@ -17,6 +17,8 @@ int cuda_status(cudaError_t e, const char* where);
 int num_sms();
 // Lets `kernel` use `bytes` of dynamic shared memory on the current device; asked of the driver once a device.
 int allow_smem(const void* kernel, int bytes, const char* where);
+// Polls after which a wait inside the exact step's kernels gives up (smaq_exact_set_wait_limit).
+uint32_t exact_wait_limit();
 
 // ---------------------------------------------------------------- dtype tags
 struct F32 {

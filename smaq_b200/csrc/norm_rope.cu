@@ -22,6 +22,7 @@ namespace {
 struct NrParams {
   smaq_norm_rope_args a;
   int heads;            // q + k (+ v with a cache)
+  uint32_t spin;        // polls before a wait gives up
   int per;              // heads that a lane group walks
   int groups, q_groups, k_groups;  // lane groups a token, of its queries and of its keys (and values)
   float inv_dim;
@@ -273,7 +274,6 @@ __global__ void __launch_bounds__(NR_THREADS, NR_CTAS) norm_rope_kernel(const __
 // to the cache by bulk copies too.  For heads that lie side by side in a token.
 constexpr int NS_THREADS = 256, NS_CTAS = 2, NS_SMEM = 112 * 1024, NS_MOST = 16;
 constexpr int NS_ROUNDS = 3;
-constexpr uint32_t NS_SPIN = 1u << 24;
 
 __device__ unsigned int g_norm_rope_fault;
 
@@ -344,11 +344,13 @@ __global__ void __launch_bounds__(NS_THREADS, NS_CTAS) norm_rope_staged_kernel(c
     if (int64_t(blockIdx.x) + gridDim.x < batches) bring(int64_t(blockIdx.x) + gridDim.x, 1);
   }
   int turn = 0;
-  for (int64_t n = blockIdx.x; n < batches; n += gridDim.x, ++turn) {
+  int64_t n = blockIdx.x;
+  for (; n < batches; n += gridDim.x, ++turn) {
     const int s = turn & 1, tokens = int(min(int64_t(p.per), a.n_tokens - n * p.per));
-    if (!mbar_wait(&bars.full[s], (turn >> 1) & 1, NS_SPIN)) bars.dead = 1;
+    const bool here = __all_sync(~0u, mbar_wait(&bars.full[s], (turn >> 1) & 1, p.spin));
+    if (!here) bars.dead = 1;
     const uint8_t* base = smem + s * batch;
-    if (v_bytes && int(threadIdx.x) < tokens) {  // values: straight on
+    if (here && v_bytes && int(threadIdx.x) < tokens) {  // values: straight on
       const int64_t t = n * p.per + threadIdx.x, at = slot_offset(p, a.slots[t]);
       if (at >= 0) {
         const uint32_t src = smem_u32(base) + threadIdx.x * token + q_bytes + k_bytes;
@@ -358,7 +360,7 @@ __global__ void __launch_bounds__(NS_THREADS, NS_CTAS) norm_rope_staged_kernel(c
       }
       asm volatile("cp.async.bulk.commit_group;" ::: "memory");
     }
-    if (mine < tokens) {
+    if (here && mine < tokens) {
       const int64_t t = n * p.per + mine;
       const uint8_t* rows = base + mine * token;
       uint64_t c[4], sn[4];
@@ -429,7 +431,10 @@ __global__ void __launch_bounds__(NS_THREADS, NS_CTAS) norm_rope_staged_kernel(c
     if (threadIdx.x < 32 && next < batches) bring(next, s);
   }
   if (v_bytes && int(threadIdx.x) < p.per) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
-  if (threadIdx.x == 0 && bars.dead) atomicOr(&g_norm_rope_fault, 1u);
+  if (!bars.dead) return;
+  for (int i = 0; i < 2; ++i, n += gridDim.x, ++turn)  // this batch and the next are under way
+    if (n < batches) mbar_drain(&bars.full[turn & 1], (turn >> 1) & 1);
+  if (threadIdx.x == 0) atomicOr(&g_norm_rope_fault, 1u);
 }
 
 __global__ void __launch_bounds__(NR_THREADS) norm_rope_any_kernel(const __grid_constant__ NrParams p) {
@@ -555,6 +560,7 @@ extern "C" int smaq_norm_rope(const smaq_norm_rope_args* args, void* stream) {
   NrParams p;
   p.a = a;
   p.heads = a.n_q_heads + a.n_kv_heads * (cache ? 2 : 1);
+  p.spin = exact_wait_limit();
   p.per = 1;
   p.groups = p.heads;
   p.inv_dim = 1.0f / float(a.head_dim);

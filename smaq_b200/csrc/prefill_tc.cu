@@ -22,11 +22,12 @@
 // Few rows with long walks: several CTAs share a tile's walk and prefill_join_kernel adds their parts in order.
 // Bound by both the products and the exponentials (2048 cycles a block each, of about 3300 in all): 8192 tokens at 32/8
 // heads of 128 in 514 us, 1070 TFLOP/s, 64% of what a library product reaches in short runs.
-// Every wait is bounded; one that runs out sets g_prefill_fault and the CTA drains.
+// Every wait is bounded; one that runs out sets g_prefill_fault, and its rows come out as NaN.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <atomic>
 
 #include "paged_prefill.cuh"
 #include "prefill_tc.cuh"
@@ -51,10 +52,6 @@ __host__ __device__ constexpr int pt_rows(int D) { return 128 * pt_tiles(D); }
 __host__ __device__ constexpr int pt_threads(int D) { return 32 * (PT_TW * pt_tiles(D) + 4); }
 constexpr uint32_t PT_COLS = 512;
 constexpr float PT_LAG = 8.0f;            // log2
-constexpr uint32_t PT_SPIN = 1u << 24;    // polls before a wait gives up
-
-// The whole warp waits, and gives up together.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity) { return __all_sync(~0u, mbar_wait(bar, parity, PT_SPIN)); }
 
 template <int D>
 struct PtCfg {
@@ -69,6 +66,7 @@ struct PtParams {
   int tma;         // keys and values come through the tensor maps where a block's pages allow it
   int box;         // slots a box: page_size, at most PT_N
   int splits;      // CTAs that share a tile's walk, at most
+  uint32_t spin;   // polls before a wait gives up
   float* parts;    // [tile][KV head][split]: accumulators [rows][D], maxima, sums, whether a special value was met
   CUtensorMap k, v;
 };
@@ -77,7 +75,7 @@ __host__ __device__ constexpr int64_t part_floats(int D) { return int64_t(pt_row
 __device__ __forceinline__ int splits_of(int n, int most) { return max(1, min(most, n / 2)); }
 
 struct PtBars {
-  uint64_t q_full, v_part, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready[2], o_step, o_full[2];
+  uint64_t q_full, v_part, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_ready[2], o_step, o_full[2], drained;
   uint32_t tmem;
   int special;
   // the tile and its walk: read from here where needed, the softmax has no registers for them
@@ -85,7 +83,7 @@ struct PtBars {
   PrefillBlocks blocks;
   int least, most;          // first and last row's position
   float row[2][2][2][128];  // [turn][tile][half]: row maxima, at the end row sums
-  int fail[2][4];           // a wait of one of the two warps that share rows ran out: both stop at their next meeting
+  int fail[2][2][4];        // [turn][tile][rows]: a wait of one of the two warps that share rows ran out: both stop at that turn's meeting
 };
 
 __device__ __forceinline__ void named_bar(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
@@ -161,6 +159,7 @@ __global__ void __launch_bounds__(pt_threads(D), 1) prefill_tc_kernel(const __gr
   if (threadIdx.x == 0) {
     mbar_init(&bars.q_full, TILES * PT_TW);
     mbar_init(&bars.o_step, 1);
+    mbar_init(&bars.drained, 1);
     mbar_init(&bars.v_part, PT_LOADERS / 32);  // one arrival a copying warp: a phase ends only when all have passed the last
     for (int s = 0; s < 2; ++s) {
       mbar_init(&bars.k_full[s], PT_LOADERS);
@@ -172,7 +171,7 @@ __global__ void __launch_bounds__(pt_threads(D), 1) prefill_tc_kernel(const __gr
       mbar_init(&bars.o_full[s], 1);
     }
     bars.special = 0;
-    for (int i = 0; i < 8; ++i) bars.fail[i >> 2][i & 3] = 0;
+    for (int i = 0; i < 16; ++i) bars.fail[i >> 3][i >> 2 & 1][i & 3] = 0;
     fence_mbar_init();
   }
   if (warp == MMA_WARP) alloc(&bars.tmem, PT_COLS);
@@ -182,6 +181,8 @@ __global__ void __launch_bounds__(pt_threads(D), 1) prefill_tc_kernel(const __gr
   constexpr uint32_t tmem = 0;  // all 512 columns are this CTA's: the allocation starts at 0
   constexpr uint32_t s_col = 0, o_col = 256;  // S of tile i (one tile: of blocks of parity i) at s_col + 128 i, O at o_col + D i
   bool failed = false;
+  // The whole warp waits, and gives up together.
+  auto warp_wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(~0u, mbar_wait(bar, parity, pt.spin)); };
 
   // a row's chunk of eight channels in an operand
   auto at = [](int r, int ch) { return uint32_t((r >> 3) * GROUP + (ch >> 3) * 1024 + (r & 7) * 128 + (((ch & 7) ^ (r & 7)) << 4)); };
@@ -279,17 +280,24 @@ __global__ void __launch_bounds__(pt_threads(D), 1) prefill_tc_kernel(const __gr
         fence_proxy_async_smem();
         mbar_arrive(bar);
       };
-      int page = page_of(0);
+      int page = page_of(0), k_sent = 0, v_sent = 0;
       for (int j = 0; j < n; ++j) {
         const int s = j % STAGES;
         const uint32_t ph = uint32_t((j / STAGES) & 1) ^ 1u;
         const int next = page_of(j + 1);
         if (!warp_wait(&bars.k_empty[s], ph)) { failed = true; break; }
         fetch(j, s, false, page);
+        ++k_sent;
         if (!warp_wait(&bars.v_empty[s], ph)) { failed = true; break; }
         fetch(j, s, true, page);
+        ++v_sent;
         if (failed) break;
         page = next;
+      }
+      if (failed) {  // copies in flight land before the block leaves
+        for (int j = max(k_sent - STAGES, 0); j < k_sent; ++j) mbar_drain(&bars.k_full[j % STAGES], (j / STAGES) & 1);
+        for (int j = max(v_sent - STAGES, 0); j < v_sent; ++j) mbar_drain(&bars.v_full[j % STAGES], (j / STAGES) & 1);
+        if (partial > 0) mbar_drain(&bars.v_part, (partial - 1) & 1);
       }
     } else if (warp == MMA_WARP && n > 0) {
       // ---- products
@@ -357,6 +365,10 @@ __global__ void __launch_bounds__(pt_threads(D), 1) prefill_tc_kernel(const __gr
         }
       }
       failed = !ok;
+      if (failed) {  // products in flight end before their tensor memory is given back
+        commit(lead, &bars.drained);
+        mbar_drain(&bars.drained, 0);
+      }
     }
   } else {
     if constexpr (TILES == 2) asm volatile("setmaxnreg.inc.sync.aligned.u32 104;");  // one tile: 384 threads have 168 anyway
@@ -387,7 +399,7 @@ __global__ void __launch_bounds__(pt_threads(D), 1) prefill_tc_kernel(const __gr
         const bool part = !seen_by_all(base - half * C);
         const int buf = TILES == 2 ? i : j & 1;  // of the scores
         const uint32_t ts = tmem + lanes + s_col + 128 * buf;
-        if (!warp_wait(&bars.s_full[buf], (TILES == 2 ? j : j >> 1) & 1)) bars.fail[i][warp & 3] = 1;
+        if (!warp_wait(&bars.s_full[buf], (TILES == 2 ? j : j >> 1) & 1)) bars.fail[j & 1][i][warp & 3] = 1;
         fence_after();
         // Two passes over the scores, 32 columns at a time, so that they need not stay in registers: the first
         // finds the maximum and puts capped, biased or masked scores back, the second makes the weights.
@@ -460,7 +472,7 @@ __global__ void __launch_bounds__(pt_threads(D), 1) prefill_tc_kernel(const __gr
         bars.row[j & 1][i][half][row] = mx;
         named_bar(meet, 64);
         mx = fmaxf(mx, bars.row[j & 1][i][half ^ 1][row]);
-        if (*reinterpret_cast<volatile int*>(&bars.fail[i][warp & 3])) { failed = true; break; }
+        if (*reinterpret_cast<volatile int*>(&bars.fail[j & 1][i][warp & 3])) { failed = true; break; }
         float factor = 1.f;
         if (mx > m + PT_LAG || (j == 0 && mx > m)) {
           factor = m == -INFINITY ? 0.f : ex2(m - mx);
@@ -470,7 +482,7 @@ __global__ void __launch_bounds__(pt_threads(D), 1) prefill_tc_kernel(const __gr
           l *= factor;
           if (j > 0) {
             if constexpr (TILES == 1) {  // these scores were multiplied before the last block's values
-              if (!warp_wait(&bars.o_step, (j - 1) & 1)) bars.fail[i][warp & 3] = 1;
+              if (!warp_wait(&bars.o_step, (j - 1) & 1)) bars.fail[(j + 1) & 1][i][warp & 3] = 1;
               fence_after();
             }
 #pragma unroll 1  // cold: unrolled, its code costs the first pass 10 us of 519
@@ -522,6 +534,8 @@ __global__ void __launch_bounds__(pt_threads(D), 1) prefill_tc_kernel(const __gr
       bars.row[n & 1][i][half][row] = l;
       named_bar(meet, 64);
       l += bars.row[n & 1][i][half ^ 1][row];
+      failed |= *reinterpret_cast<volatile int*>(&bars.fail[n & 1][i][warp & 3]) != 0;
+      if (failed) l = __int_as_float(0x7FC00000);  // a row whose wait ran out is NaN, here or from the join
       if (alone) {
         const float inv = l == 0.f ? 0.f : 1.0f / l;
         T* out = static_cast<T*>(a.out) + int64_t(t.first + tok) * a.o_stride_t + h * a.o_stride_h + half * (D / PT_SPLIT);
@@ -541,7 +555,7 @@ __global__ void __launch_bounds__(pt_threads(D), 1) prefill_tc_kernel(const __gr
             odd += (u + v) * 0.f;
             w[e / 2] = pack2<DT>(u, v);
           }
-          if (f < last && !failed) {
+          if (f < last) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) reinterpret_cast<uint4*>(out + 32 * c)[e] = make_uint4(w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
           }
@@ -705,6 +719,7 @@ int launch(const PagedParams& p, cudaStream_t st) {
   }
   const int64_t units = grid_tiles(a.n_rows, a.batch, p.group, D) * a.n_kv_heads;
   pt.splits = splits_for(units, int64_t(a.max_blocks) * a.page_size);
+  pt.spin = exact_wait_limit();
   pt.parts = static_cast<float*>(a.workspace);
   if (units * pt.splits * (pt_rows(D) / PJ_ROWS) >= (int64_t(1) << 31)) return fail(SMAQ_ERR_UNSUPPORTED, "paged_prefill: too many rows");
   const size_t need = prefill_tc_workspace(a.n_rows, a.batch, a.n_q_heads, a.n_kv_heads, D, int64_t(a.max_blocks) * a.page_size);
@@ -755,6 +770,16 @@ int launch_prefill_tc(const PagedParams& p, cudaStream_t st) {
 
 namespace smaq {
 int norm_rope_fault(bool& set);  // norm_rope.cu
+}
+
+namespace smaq {
+// A poll lasts 4 us (the hardware suspends it): a wait gives up after a second.
+static std::atomic<uint32_t> g_wait_limit{1u << 18};
+uint32_t exact_wait_limit() { return g_wait_limit.load(std::memory_order_relaxed); }
+}  // namespace smaq
+
+extern "C" void smaq_exact_set_wait_limit(int64_t polls) {
+  smaq::g_wait_limit.store(polls < 0 ? 1u << 18 : uint32_t(std::min<int64_t>(polls, 1 << 18)), std::memory_order_relaxed);
 }
 
 extern "C" int smaq_exact_status(void* stream) {

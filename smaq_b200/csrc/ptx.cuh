@@ -41,7 +41,7 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, uint32
   return false;
 }
 
-// One non-blocking probe of an mbarrier phase (profiling builds).
+// One non-blocking probe of an mbarrier phase.
 __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
   uint32_t done;
   asm volatile(
@@ -52,6 +52,12 @@ __device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
       : "r"(smem_u32(bar)), "r"(parity)
       : "memory");
   return done != 0;
+}
+
+// After a wait that ran out: gives what is still in flight towards `bar` some milliseconds to land.
+__device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity) {
+#pragma unroll 1
+  for (int i = 0; i < (1 << 14) && !mbar_test(bar, parity); ++i) __nanosleep(200);
 }
 
 // Bulk copy global -> shared (no multicast); completes `bytes` on the mbarrier.

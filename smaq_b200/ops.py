@@ -810,6 +810,12 @@ def exact_status() -> None:
     _lib.check(_lib.load().smaq_exact_status(_stream()), "smaq_exact_status")
 
 
+def exact_wait_limit(polls: Optional[int] = None) -> None:
+    """Polls (4 us each) after which those waits give up, for later calls; None: the default, a second
+    (smaq_exact_set_wait_limit).  Small limits are for testing that a wait that runs out is reported."""
+    _lib.load().smaq_exact_set_wait_limit(-1 if polls is None else polls)
+
+
 def selftest_wait_timeout(spin_limit: int = 1 << 12) -> int:
     """Run a kernel whose mbarrier wait can never complete with a ``spin_limit`` poll bound;
     returns the library status (``5`` = SMAQ_ERR_DEVICE when the timeout path works)."""
