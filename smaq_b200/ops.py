@@ -711,7 +711,7 @@ def _paged(name, q, k_cache, v_cache, block_table, seq_lens, cu_query, prefix_le
     if block_table.dtype is not torch.int32:
         block_table = block_table.to(torch.int32)
     row, col = block_table.stride()
-    if M > 1 and col != 1:
+    if (M > 1 and col != 1) or (B > 1 and row < M):  # rows that overlap, such as one row expanded over requests
         block_table = block_table.contiguous()
         row = M
     seq_lens = _int32("seq_lens", seq_lens, B)

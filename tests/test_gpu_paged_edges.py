@@ -3,7 +3,8 @@
 import pytest
 import torch
 
-from test_gpu_paged_attention import BF, HF, SF, decode, prefill
+from paged_ref import paged_case
+from test_gpu_paged_attention import BF, HF, SF, decode, prefill, queries
 
 pytestmark = pytest.mark.gpu
 
@@ -26,3 +27,19 @@ def test_prefill_neighbouring_blocks_with_cleared_rows(cuda, D, page, news, ctx,
     from smaq_b200 import ops
     prefill(cuda, news, ctx, 8, 2, D, page, BF, **kw)
     ops.exact_status()
+
+
+def ints(x, cuda):
+    return torch.tensor(x, dtype=torch.int32, device=cuda)
+
+
+def test_tables_whose_rows_overlap(cuda):
+    """One row expanded over the requests, and rows a single column apart: as with a copy of the table."""
+    from smaq_b200 import ops
+    k, v, table = paged_case(cuda, [500], 2, 64, 16, BF, fill=0.0)
+    q, n, cu = queries(cuda, 6, 4, 64, BF), ints([500, 490, 17], cuda), ints([0, 1, 4, 6], cuda)
+    row = table[0]
+    for shared in (row.expand(3, -1), row.as_strided((3, 20), (1, 1)), row[:1].expand(3, 1), table.expand(3, -1)):
+        copy = shared.contiguous()
+        assert torch.equal(ops.paged_decode(q[:3], k, v, shared, n), ops.paged_decode(q[:3], k, v, copy, n))
+        assert torch.equal(ops.paged_prefill(q, k, v, shared, n, cu), ops.paged_prefill(q, k, v, copy, n, cu))
