@@ -528,8 +528,8 @@ def step_tables(free_blocks: torch.Tensor, free_count: torch.Tensor, context_len
         raise ValueError("free_blocks must be a contiguous int32 vector (it is updated in place)")
     width = block_table.shape
     if block_table.dtype is not torch.int32 or len(width) != 2 or width[0] != B or (
-            width[1] > 1 and block_table.stride(1) != 1):
-        raise ValueError(f"block_table must be int32 [{B}, M] with contiguous rows (it is updated in place)")
+            width[1] > 1 and block_table.stride(1) != 1) or (B > 1 and block_table.stride(0) < width[1]):
+        raise ValueError(f"block_table must be int32 [{B}, M] with contiguous rows of their own (it is updated in place)")
     if num_tokens < 0 or block_size < 1:
         raise ValueError(f"num_tokens {num_tokens} or block_size {block_size} out of range")
     free_count = _int32("free_count", free_count, 1)
