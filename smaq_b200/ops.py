@@ -744,6 +744,8 @@ def _paged(name, q, k_cache, v_cache, block_table, seq_lens, cu_query, prefix_le
     if workspace is None and need:
         workspace = q.new_empty(need, dtype=torch.uint8)
     if workspace is not None:
+        if not workspace.is_contiguous():
+            raise ValueError("workspace must be contiguous")
         ws, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
     st = call(
         _lib.pack_paged(q.data_ptr(), qt, qh, k_cache.data_ptr(), v_cache.data_ptr(), cp, cs, ch,

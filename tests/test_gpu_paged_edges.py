@@ -43,3 +43,18 @@ def test_tables_whose_rows_overlap(cuda):
         copy = shared.contiguous()
         assert torch.equal(ops.paged_decode(q[:3], k, v, shared, n), ops.paged_decode(q[:3], k, v, copy, n))
         assert torch.equal(ops.paged_prefill(q, k, v, shared, n, cu), ops.paged_prefill(q, k, v, copy, n, cu))
+
+
+def test_a_workspace_with_gaps_is_refused(cuda):
+    """Its size in bytes is counted from its elements, which have to lie side by side."""
+    from smaq_b200 import ops
+    k, v, table = paged_case(cuda, [500, 90], 2, 64, 16, BF)
+    q, n = queries(cuda, 2, 4, 64, BF), ints([500, 90], cuda)
+    need = ops.paged_decode_workspace_bytes(2, 4, 2, 64)
+    for gappy in (torch.empty(need, 2, dtype=torch.uint8, device=cuda)[:, 0], torch.empty(1, dtype=torch.uint8, device=cuda).expand(need)):
+        with pytest.raises(ValueError, match="contiguous"):
+            ops.paged_decode(q, k, v, table, n, workspace=gappy)
+        with pytest.raises(ValueError, match="contiguous"):
+            ops.paged_prefill(q, k, v, table, n, ints([0, 1, 2], cuda), workspace=gappy)
+    whole = torch.empty(need // 4 + 1, dtype=torch.float32, device=cuda)
+    assert torch.equal(ops.paged_decode(q, k, v, table, n, workspace=whole), ops.paged_decode(q, k, v, table, n))
