@@ -396,6 +396,7 @@ int smaq_kmeans(const float* data, int n_blocks, int64_t n_points, int dim, int 
  *   - request b grows by query_lens[b] (>= 0) tokens and takes the pages it lacks, in request order.
  *     It is admitted if its blocks fit its table row and the pages taken so far, its own included,
  *     do not exceed the stack; one that lacks no page needs none to be left.
+ * Lengths may be anything: negative ones count as 0, sums stop at 2^31 - 1, and a request that reaches it is not admitted.
  * free_blocks and block_table are updated in place (the same call on the same inputs writes the
  * same values again); everything else is written out of place:
  *   cu_query [batch + 1]: prefix sums of query_lens; seq_lens [batch]: context + query, 0 for a

@@ -21,7 +21,12 @@ constexpr int TB_THREADS = 512;
 constexpr int TB_PER = 4;            // tokens a thread
 constexpr int TB_MAX_BATCH = 16384;  // 12 bytes of shared memory a request
 
-__device__ __forceinline__ int3 add3(int3 a, int3 b) { return make_int3(a.x + b.x, a.y + b.y, a.z + b.z); }
+constexpr int kMost = 0x7FFFFFFF;
+
+// Sums of non-negative numbers, at most 2^31 - 1: lengths come from the device and may be anything.
+__device__ __forceinline__ int add(int a, int b) { return int(min(unsigned(a) + unsigned(b), unsigned(kMost))); }
+__device__ __forceinline__ int3 add3(int3 a, int3 b) { return make_int3(add(a.x, b.x), add(a.y, b.y), add(a.z, b.z)); }
+__device__ __forceinline__ int pages_of(int tokens, int s) { return tokens ? (tokens - 1) / s + 1 : 0; }
 
 // Inclusive prefix sum over the block of one int3 a thread; `total` gets the block's sum.
 __device__ __forceinline__ int3 scan3(int3 v, int3* warp_sums, int3& total) {
@@ -60,22 +65,22 @@ __global__ void __launch_bounds__(TB_THREADS) step_tables_kernel(const __grid_co
   int* base = smem + a.batch;   // [B] page j of request b (j >= h_b) is stack entry base - j; < 0: not admitted
   int* back = base + a.batch;   // [B] pages given back up to and with request b
   __shared__ int3 warp_sums[TB_THREADS / 32];
-  __shared__ int used;
+  __shared__ int used, opened;  // pages taken; tokens up to the last request that took one
   const int B = a.batch, s = a.page_size, M = a.max_blocks;
   const int F = min(max(*a.free_count, 0), int(a.pool_size));
-  if (threadIdx.x == 0) used = 0;
+  const int room = int(min(int64_t(M) * s, int64_t(kMost) - 1));  // tokens that a table row holds
+  if (threadIdx.x == 0) used = opened = 0;
   int3 carry = make_int3(0, 0, 0);
   for (int b0 = 0; b0 < B; b0 += TB_THREADS) {
     const int b = b0 + threadIdx.x;
     int3 v = make_int3(0, 0, 0);
     if (b < B) {
-      const int c = max(a.context_lens[b], 0), n = max(a.query_lens[b], 0), held = (c + s - 1) / s;
+      const int c = max(a.context_lens[b], 0), n = max(a.query_lens[b], 0), held = pages_of(c, s);
       if (a.finished && a.finished[b]) {
         v.z = min(held, M);
       } else {
-        const int end = (c + n + s - 1) / s;
         v.x = n;
-        v.y = n > 0 && end <= M ? end - held : 0;
+        v.y = n > 0 && add(c, n) <= room ? pages_of(c + n, s) - held : 0;
       }
     }
     int3 total;
@@ -88,16 +93,19 @@ __global__ void __launch_bounds__(TB_THREADS) step_tables_kernel(const __grid_co
     }
   }
   __syncthreads();
-  const int top = F + carry.z;
+  const int top = add(F, carry.z);
   for (int b = threadIdx.x; b < B; b += TB_THREADS) {
     const int c = max(a.context_lens[b], 0), n = upto[b] - (b ? upto[b - 1] : 0);
-    const int held = (c + s - 1) / s, end = (c + n + s - 1) / s, total = base[b];
-    const bool over = a.finished && a.finished[b];
-    const int need = !over && n > 0 && end <= M ? end - held : 0;
-    const bool ok = !over && end <= M && (need == 0 || total <= top);
+    const int held = pages_of(c, s), total = base[b];
+    const bool over = a.finished && a.finished[b], fits = !over && add(c, n) <= room && upto[b] < kMost;
+    const int need = fits && n > 0 ? pages_of(c + n, s) - held : 0;
+    const bool ok = fits && (need == 0 || total <= top);
     // written over what only this thread reads
-    base[b] = ok ? max(top - 1 - (total - need) + held, 0) : -1;
-    if (ok && need) atomicMax(&used, total);
+    base[b] = ok ? add(max(top - 1 - (total - need), 0), held) : -1;
+    if (ok && need) {
+      atomicMax(&used, total);
+      atomicMax(&opened, upto[b]);
+    }
     if (blockIdx.x == 0) {
       a.cu_query[b + 1] = upto[b];
       a.seq_lens[b] = ok ? c + n : 0;
@@ -120,7 +128,7 @@ __global__ void __launch_bounds__(TB_THREADS) step_tables_kernel(const __grid_co
 
   const int tokens = B ? upto[B - 1] : 0;
   // tokens past n_tokens have no slot to report, but the pages they open are the request's all the same
-  const int64_t end = max(a.n_tokens, int64_t(tokens));
+  const int64_t end = max(a.n_tokens, int64_t(opened));
   for (int64_t t0 = tid * TB_PER; t0 < end; t0 += threads * TB_PER) {
     int pos[TB_PER];
     int64_t slot[TB_PER];
@@ -149,7 +157,7 @@ __global__ void __launch_bounds__(TB_THREADS) step_tables_kernel(const __grid_co
       pos[i] = p;
       if (base[b] < 0) continue;
       if (page < 0) {
-        const int held = (max(a.context_lens[b], 0) + s - 1) / s;
+        const int held = pages_of(max(a.context_lens[b], 0), s);
         if (blk < held) {
           page = a.block_table[b * a.table_stride + blk];
         } else {
