@@ -72,3 +72,17 @@ def test_slow_garbage_does_not_disturb_the_next_step(cuda):
         ops.step_tables(free, ints([BIG], cuda), ints([-2 ** 31, BIG], cuda), ints([BIG, BIG], cuda), table, block_size=4, num_tokens=5)
         t = ops.step_tables(free, ints([8], cuda), ints([0, 0], cuda), ints([4, 5], cuda), table, block_size=4, num_tokens=9)
         assert t.slots.tolist() == [28, 29, 30, 31, 24, 25, 26, 27, 20] and t.free_count.tolist() == [5]
+
+
+@pytest.mark.parametrize("B", [4096, 4079, 4080, 4081, 4097, 16384])   # 4096 before any larger batch of the process
+def test_batches_around_the_default_limit_of_shared_memory(cuda, B):
+    from smaq_b200 import ops
+    page, M = 16, 4
+    ctx, new = [b % 40 for b in range(B)], [(b * 7) % 5 for b in range(B)]
+    stack = list(range(3 * B, 3 * B + B // 8))
+    table = torch.arange(3 * B, dtype=torch.int32).view(B, 3)
+    table = torch.cat([table, torch.full((B, 1), -1, dtype=torch.int32)], 1).to(cuda)
+    want = walk(ctx, new, page, M, stack, table.tolist())
+    t = ops.step_tables(ints(stack, cuda), ints([len(stack)], cuda), ints(ctx, cuda), ints(new, cuda), table, block_size=page, num_tokens=sum(new))
+    assert (t.cu_query.tolist(), t.admitted.tolist(), t.seq_lens.tolist()) == want[:3]
+    assert t.slots.tolist() == want[3] and t.free_count.tolist() == [want[4]] and table.tolist() == want[5]
