@@ -716,11 +716,10 @@ __global__ void __launch_bounds__(PD_THREADS, Stages<4 * D>::CTAS) paged_decode_
         float x = 0.f, sum = 0.f;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
+          // a warp without tokens holds zeros; one whose scores are NaN has no maximum either, and its sum stays NaN times zero
           const float f = ex2(areas[w * Q::AREA + r * LD + D] - z);
-          if (f > 0.f || f != f) {  // a warp without tokens holds zeros
-            x += f * areas[w * Q::AREA + r * LD + e];
-            sum += f * areas[w * Q::AREA + r * LD + D + 1];
-          }
+          x += f * areas[w * Q::AREA + r * LD + e];
+          sum += f * areas[w * Q::AREA + r * LD + D + 1];
         }
         if (all) {
           static_cast<float*>(a.out)[at.b * a.o_stride_t + (first + r) * a.o_stride_h + e] = sum == 0.f ? 0.f : x / sum;

@@ -58,3 +58,25 @@ def test_a_workspace_with_gaps_is_refused(cuda):
             ops.paged_prefill(q, k, v, table, n, ints([0, 1, 2], cuda), workspace=gappy)
     whole = torch.empty(need // 4 + 1, dtype=torch.float32, device=cuda)
     assert torch.equal(ops.paged_decode(q, k, v, table, n, workspace=whole), ops.paged_decode(q, k, v, table, n))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, SF])
+@pytest.mark.parametrize("D", [64, 128, 96, 256])
+def test_decode_nan_reaches_those_who_see_it(cuda, dtype, D):
+    """A NaN query, and a NaN key at the newest token, alone in its warp's share or not, make their rows NaN and no others."""
+    from smaq_b200 import ops
+    lens = [1, 17, 65, 700, 1025, 33]
+    k, v, table = paged_case(cuda, lens, 2, D, 16, dtype)
+    q, n = queries(cuda, len(lens), 8, D, dtype), ints(lens, cuda)
+    want, lse = ops.paged_decode(q, k, v, table, n, return_lse=True)
+    bad = q.clone()
+    bad[:, 5, D // 2] = float("nan")
+    got, gl = ops.paged_decode(bad, k, v, table, n, return_lse=True)
+    others = [h for h in range(8) if h != 5]
+    assert bool(torch.isnan(got[:, 5]).all()) and bool(torch.isnan(gl[:, 5]).all())
+    assert torch.equal(got[:, others], want[:, others]) and torch.equal(gl[:, others], lse[:, others])
+    for b, L in enumerate(lens):
+        k[table[b, (L - 1) // 16].long(), (L - 1) % 16, 1, 3] = float("nan")
+    got, gl = ops.paged_decode(q, k, v, table, n, return_lse=True)
+    assert bool(torch.isnan(got[:, 4:]).all()) and bool(torch.isnan(gl[:, 4:]).all())
+    assert torch.equal(got[:, :4], want[:, :4]) and torch.equal(gl[:, :4], lse[:, :4])
