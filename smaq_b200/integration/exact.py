@@ -37,12 +37,15 @@ class RequestPool:
     def step(self, query_lens: torch.Tensor, num_tokens: int,
              finished: Optional[torch.Tensor] = None) -> ops.StepTables:
         """Pages for ``query_lens [max_requests]`` new tokens (0: the row sits this step out) after the
-        rows marked ``finished`` gave theirs back.  A row that is not admitted keeps what it holds."""
+        rows marked ``finished`` gave theirs back.  A row that is not admitted keeps what it holds.  The
+        pool's tensors are updated in place, so that a step captured in a CUDA graph goes on where the last
+        replay ended."""
         t = ops.step_tables(self.free_blocks, self.free_count, self.context, query_lens, self.block_table,
                             block_size=self.block_size, num_tokens=num_tokens, finished=finished)
-        self.free_count = t.free_count
-        held = self.context if finished is None else self.context.masked_fill(finished, 0)
-        self.context = torch.where(t.admitted, t.seq_lens, held)
+        self.free_count.copy_(t.free_count)
+        if finished is not None:
+            self.context.masked_fill_(finished, 0)
+        torch.where(t.admitted, t.seq_lens, self.context, out=self.context)
         return t
 
 
