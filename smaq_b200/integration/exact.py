@@ -37,9 +37,11 @@ class RequestPool:
     def step(self, query_lens: torch.Tensor, num_tokens: int,
              finished: Optional[torch.Tensor] = None) -> ops.StepTables:
         """Pages for ``query_lens [max_requests]`` new tokens (0: the row sits this step out) after the
-        rows marked ``finished`` gave theirs back.  A row that is not admitted keeps what it holds.  The
-        pool's tensors are updated in place, so that a step captured in a CUDA graph goes on where the last
-        replay ended."""
+        rows marked ``finished`` (bool or uint8) gave theirs back.  A row that is not admitted keeps what
+        it holds.  The pool's tensors are updated in place, so that a step captured in a CUDA graph goes on
+        where the last replay ended."""
+        if finished is not None and finished.dtype is torch.uint8:
+            finished = finished.bool()  # nothing may fail once the stack and the table are updated
         t = ops.step_tables(self.free_blocks, self.free_count, self.context, query_lens, self.block_table,
                             block_size=self.block_size, num_tokens=num_tokens, finished=finished)
         self.free_count.copy_(t.free_count)

@@ -60,3 +60,17 @@ def test_a_step_keeps_no_other_buffers_alive(cuda):
     pool = RequestPool(8, 4, 2, 4, cuda)
     pool.step(torch.tensor([3, 1], dtype=torch.int32, device=cuda), 4)
     assert pool.free_count.untyped_storage().nbytes() == 4 and pool.context.untyped_storage().nbytes() == 8
+
+
+@pytest.mark.parametrize("dtype", [torch.bool, torch.uint8])
+def test_masks_of_ended_rows(cuda, dtype):
+    from smaq_b200.integration.exact import RequestPool
+    pool = RequestPool(8, 4, 3, 4, cuda)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=cuda)  # noqa: E731
+    pool.step(i32([9, 4, 3]), 16)
+    assert pool.context.tolist() == [9, 4, 3] and int(pool.free_count) == 3
+    for ended in ([1, 0, 0], [0, 0, 2 if dtype == torch.uint8 else 1]):
+        pool.step(i32([0, 1, 0]), 1, finished=torch.tensor(ended, device=cuda).to(dtype))
+    assert pool.context.tolist() == [0, 6, 0] and int(pool.free_count) == 6
+    held = pool.block_table[1, :2].tolist()
+    assert sorted(held + pool.free_blocks[:6].tolist()) == list(range(8))
