@@ -15,6 +15,7 @@ struct PagedParams {
   float scale_log2;      // scale * log2 e: factor of a plain score
   float cap_in;          // capped scores: 2 log2 e * scale / cap, factor inside tanh's exponential
   float cap_log2;        // softcap * log2 e
+  float cap_z;           // caps above kCapNear: scale / cap, factor of tanh's argument; 0: others
   FastDiv page_div, group_div;
 };
 
@@ -34,14 +35,25 @@ __device__ __forceinline__ float rcp_approx(float x) {
   return r;
 }
 
-// log2-domain score of the product q.k: tanh z = 1 - 2 / (e^(2z) + 1), whose absolute error (about
-// 2e-7 here) times the cap is what matters; it saturates by itself at both ends.  tanh.approx (2^-11)
-// would put 1% errors into the weights at a cap of 30.
-template <bool CAP>
+// log2-domain score of the product q.k.  Capped: tanh z = 1 - 2 / (e^(2z) + 1), which saturates by itself at both
+// ends.  Its absolute error (about 2e-7 here) times the cap is the score's: up to a cap of kCapNear 1.3e-5, a twentieth of
+// what rounding a weight to fp16 costs.  Above, scores far below the cap (|z| < 0.3) take the Taylor series of tanh,
+// whose first term left out is 5e-8 z, and every score is within 1e-6 of itself.  The series for all caps costs the capped
+// decode of 4 x 128K tokens 354 us instead of 337, a branch around it 341, hence CAP_ANY beside CAP_LOW (up to
+// kCapNear).  tanh.approx (2^-11) would put 1% errors into the weights at a cap of 30.
+constexpr float kCapNear = 64.0f;
+enum { CAP_NONE = 0, CAP_LOW = 1, CAP_ANY = 2 };
+inline int cap_mode(const smaq_paged_args& a) { return a.softcap > kCapNear ? CAP_ANY : a.softcap > 0.f ? CAP_LOW : CAP_NONE; }
+template <int CAP>
 __device__ __forceinline__ float score_log2(float qk, const PagedParams& p) {
-  if constexpr (CAP) {
-    const float t = ex2(qk * p.cap_in);
-    return fmaf(-2.0f * p.cap_log2, rcp_approx(t + 1.0f), p.cap_log2);
+  if constexpr (CAP != CAP_NONE) {
+    float x = fmaf(-2.0f * p.cap_log2, rcp_approx(ex2(qk * p.cap_in) + 1.0f), p.cap_log2);
+    if (CAP == CAP_ANY && p.cap_z != 0.f) {  // alike for all
+      const float z = qk * p.cap_z, zz = z * z;
+      const float near = fmaf(zz, fmaf(zz, fmaf(zz, fmaf(zz, 62.0f / 2835.0f, -17.0f / 315.0f), 2.0f / 15.0f), -1.0f / 3.0f), 1.0f);
+      if (fabsf(z) < 0.3f) x = p.cap_log2 * z * near;
+    }
+    return x;
   } else {
     return qk * p.scale_log2;
   }

@@ -56,6 +56,7 @@ int paged_check(const smaq_paged_args* args, bool prefill, PagedParams& p) {
   p.scale_log2 = a.scale * kLog2e;
   p.cap_in = a.softcap > 0.f ? 2.0f * kLog2e * a.scale / a.softcap : 0.f;
   p.cap_log2 = a.softcap * kLog2e;
+  p.cap_z = a.softcap > kCapNear ? a.scale / a.softcap : 0.f;
   p.page_div = make_fastdiv(a.page_size);
   p.group_div = make_fastdiv(p.group);
   return SMAQ_OK;
@@ -216,7 +217,7 @@ __device__ __forceinline__ void write_empty(const DecodeParamsX& d) {
 // Accumulator of one row over tokens [lo, hi) for a known maximum m, by one warp in 32 bits, into acc[0, D).
 // The hi + lo parts of a weight times an infinite value give NaN where their sum gives the infinity; a row that
 // comes out without a finite value is redone here.
-template <bool CAP>
+template <int CAP>
 __device__ __noinline__ void redo_row(const PagedParams& p, int b, int h, int lo, int hi, int last, float m, float* acc) {
   const smaq_paged_args& a = p.a;
   const int lane = threadIdx.x & 31, D = a.head_dim;
@@ -327,7 +328,7 @@ struct Cfg {
   static constexpr int SMEM = 4 * S::N * S::BYTES + 2 * 16 * LD * 4;
 };
 
-template <class DT, int D, bool CAP>
+template <class DT, int D, int CAP>
 __global__ void __launch_bounds__(PD_THREADS, Stages<2 * D>::CTAS) paged_decode_kernel(const __grid_constant__ DecodeParamsX d) {
   using T = typename DT::T;
   constexpr int LD = Cfg<D>::LD;
@@ -1002,8 +1003,11 @@ int launch_ring(K kern, int smem, const DecodeParamsX& d, cudaStream_t st) {
 }
 template <class DT, int D>
 int launch_mma(const DecodeParamsX& d, cudaStream_t st) {
-  return d.p.a.softcap > 0.f ? launch_ring(paged_decode_kernel<DT, D, true>, Cfg<D>::SMEM, d, st)
-                             : launch_ring(paged_decode_kernel<DT, D, false>, Cfg<D>::SMEM, d, st);
+  switch (cap_mode(d.p.a)) {
+    case CAP_NONE: return launch_ring(paged_decode_kernel<DT, D, CAP_NONE>, Cfg<D>::SMEM, d, st);
+    case CAP_LOW: return launch_ring(paged_decode_kernel<DT, D, CAP_LOW>, Cfg<D>::SMEM, d, st);
+    default: return launch_ring(paged_decode_kernel<DT, D, CAP_ANY>, Cfg<D>::SMEM, d, st);
+  }
 }
 template <class DT>
 int launch_mma_dim(const DecodeParamsX& d, cudaStream_t st) {

@@ -29,7 +29,7 @@ struct PmCfg {
   static constexpr int SMEM = Q + 2 * STAGE;
 };
 
-template <class DT, int D, bool CAP>
+template <class DT, int D, int CAP>
 __global__ void __launch_bounds__(PM_THREADS, 2) prefill_mma_kernel(const __grid_constant__ PagedParams p) {
   using T = typename DT::T;
   constexpr int N = PmCfg<D>::N, STAGE = PmCfg<D>::STAGE, CH = D / 8, NT = D / 8;
@@ -544,7 +544,7 @@ int64_t grid_tiles(const PagedParams& p, int size) {
 
 template <class DT, int D>
 int launch_mma(const PagedParams& p, cudaStream_t st) {
-  auto kern = p.a.softcap > 0.f ? prefill_mma_kernel<DT, D, true> : prefill_mma_kernel<DT, D, false>;
+  auto kern = p.a.softcap > 0.f ? prefill_mma_kernel<DT, D, CAP_ANY> : prefill_mma_kernel<DT, D, CAP_NONE>;
   if (const int rc = allow_smem(reinterpret_cast<const void*>(kern), PmCfg<D>::SMEM, "paged_prefill")) return rc;
   kern<<<dim3(unsigned(grid_tiles(p, PmCfg<D>::ROWS)), p.a.n_kv_heads), PM_THREADS, PmCfg<D>::SMEM, st>>>(p);
   return cuda_status(cudaGetLastError(), "paged_prefill");

@@ -89,6 +89,7 @@ struct PtBars {
 __device__ __forceinline__ void named_bar(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
 
 enum { PT_PLAIN = 0, PT_CAP = 1, PT_ANY = 2 };  // scores: scaled by a positive factor; capped; everything else
+// PT_CAP's tanh is that of caps up to kCapNear; the series beside it would be half of its softmax again.
 // Of every PT_OF pairs of exponentials so many come from the polynomial, the others from the special-function unit,
 // which alone would need as long as the products.  At 8192 tokens and 32/8 heads 0, 1, 2, 3 of 8 took 515, 514, 533,
 // 548 us; a capped score takes two exponentials and a reciprocal: (4, 2), (5, 2), (5, 3), (4, 1), (6, 3) of 8 for (tanh,
@@ -413,7 +414,7 @@ __global__ void __launch_bounds__(pt_threads(D), 1) prefill_tc_kernel(const __gr
           if constexpr (MODE == PT_CAP) {
             const uint64_t in2 = pair(p.cap_in, p.cap_in), out2 = pair(-2.0f * p.cap_log2, -2.0f * p.cap_log2), cap2 = pair(p.cap_log2, p.cap_log2);
 #pragma unroll
-            for (int c = 0; c < 32; c += 2 * PT_OF) {  // cap tanh, as score_log2
+            for (int c = 0; c < 32; c += 2 * PT_OF) {  // cap tanh, as score_log2 far from zero
               uint64_t y[PT_OF];
 #pragma unroll
               for (int e = 0; e < PT_OF; ++e) {
@@ -437,7 +438,7 @@ __global__ void __launch_bounds__(pt_threads(D), 1) prefill_tc_kernel(const __gr
           } else if constexpr (MODE == PT_ANY) {
             if (p.a.softcap > 0.f) {
 #pragma unroll
-              for (int c = 0; c < 32; ++c) x[c] = score_log2<true>(x[c], p);
+              for (int c = 0; c < 32; ++c) x[c] = score_log2<CAP_ANY>(x[c], p);
             } else {
 #pragma unroll
               for (int c = 0; c < 32; ++c) x[c] *= p.scale_log2;
@@ -700,7 +701,7 @@ int launch(const PagedParams& p, cudaStream_t st) {
   pt.box = a.page_size < PT_N ? a.page_size : PT_N;
   pt.tma = a.page_size >= 8 && (a.page_size < PT_N ? PT_N % a.page_size : a.page_size % PT_N) == 0 && a.n_pages > 0 && a.n_pages < (int64_t(1) << 31) &&
            a.n_kv_heads * a.c_stride_h < (int64_t(1) << 31) && encode(&pt.k, a, a.k_cache, pt.box) && encode(&pt.v, a, a.v_cache, pt.box);
-  auto kern = a.slopes || !(a.scale > 0.f) ? prefill_tc_kernel<DT, D, PT_ANY>
+  auto kern = a.slopes || !(a.scale > 0.f) || a.softcap > kCapNear ? prefill_tc_kernel<DT, D, PT_ANY>
               : a.softcap > 0.f            ? prefill_tc_kernel<DT, D, PT_CAP>
                                            : prefill_tc_kernel<DT, D, PT_PLAIN>;
   if (const int rc = allow_smem(reinterpret_cast<const void*>(kern), PtCfg<D>::SMEM, "paged_prefill")) return rc;

@@ -3,8 +3,8 @@
 import pytest
 import torch
 
-from paged_ref import paged_case
-from test_gpu_paged_attention import BF, HF, SF, decode, prefill, queries
+from paged_ref import UNIT, attention64, check_attention, paged_case
+from test_gpu_paged_attention import BF, HF, SF, check_lse, decode, prefill, queries, slopes_of
 
 pytestmark = pytest.mark.gpu
 
@@ -80,3 +80,33 @@ def test_decode_nan_reaches_those_who_see_it(cuda, dtype, D):
     got, gl = ops.paged_decode(q, k, v, table, n, return_lse=True)
     assert bool(torch.isnan(got[:, 4:]).all()) and bool(torch.isnan(gl[:, 4:]).all())
     assert torch.equal(got[:, :4], want[:, :4]) and torch.equal(gl[:, :4], lse[:, :4])
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, SF])
+@pytest.mark.parametrize("cap", [50.0, 65.0, 3000.0, 1e6])
+@pytest.mark.parametrize("D,slopes,scale", [(64, False, None), (128, False, 0.6), (128, True, None), (96, False, None), (256, False, -0.1)])
+def test_caps_far_above_the_scores(cuda, dtype, cap, D, slopes, scale):
+    """A score far below the cap is as exact as one without a cap: within 2^-24 of the sum of its products' sizes, D/8 + 16 times.
+    (A tanh of fixed absolute error would be off by that error times the cap.)"""
+    from smaq_b200 import ops
+    sl = slopes_of(8, cuda) if slopes else None
+    u = UNIT[dtype] if dtype != SF else 0.0
+
+    def check(got, lse, q, k, v, table, lens, cu, u_p):
+        ref, rl, capped = attention64(q, k, v, table, lens, cu, softcap=cap, slopes=sl, scale=scale)
+        plain = attention64(q, k, v, table, lens, cu, slopes=sl, scale=scale)[2]
+        mass, share = capped(1.0) - capped(0.0), plain(0.0) / (plain(1.0) - plain(0.0))   # of the capped weights; what scores without a cap allow
+        # capped at 50 and 65 the absolute error 2^-22 of tanh counts too, in the weight and in the sum, as long as it stays below the output's rounding
+        more = 2.0 ** -20 * cap if cap < 100 else 0.0
+        check_attention(got, ref, lambda x: (x + share + more) * mass, dtype, u_p)
+        check_lse(lse, rl)
+    lens = [700, 1, 99]
+    k, v, table = paged_case(cuda, lens, 2, D, 16, dtype)
+    q, n = queries(cuda, 3, 8, D, dtype), ints(lens, cuda)
+    check(*ops.paged_decode(q, k, v, table, n, softcap=cap, slopes=sl, scale=scale, return_lse=True), q, k, v, table, lens, [0, 1, 2, 3], u * u)
+    for lens, news in (([400, 130, 9], [300, 130, 1]), ([100, 64], [90, 64])):       # the second: a table of one block
+        k, v, table = paged_case(cuda, lens, 2, D, 16, dtype)
+        cu = [sum(news[:i]) for i in range(len(news) + 1)]
+        q = queries(cuda, cu[-1], 8, D, dtype)
+        got = ops.paged_prefill(q, k, v, table, ints(lens, cuda), ints(cu, cuda), softcap=cap, slopes=sl, scale=scale, return_lse=True)
+        check(*got, q, k, v, table, lens, cu, u)
