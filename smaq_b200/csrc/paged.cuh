@@ -59,6 +59,11 @@ __device__ __forceinline__ float score_log2(float qk, const PagedParams& p) {
   }
 }
 
+// Weights are 2^(x - m + kUp): in fp16, whose smallest step is 2^-24, up to 2^15, so that many tokens far below the largest
+// still count (at weights of at most 1, those below 2^-25 of it were zero, and 128K of them are 0.4% of an answer).
+template <class DT>
+constexpr float kUp = DT::code == SMAQ_F16 ? 15.0f : 0.0f;
+
 // Element offset of token j of the request whose table row is `table`, in the K and V caches; the page
 // number is clamped to the cache.
 __device__ __forceinline__ int64_t token_offset(const PagedParams& p, const int32_t* table, int j) {

@@ -16,8 +16,8 @@
 // 16-token stages (keys + values, cp.async, 96 KB a CTA and two CTAs an SM in flight), its own softmax
 // state and no block-wide barrier until the segment ends.  The page lookups of a stage are made one stage
 // before its copies.  Scores by m16n8k16 (rows = query heads of the group, zero rows above it); weights enter
-// the second product as hi + lo parts in the cache's type, which costs tensor time that is idle here and
-// keeps 16-bit rounding out of the weights.  Slots past the visible range are filled with zeros by the copy and
+// the second product as hi + lo parts in the cache's type (fp16: scaled by 2^15), which costs tensor time that is idle here
+// and keeps 16-bit rounding out of the weights.  Slots past the visible range are filled with zeros by the copy and
 // their scores replaced, so what they hold never matters.  64 requests of 1K to 64K tokens at 28/4 heads of 128:
 // 323 us, 6.3 TB/s; 4 of 128K at 64/8: 357 us, 6.0 TB/s (both of 6.45 for a plain copy).
 //
@@ -415,6 +415,8 @@ __global__ void __launch_bounds__(PD_THREADS, Stages<2 * D>::CTAS) paged_decode_
         mx0 = fmaxf(mx0, __shfl_xor_sync(~0u, mx0, w));
         mx1 = fmaxf(mx1, __shfl_xor_sync(~0u, mx1, w));
       }
+      mx0 -= kUp<DT>;  // m lies that much below the maximum from here on, in the slots too
+      mx1 -= kUp<DT>;
       if (__any_sync(~0u, mx0 > m0 || mx1 > m1)) {
         const float n0 = fmaxf(m0, mx0), n1 = fmaxf(m1, mx1);
         const float f0 = m0 == -INFINITY ? 0.f : ex2(m0 - n0), f1 = m1 == -INFINITY ? 0.f : ex2(m1 - n1);

@@ -140,6 +140,8 @@ __global__ void __launch_bounds__(PM_THREADS, 2) prefill_mma_kernel(const __grid
       mx0 = fmaxf(mx0, __shfl_xor_sync(~0u, mx0, w));
       mx1 = fmaxf(mx1, __shfl_xor_sync(~0u, mx1, w));
     }
+    mx0 -= kUp<DT>;
+    mx1 -= kUp<DT>;
     if (__any_sync(~0u, mx0 > m0 || mx1 > m1)) {
       const float n0 = fmaxf(m0, mx0), n1 = fmaxf(m1, mx1);
       const float g0 = m0 == -INFINITY ? 0.f : ex2(m0 - n0), g1 = m1 == -INFINITY ? 0.f : ex2(m1 - n1);

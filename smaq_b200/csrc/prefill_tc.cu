@@ -14,8 +14,8 @@
 //   warp 19          issues all products.
 // Tensor memory: S0 S1 (128 columns each), O0 O1 (head_dim each); P overwrites its S.  The product for the next S of a tile is
 // issued right behind the product that reads its P, and its completion also says that O is at rest: a softmax warp may
-// then rescale O, which it does only when a row's maximum grew by more than 2^8 (the reference maximum of a row
-// lags by at most that, so weights stay below 2^8 in either type).
+// then rescale O, which it does only when a row's maximum grew by more than 2^8, in fp16 2^3 (the reference of a row lags by
+// at most that, so weights stay below 2^8 in bf16 and 2^15 in fp16).
 // At head_dim 256 there is room for one tile (128 rows, half the softmax warps): S0 and S1 are then blocks of even and odd
 // number, the next block's scores are computed during this block's softmax, and O is waited for by itself.
 // Weights are rounded once, to the cache's type; the sums are of the unrounded ones.
@@ -51,7 +51,12 @@ __host__ __device__ constexpr int pt_tiles(int D) { return D == 256 ? 1 : 2; }
 __host__ __device__ constexpr int pt_rows(int D) { return 128 * pt_tiles(D); }
 __host__ __device__ constexpr int pt_threads(int D) { return 32 * (PT_TW * pt_tiles(D) + 4); }
 constexpr uint32_t PT_COLS = 512;
-constexpr float PT_LAG = 8.0f;            // log2
+// log2: how far a row's maximum may grow above its reference before O is rescaled.  In fp16 the weights have room for 2^15
+// (paged.cuh): the reference lies 2^12 below the maximum it was taken from, which leaves 2^3.
+template <class DT>
+constexpr float PT_LAG = DT::code == SMAQ_F16 ? 3.0f : 8.0f;
+template <class DT>
+constexpr float PT_UP = kUp<DT> > 0.f ? kUp<DT> - PT_LAG<DT> : 0.0f;
 
 template <int D>
 struct PtCfg {
@@ -394,7 +399,7 @@ __global__ void __launch_bounds__(pt_threads(D), 1) prefill_tc_kernel(const __gr
       const float slope = a.slopes && f < last ? a.slopes[h] * kLog2e : 0.f;
       const uint32_t lanes = uint32_t(32 * (warp & 3)) << 16;
       const uint32_t to = tmem + lanes + o_col + D * i + half * (D / PT_SPLIT);
-      float m = -INFINITY;  // reference maximum of the row, log2
+      float m = -INFINITY;  // reference of the row, log2
       for (int j = 0; j < n; ++j) {
         const int base = base_of(j) + half * C;
         const bool part = !seen_by_all(base - half * C);
@@ -474,8 +479,9 @@ __global__ void __launch_bounds__(pt_threads(D), 1) prefill_tc_kernel(const __gr
         named_bar(meet, 64);
         mx = fmaxf(mx, bars.row[j & 1][i][half ^ 1][row]);
         if (*reinterpret_cast<volatile int*>(&bars.fail[j & 1][i][warp & 3])) { failed = true; break; }
+        mx -= PT_UP<DT>;
         float factor = 1.f;
-        if (mx > m + PT_LAG || (j == 0 && mx > m)) {
+        if (mx > m + PT_LAG<DT> || (j == 0 && mx > m)) {
           factor = m == -INFINITY ? 0.f : ex2(m - mx);
           m = mx;
         }

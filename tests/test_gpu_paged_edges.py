@@ -110,3 +110,51 @@ def test_caps_far_above_the_scores(cuda, dtype, cap, D, slopes, scale):
         q = queries(cuda, cu[-1], 8, D, dtype)
         got = ops.paged_prefill(q, k, v, table, ints(lens, cuda), ints(cu, cuda), softcap=cap, slopes=sl, scale=scale, return_lse=True)
         check(*got, q, k, v, table, lens, cu, u)
+
+
+def one_score_above_the_others(cuda, L, D, dtype, gap, value):
+    """A cache whose token 0 scores `gap` (natural) above all others for a query along channel 0; its value is 0, theirs `value`."""
+    page = 16
+    pages = -(-L // page)
+    k = torch.zeros(pages, page, 1, D, device=cuda, dtype=dtype)
+    v = torch.full_like(k, value)
+    k[0, 0, 0, 0], v[0, 0] = 8.0, 0.0
+    q0 = gap * D ** 0.5 / 8.0
+    return k, v, torch.arange(pages, dtype=torch.int32, device=cuda)[None], q0
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("D", [64, 128, 256, 96])
+@pytest.mark.parametrize("gap", [9.0, 14.0, 18.5, 20.0])
+def test_small_weights_add_up(cuda, dtype, D, gap):
+    """Many tokens far below one that outweighs each of them: together they count, in either 16-bit type.
+
+    The weights relative to the largest are e^-gap, about 2^-13 to 2^-29.  Decode keeps them in two parts, each a multiple of 2^-24
+    2^-15 of the largest; prefill rounds them once, to a multiple of 2^-24 2^-12 of the largest or of one up to 2^3 below."""
+    from smaq_b200 import ops
+    L, value = 30000, 1000.0
+    k, v, table, q0 = one_score_above_the_others(cuda, L, D, dtype, gap, value)
+    q = torch.zeros(40, 2, D, device=cuda, dtype=dtype)
+    q[:, 0, 0], q[:, 1, 0] = q0, q0 / 2
+    n = ints([L], cuda)
+
+    def check(got, rows, tokens, u_p, grain):
+        x = q[rows].double()[..., 0] * k[0, 0, 0, 0].double() / D ** 0.5      # the score of token 0; the others' is 0
+        w = torch.exp(-x)
+        ref = (tokens - 1) * w / (1 + (tokens - 1) * w) * v[-1, 0, 0, 0].double()
+        # one rounding of the output, 32-bit scores and sums, the weights' own rounding and their grain
+        tol = (UNIT[dtype] + u_p + (D / 8 + 16) * 2.0 ** -24 * x.abs() + 2.0 ** -16) * ref + tokens * grain * value + 2.0 ** -25
+        over = (got.double() - ref[..., None]).abs() - tol[..., None]
+        assert float(over.max()) <= 0, (got.double()[0, :, 0].tolist(), ref[0].tolist(), tol[0].tolist())
+    u, half = UNIT[dtype], dtype == HF
+    check(ops.paged_decode(q[:1], k, v, table, n), slice(0, 1), L, u * u, 2.0 ** -39 if half else 0.0)
+    out = ops.paged_prefill(q, k, v, table, n, ints([0, 40], cuda))              # rows 0 .. 39 see L - 39 .. L tokens
+    for r in (0, 39):
+        check(out[r:r + 1], slice(r, r + 1), L - 39 + r, u, 2.0 ** -36 if half else 0.0)
+    many = torch.zeros(4000, 2, D, device=cuda, dtype=dtype) + q[:1]             # rows enough for walks of their own
+    out = ops.paged_prefill(many, k, v, table, n, ints([0, 4000], cuda))
+    for r in (0, 3999):
+        check(out[r:r + 1], slice(0, 1), L - 3999 + r, u, 2.0 ** -36 if half else 0.0)
+    out = ops.paged_prefill(q[:2], k, v, table[:, :8].contiguous(), ints([128], cuda), ints([0, 2], cuda))   # a table of one block
+    for r in (0, 1):
+        check(out[r:r + 1], slice(0, 1), 127 + r, u, 2.0 ** -36 if half else 0.0)
