@@ -73,10 +73,11 @@ __device__ __forceinline__ int64_t token_offset(const PagedParams& p, const int3
 }
 
 // Length of request b, within its table's width.
+constexpr int kLongest = 0x7FFFFF00;
 __device__ __forceinline__ int paged_len(const PagedParams& p, int b) {
   const int64_t room = int64_t(p.a.max_blocks) * p.a.page_size;
   const int L = max(__ldg(p.a.seq_lens + b), 0);
-  return int(min(min(int64_t(L), room), int64_t(0x7FFFFF00)));
+  return int(min(min(int64_t(L), room), int64_t(kLongest)));
 }
 
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }

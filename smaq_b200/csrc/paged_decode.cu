@@ -26,6 +26,8 @@
 // 12/4 heads of 64: 47 us, of which start and join are 12.
 // paged_simt_kernel (other head dims and alignments): 16 groups of eight lanes, one token a group, four query
 // rows a tile.
+#include <algorithm>
+
 #include "paged.cuh"
 
 namespace smaq {
@@ -52,6 +54,8 @@ int paged_check(const smaq_paged_args* args, bool prefill, PagedParams& p) {
   }
   p.a = a;
   if (a.n_pages == 0) p.a.max_blocks = 0;  // an empty cache: every request reads as empty
+  // a window that no request outgrows is none; positions minus it would leave 32 bits
+  if (a.window >= std::min(int64_t(a.max_blocks) * a.page_size, int64_t(kLongest))) p.a.window = 0;
   p.group = a.n_q_heads / a.n_kv_heads;
   p.scale_log2 = a.scale * kLog2e;
   p.cap_in = a.softcap > 0.f ? 2.0f * kLog2e * a.scale / a.softcap : 0.f;

@@ -158,3 +158,38 @@ def test_small_weights_add_up(cuda, dtype, D, gap):
     out = ops.paged_prefill(q[:2], k, v, table[:, :8].contiguous(), ints([128], cuda), ints([0, 2], cuda))   # a table of one block
     for r in (0, 1):
         check(out[r:r + 1], slice(0, 1), 127 + r, u, 2.0 ** -36 if half else 0.0)
+
+
+@pytest.mark.parametrize("dtype", [BF, SF])
+@pytest.mark.parametrize("D", [64, 128, 256, 96])
+@pytest.mark.parametrize("prefix", [None, [100, 0, 270]])
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 100, 400])
+def test_windows_wider_than_any_request(cuda, dtype, D, prefix, window):
+    """As without one, up to the widest that an int holds."""
+    from smaq_b200 import ops
+    lens, news = [400, 90, 301], [260, 90, 1]
+    k, v, table = paged_case(cuda, lens, 2, D, 16, dtype)
+    q, n, cu = queries(cuda, 351, 8, D, dtype), ints(lens, cuda), ints([0, 260, 350, 351], cuda)
+    pre = None if prefix is None else ints(prefix, cuda)
+    want, lse = ops.paged_prefill(q, k, v, table, n, cu, prefix_lens=pre, return_lse=True)
+    got, gl = ops.paged_prefill(q, k, v, table, n, cu, prefix_lens=pre, window=window, return_lse=True)
+    assert torch.equal(got, want) and torch.equal(gl, lse)
+    one = ops.paged_decode(q[:3], k, v, table, n)
+    assert torch.equal(one, ops.paged_decode(q[:3], k, v, table, n, window=window))
+
+
+@pytest.mark.parametrize("dtype", [BF, SF])
+@pytest.mark.parametrize("D", [64, 128, 256, 96])
+@pytest.mark.parametrize("width", [25, 5])     # tables of 400 and 80 tokens
+def test_more_rows_than_tokens_under_a_wide_window(cuda, dtype, D, width):
+    """Rows before a request's first token see nothing, and the others are not disturbed by their positions below zero."""
+    from smaq_b200 import ops
+    lens = [70, 33]
+    k, v, table = paged_case(cuda, [400, 90], 2, D, 16, dtype)
+    table = table[:, :width].contiguous()
+    q, n, cu = queries(cuda, 300, 8, D, dtype), ints(lens, cuda), ints([0, 200, 300], cuda)
+    want, lse = ops.paged_prefill(q, k, v, table, n, cu, return_lse=True)
+    assert not want[:130].any() and bool(want[130:200].any()) and not want[200:267].any()
+    for window in (2 ** 31 - 1, 2 ** 31 - 70):
+        got, gl = ops.paged_prefill(q, k, v, table, n, cu, window=window, return_lse=True)
+        assert torch.equal(got, want) and torch.equal(gl, lse)
