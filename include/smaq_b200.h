@@ -457,8 +457,8 @@ int smaq_norm_rope(const smaq_norm_rope_args* args, void* stream);
  * n_b + (t - cu_query[b]) with n_b = cu_query[b + 1] - cu_query[b]; it sees token j when
  *   j < prefix_lens[b], or j <= i and (window == 0 or j > i - window)      (0 <= j < seq_lens[b]).
  * Scores: x = scale q.k;  softcap > 0: x = softcap tanh(x / softcap);  slopes: x -= slopes[h] |i - j|.
- * Query head h reads KV head h / (n_q_heads / n_kv_heads).  A row that sees nothing, and rows past
- * the last request's, give zeros and lse -infinity.  Slots that no row sees are never used, whatever
+ * Query head h reads KV head h / (n_q_heads / n_kv_heads).  A row that sees nothing, and rows before
+ * the first request's and past the last one's, give zeros and lse -infinity.  Slots that no row sees are never used, whatever
  * they hold.  Page numbers are clamped to the cache and seq_lens to the table's width, so that no
  * read leaves the cache.  lse: natural log of the sum of exp(score), [rows, n_q_heads].
  *   smaq_paged_decode: one row per request (cu_query, prefix_lens unused), the cache split over the

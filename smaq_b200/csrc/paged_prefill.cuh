@@ -110,16 +110,18 @@ struct PrefillBlocks {
   __device__ __forceinline__ int base(int k, int N) const { return (k < head ? k : k + jump) * N; }
 };
 
-// Rows past the last request's: zeros for this block's share.
+// Rows before the first request's and past the last one's: zeros for this block's share.
 __device__ __forceinline__ void write_padding(const PagedParams& p, int kvh, int block, int blocks) {
   const smaq_paged_args& a = p.a;
-  const int64_t end = a.batch ? cu_at(p, a.batch) : 0;
-  for (int64_t t = end + block; t < a.n_rows; t += blocks)
+  const int64_t end = a.batch ? cu_at(p, a.batch) : 0, head = a.batch ? min(int64_t(cu_at(p, 0)), end) : 0;
+  for (int64_t r = block; r < head + a.n_rows - end; r += blocks) {
+    const int64_t t = r < head ? r : r - head + end;
     for (int i = threadIdx.x; i < p.group * a.head_dim; i += blockDim.x) {
       const int h = kvh * p.group + i / a.head_dim;
       store_elem(a.out, a.dtype, t * a.o_stride_t + h * a.o_stride_h + i % a.head_dim, 0.f);
       if (a.lse && i % a.head_dim == 0) a.lse[t * a.n_q_heads + h] = -INFINITY;
     }
+  }
 }
 
 // Whether one of eight 16-bit elements is an infinity or NaN.

@@ -785,7 +785,8 @@ def paged_prefill(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
     last ones of its ``seq_lens[b]``, already written): row ``i`` sees tokens up to its own, the last
     ``window`` of them if given, and the first ``prefix_lens[b]`` in any case.  Requests never see one
     another.  Other arguments as ``paged_decode`` (``workspace``: ``paged_prefill_workspace_bytes``
-    bytes, which are 0 for many rows); rows past ``cu_query[B]`` give zeros."""
+    bytes, which are 0 for many rows); rows before ``cu_query[0]`` and
+    past ``cu_query[B]`` give zeros."""
     if cu_query is None:
         raise ValueError("paged_prefill needs cu_query")
     return _paged("smaq_paged_prefill", q, k_cache, v_cache, block_table, seq_lens, cu_query, prefix_lens, scale,

@@ -193,3 +193,25 @@ def test_more_rows_than_tokens_under_a_wide_window(cuda, dtype, D, width):
     for window in (2 ** 31 - 1, 2 ** 31 - 70):
         got, gl = ops.paged_prefill(q, k, v, table, n, cu, window=window, return_lse=True)
         assert torch.equal(got, want) and torch.equal(gl, lse)
+
+
+@pytest.mark.parametrize("dtype", [BF, SF])
+@pytest.mark.parametrize("D", [64, 256, 96])
+@pytest.mark.parametrize("width,news,heads", [(20, [3, 5], 8), (20, [90, 100], 8), (5, [40, 33], 2)])
+def test_rows_before_the_first_requests(cuda, dtype, D, width, news, heads):
+    """cu_query may start behind the first row: rows of no request give zeros at either end."""
+    from smaq_b200 import ops
+    lens = [80, 70]
+    k, v, table = paged_case(cuda, [300, 70], 2, D, 16, dtype)
+    table, n, (a, b) = table[:, :width].contiguous(), ints(lens, cuda), news
+    q = queries(cuda, 19 + a + b + 6, heads, D, dtype)
+    want, lse = ops.paged_prefill(q[19:19 + a + b].contiguous(), k, v, table, n, ints([0, a, a + b], cuda), return_lse=True)
+    out = torch.full_like(q, 7.0)
+    got, gl = ops.paged_prefill(q, k, v, table, n, ints([19, 19 + a, 19 + a + b], cuda), out=out, return_lse=True)
+    mine = slice(19, 19 + a + b)
+    tol = 4 * UNIT[dtype] * float(want.float().abs().max()) if dtype != SF else 1e-5
+    assert float((got[mine].float() - want.float()).abs().max()) <= tol
+    none = torch.ones(q.shape[0], dtype=torch.bool, device=cuda)
+    none[mine] = False
+    assert not got[none].any() and bool((gl[none] == -float("inf")).all())
+    check_lse(gl[mine], lse.double())
