@@ -26,7 +26,7 @@ constexpr int kMost = 0x7FFFFFFF;
 // Sums of non-negative numbers, at most 2^31 - 1: lengths come from the device and may be anything.
 __device__ __forceinline__ int add(int a, int b) { return int(min(unsigned(a) + unsigned(b), unsigned(kMost))); }
 __device__ __forceinline__ int3 add3(int3 a, int3 b) { return make_int3(add(a.x, b.x), add(a.y, b.y), add(a.z, b.z)); }
-__device__ __forceinline__ int pages_of(int tokens, int s) { return tokens ? (tokens - 1) / s + 1 : 0; }
+__device__ __forceinline__ int pages_of(int tokens, int s) { return int((unsigned(tokens) + unsigned(s) - 1u) / unsigned(s)); }
 
 // Inclusive prefix sum over the block of one int3 a thread; `total` gets the block's sum.
 __device__ __forceinline__ int3 scan3(int3 v, int3* warp_sums, int3& total) {
