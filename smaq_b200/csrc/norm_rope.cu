@@ -9,7 +9,7 @@
 // rotation needs no exchange; only the sum of squares crosses lanes.  The cosines and sines of a token
 // are read once into registers and serve all heads that the lane group walks; it walks more heads a token
 // when there are enough tokens to fill the GPU, and loads a head ahead.  Values are copied by the same
-// walk.  Bound by HBM bytes for prompts, by latency for decode steps.
+// walk.  Bound by latency: of a launch for decode steps, of loads and dependent arithmetic for prompts.
 // norm_rope_staged_kernel: the same arithmetic for many tokens, rows staged in shared memory by bulk copies.
 // norm_rope_any_kernel: any head_dim and alignment, one warp a head, element by element.
 #include "common.cuh"
@@ -270,8 +270,9 @@ __global__ void __launch_bounds__(NR_THREADS, NR_CTAS) norm_rope_kernel(const __
 // ---------------------------------------------------------------- many tokens
 // The rows of `per` tokens at a time come to shared memory by bulk copies, two batches in turn, so that bytes in
 // flight do not cost registers; a lane group then takes head after head of one token from there (8192 tokens at 32/8 heads:
-// 49 us, 4.2 TB/s; an elementwise pass over as many bytes takes 33).  Values go from shared memory
-// to the cache by bulk copies too.  For heads that lie side by side in a token.
+// 45.5 us, 4.5 TB/s; an elementwise pass over as many bytes takes 33).  Values go from shared memory
+// to the cache by bulk copies too.  For heads that lie side by side in a token.  Sixteen warps an SM issue in 41% of the
+// cycles; the others go to the barrier between batches, to loads, and to results that the next instruction waits for.
 constexpr int NS_THREADS = 256, NS_CTAS = 2, NS_SMEM = 112 * 1024, NS_MOST = 16;
 constexpr int NS_ROUNDS = 3;
 
@@ -488,8 +489,9 @@ __global__ void __launch_bounds__(NR_THREADS) norm_rope_any_kernel(const __grid_
 
 // Tokens a batch of the staged kernel, 0 where it does not serve: heads side by side, batches of 32 KB or more, and tokens
 // enough for three rounds of batches on every CTA.  Against the other kernel, with the cache write: 32/8 heads of 128,
-// 16384 tokens 88 us / 101, 8192 (7 rounds) 49 / 54, 4096 (3.5) 31 / 30, 2000 (1.7) 16.5 / 15.8; 32/8 of 256, 4000
-// tokens 47 / 53; 12/4 of 64, 16000 tokens 30 / 33; 8/1 of 64, 16000 tokens in batches of 25 KB 26 / 21.
+// 16384 tokens 88 us / 101, 8192 (7 rounds) 49 / 54, 2000 (1.7) 16.5 / 15.8; 32/8 of 256, 4000 tokens 47 / 53; 12/4 of
+// 64, 16000 tokens 30 / 33; 8/1 of 64, 16000 tokens in batches of 25 KB 26 / 21.  Near the crossover, at 3.5 rounds, 4096
+// normed tokens of 32/8 heads of 128 with the cache write take 31 / 30, 4099 half-rotated ones without norm and cache 20.3 / 22.5.
 int staged_tokens(const smaq_norm_rope_args& a, int size, int groups) {
   const bool cache = a.k_cache != nullptr;
   if (a.q_stride_h != a.head_dim || a.k_stride_h != a.head_dim || (cache && a.v_stride_h != a.head_dim)) return 0;

@@ -19,11 +19,12 @@
 // the second product as hi + lo parts in the cache's type (fp16: scaled by 2^15), which costs tensor time that is idle here
 // and keeps 16-bit rounding out of the weights.  Slots past the visible range are filled with zeros by the copy and
 // their scores replaced, so what they hold never matters.  64 requests of 1K to 64K tokens at 28/4 heads of 128:
-// 323 us, 6.3 TB/s; 4 of 128K at 64/8: 357 us, 6.0 TB/s (both of 6.45 for a plain copy).
+// 315 to 320 us on the device in short runs, 6.4 TB/s; 4 of 128K at 64/8, capped: 337 us, 6.4 TB/s (a plain copy has 6.45).
+// In long runs, under the power cap, 346 to 358 and 387 to 393 us a call.
 //
 // paged_decode_f32_kernel (fp32, head_dim 64 / 128): the same rings; FMA throughout, since tf32 products in three parts
 // left 2e-6 in the scores (rounding inside the tensor cores' sums).  33 requests of 100 to 32K tokens, window 4096,
-// 12/4 heads of 64: 47 us, of which start and join are 12.
+// 12/4 heads of 64: 43 us, of which start and join are 12.
 // paged_simt_kernel (other head dims and alignments): 16 groups of eight lanes, one token a group, four query
 // rows a tile.
 #include <algorithm>
@@ -220,7 +221,8 @@ __device__ __forceinline__ void write_empty(const DecodeParamsX& d) {
 
 // Accumulator of one row over tokens [lo, hi) for a known maximum m, by one warp in 32 bits, into acc[0, D).
 // The hi + lo parts of a weight times an infinite value give NaN where their sum gives the infinity; a row that
-// comes out without a finite value is redone here.
+// comes out without a finite value is redone here, token by token: such values are rare, and a call that meets one is slow
+// (4 requests of 64K tokens at 32/8 heads, one infinity: 68 ms instead of 0.26).
 template <int CAP>
 __device__ __noinline__ void redo_row(const PagedParams& p, int b, int h, int lo, int hi, int last, float m, float* acc) {
   const smaq_paged_args& a = p.a;

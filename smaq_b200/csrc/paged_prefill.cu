@@ -538,7 +538,7 @@ __global__ void __launch_bounds__(PF_THREADS, DP <= 128 ? 2 : 1) prefill_fma_ker
   }
 }
 
-// At least one CTA a KV head, for the rows past the last request's.
+// At least one CTA a KV head, for the rows of no request.
 int64_t grid_tiles(const PagedParams& p, int size) {
   const int64_t n = most_tiles(p.a.n_rows, p.a.batch, p.group, size);
   return n > 0 ? n : 1;

@@ -135,7 +135,8 @@ __device__ __forceinline__ bool any_special(uint4 v) {
 // One row by one warp over its visible tokens alone, in 32 bits.  The matrix kernels multiply the values of
 // tokens that a row does not see by a weight of zero, which an infinity or NaN there turns into NaN.  They
 // look for such values in the blocks that some rows see in part, and only where there is one are that
-// tile's rows without a finite result redone here.
+// tile's rows without a finite result redone here.  That is slow: 8192 tokens at 32/8 heads, one infinity
+// at token 3203, whose tile has 256 rows to redo: 239 ms instead of 0.6.
 static __device__ __noinline__ void exact_row(const PagedParams& p, const PrefillTile& t, int kvh, int f) {
   const smaq_paged_args& a = p.a;
   const int lane = threadIdx.x & 31, D = a.head_dim;

@@ -18,10 +18,15 @@
 // at most that, so weights stay below 2^8 in bf16 and 2^15 in fp16).
 // At head_dim 256 there is room for one tile (128 rows, half the softmax warps): S0 and S1 are then blocks of even and odd
 // number, the next block's scores are computed during this block's softmax, and O is waited for by itself.
-// Weights are rounded once, to the cache's type; the sums are of the unrounded ones.
+// Weights are rounded once, to the cache's type, as the operand of the second product; the sums are of the unrounded ones.
+// Two parts a weight, as in decode, would double that product and leave no tensor memory for a second tile.  Against 64 bits
+// an answer is off by 0.0018 to 0.0020 of its size in bf16 and 0.0003 in fp16, of which the output's own rounding is 0.0016
+// and 0.0002.
 // Few rows with long walks: several CTAs share a tile's walk and prefill_join_kernel adds their parts in order.
-// Bound by both the products and the exponentials (2048 cycles a block each, of about 3300 in all): 8192 tokens at 32/8
-// heads of 128 in 514 us, 1070 TFLOP/s, 64% of what a library product reaches in short runs.
+// Products and exponentials take 2048 cycles a block each, side by side, of about 3300 in all; the rest is the way from a
+// block's scores to its weights, which two tiles do not hide.  8192 tokens at 32/8 heads of 128: 522 to 527 us on the device
+// in short runs (1050 TFLOP/s, 63% of what a library product reaches there), 586 to 605 a call in long ones (915 to 938),
+// under the power cap.
 // Every wait is bounded; one that runs out sets g_prefill_fault, and its rows come out as NaN.
 #include <cuda.h>
 #include <cudaTypedefs.h>

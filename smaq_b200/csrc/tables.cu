@@ -10,7 +10,7 @@
 // then serves its share of the tokens, four consecutive ones a thread: the request is found by
 // bisection in shared memory once, and a page is looked up once per page.  The token that opens a page
 // writes the table entry.  Bound by latency (lengths -> sums -> stack -> stores), not by bytes.
-// On the device 64 requests of one token take 7.9 us, 1001 requests with 285K tokens 11.1 us (0.6 us of bytes).
+// On the device 64 requests of one token take 8.2 us, 1001 requests with 285K tokens 11.4 us (0.6 us of bytes).
 #include "common.cuh"
 
 namespace smaq {

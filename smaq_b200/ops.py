@@ -769,7 +769,7 @@ def paged_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, 
     ``softcap``: scores become ``c * tanh(x / c)``; ``slopes [Hq]``: ``slope * distance`` is taken off.
     A request of length 0 gives zeros.  Returns ``out [B, Hq, D]``, with ``return_lse`` also the
     natural log-sum-exp ``[B, Hq]`` (fp32).  ``workspace``: ``paged_decode_workspace_bytes`` bytes (uint8),
-    allocated per call when None."""
+    allocated per call when None.  ``out`` must not overlap ``q``."""
     return _paged("smaq_paged_decode", q, k_cache, v_cache, block_table, seq_lens, None, None, scale, window, softcap,
                   slopes, out, return_lse, workspace)
 
