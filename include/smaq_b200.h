@@ -456,7 +456,7 @@ int smaq_norm_rope(const smaq_norm_rope_args* args, void* stream);
 /* Attention over the exact paged cache.  Row t of request b is its token i = seq_lens[b] -
  * n_b + (t - cu_query[b]) with n_b = cu_query[b + 1] - cu_query[b]; it sees token j when
  *   j < prefix_lens[b], or j <= i and (window == 0 or j > i - window)      (0 <= j < seq_lens[b]).
- * Scores: x = scale q.k;  softcap > 0: x = softcap tanh(x / softcap);  slopes: x -= slopes[h] |i - j|.
+ * Scores: x = scale q.k;  0 < softcap <= 1e30: x = softcap tanh(x / softcap);  slopes: x -= slopes[h] |i - j|.
  * Query head h reads KV head h / (n_q_heads / n_kv_heads).  A row that sees nothing, and rows before
  * the first request's and past the last one's, give zeros and lse -infinity.  Slots that no row sees are never used, whatever
  * they hold.  Page numbers are clamped to the cache and seq_lens to the table's width, so that no

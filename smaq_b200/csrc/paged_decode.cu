@@ -58,10 +58,11 @@ int paged_check(const smaq_paged_args* args, bool prefill, PagedParams& p) {
   // a window that no request outgrows is none; positions minus it would leave 32 bits
   if (a.window >= std::min(int64_t(a.max_blocks) * a.page_size, int64_t(kLongest))) p.a.window = 0;
   p.group = a.n_q_heads / a.n_kv_heads;
+  const float cap = p.a.softcap = a.softcap > 1e30f ? 0.f : a.softcap;  // tanh is the identity at every score: none
   p.scale_log2 = a.scale * kLog2e;
-  p.cap_in = a.softcap > 0.f ? 2.0f * kLog2e * a.scale / a.softcap : 0.f;
-  p.cap_log2 = a.softcap * kLog2e;
-  p.cap_z = a.softcap > kCapNear ? a.scale / a.softcap : 0.f;
+  p.cap_in = cap > 0.f ? 2.0f * kLog2e * a.scale / cap : 0.f;
+  p.cap_log2 = cap * kLog2e;
+  p.cap_z = cap > kCapNear ? a.scale / cap : 0.f;
   p.page_div = make_fastdiv(a.page_size);
   p.group_div = make_fastdiv(p.group);
   return SMAQ_OK;

@@ -751,7 +751,8 @@ def _paged(name, q, k_cache, v_cache, block_table, seq_lens, cu_query, prefix_le
         _lib.pack_paged(q.data_ptr(), qt, qh, k_cache.data_ptr(), v_cache.data_ptr(), cp, cs, ch,
                         block_table.data_ptr(), max(row, M), seq_lens.data_ptr(), _addr(cu_query), _addr(prefix_lens),
                         _addr(slopes), out.data_ptr(), ot, oh, _addr(lse), ws, ws_bytes, P, T, B, M, page_size, Hq, Hk,
-                        D, code, window or 0, 1.0 / math.sqrt(D) if scale is None else scale, softcap or 0.0), stream)
+                        D, code, min(window or 0, 2 ** 31 - 1), 1.0 / math.sqrt(D) if scale is None else scale,
+                        min(softcap or 0.0, 1e38)), stream)
     if st:
         _lib.check(st, name)
     return (out, lse) if return_lse else out

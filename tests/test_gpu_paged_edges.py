@@ -215,3 +215,20 @@ def test_rows_before_the_first_requests(cuda, dtype, D, width, news, heads):
     none[mine] = False
     assert not got[none].any() and bool((gl[none] == -float("inf")).all())
     check_lse(gl[mine], lse.double())
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, SF])
+@pytest.mark.parametrize("D", [64, 96])
+@pytest.mark.parametrize("kw", [dict(window=2 ** 31), dict(window=10 ** 18), dict(softcap=1e32), dict(softcap=1e37), dict(softcap=1e200),
+                                dict(softcap=float("inf")), dict(softcap=float("inf"), window=2 ** 63)])
+def test_limits_beyond_every_score_and_length(cuda, dtype, D, kw):
+    """A window or a cap too large for the C types is none."""
+    from smaq_b200 import ops
+    lens, news = [400, 90], [260, 90]
+    k, v, table = paged_case(cuda, lens, 2, D, 16, dtype)
+    q, n, cu, sl = queries(cuda, 350, 8, D, dtype), ints(lens, cuda), ints([0, 260, 350], cuda), slopes_of(8, cuda)
+    for slopes in (None, sl):
+        want, lse = ops.paged_prefill(q, k, v, table, n, cu, slopes=slopes, return_lse=True)
+        got, gl = ops.paged_prefill(q, k, v, table, n, cu, slopes=slopes, return_lse=True, **kw)
+        assert torch.equal(got, want) and torch.equal(gl, lse)
+        assert torch.equal(ops.paged_decode(q[:2], k, v, table, n, slopes=slopes), ops.paged_decode(q[:2], k, v, table, n, slopes=slopes, **kw))
