@@ -20,7 +20,7 @@
 // and keeps 16-bit rounding out of the weights.  Slots past the visible range are filled with zeros by the copy and
 // their scores replaced, so what they hold never matters.  64 requests of 1K to 64K tokens at 28/4 heads of 128:
 // 315 to 320 us on the device in short runs, 6.4 TB/s; 4 of 128K at 64/8, capped: 337 us, 6.4 TB/s (a plain copy has 6.45).
-// In long runs, under the power cap, 346 to 358 and 387 to 393 us a call.
+// In long runs, under the power cap, 334 to 358 and 363 to 393 us a call.
 //
 // paged_decode_f32_kernel (fp32, head_dim 64 / 128): the same rings; FMA throughout, since tf32 products in three parts
 // left 2e-6 in the scores (rounding inside the tensor cores' sums).  33 requests of 100 to 32K tokens, window 4096,
